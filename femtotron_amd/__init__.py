@@ -7,11 +7,11 @@ LlamaPartialModel/LlamaForTraining API) and wrap it with
 checkpoint_fn=femtotron_amd.fused_checkpoint)``.  Decoder-layer calls on a HIP
 device then run on the hand-written gfx950 kernels of ``libfemtohip.so``.
 """
-from .fused_checkpoint import (dispatch_counts, fused_checkpoint, last_fallback_reason,
+from .fused_checkpoint import (dispatch_counts, eight_bit_checkpoint, fused_checkpoint, last_fallback_reason,
                                reset_dispatch_counts)
 from .boundary_ops import fuse_boundary_ops
 from .fused_attention import fuse_attention
 from .weight_packing import pack_layer_weights
 
 __all__ = ["fused_checkpoint", "dispatch_counts", "reset_dispatch_counts", "last_fallback_reason",
-           "pack_layer_weights", "fuse_boundary_ops", "fuse_attention"]
+           "pack_layer_weights", "fuse_boundary_ops", "fuse_attention", "eight_bit_checkpoint"]

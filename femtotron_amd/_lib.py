@@ -1,4 +1,5 @@
-"""ctypes binding of ``libfemtohip.so`` (the C ABI declared in include/femtohip.h).
+"""ctypes binding of ``libfemtohip.so`` (the C ABI declared in include/femtohip.h
+and, for what stands around a checkpointed block, include/femtohip_blocks.h).
 
 The library is built in-tree by ``femtotron_amd.csrc.build`` (``__graft_entry__.build()``).
 There is no fallback: if the library is missing or does not load, ``lib()`` raises,
@@ -13,9 +14,13 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfemtohip.so"
 ABI_VERSION = 7
+BLOCKS_ABI_VERSION = 1
 
 FH_BF16 = 0
 FH_F32 = 1
+
+FH_INT8 = 0
+FH_E4M3 = 1
 
 FH_OK = 0
 
@@ -102,6 +107,18 @@ SIGNATURES: dict[str, tuple] = {
     "fh_adamw_step": (c_int, [c_int, _V, _V, c_int, _I64, FhAdamHyper, _F, _V, _V]),
 }
 
+# The same of include/femtohip_blocks.h.
+BLOCK_SIGNATURES: dict[str, tuple] = {
+    "fh_blocks_abi_version": (c_int, []),
+    "fh_pack8": (c_int, [c_int, c_int, _V, _V, _V, _I64, _I64, _V]),
+    "fh_unpack8": (c_int, [c_int, c_int, _V, _V, _V, _I64, _I64, _V]),
+    "fh_rmsnorm_fwd_pack8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, POINTER(c_float), _I64, _I64, _F, _V]),
+    "fh_rmsnorm_fwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, POINTER(c_float), _I64, _I64, _F, _V]),
+    "fh_add_rmsnorm_fwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, _V, POINTER(c_float), _I64, _I64, _F, _V]),
+    "fh_rmsnorm_bwd8_workspace_size": (c_size_t, [_I64, _I64]),
+    "fh_rmsnorm_bwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, POINTER(c_float), _V, _V, _V, _V, _I64, _I64, _F, _V]),
+}
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -129,7 +146,11 @@ def lib() -> ctypes.CDLL:
         got = handle.fh_abi_version()
         if got != ABI_VERSION:
             raise FemtoHipError(f"libfemtohip ABI {got} != expected {ABI_VERSION}: rebuild it")
-        for name, (restype, argtypes) in SIGNATURES.items():
+        blocks = getattr(handle, "fh_blocks_abi_version", None)
+        got = 0 if blocks is None else blocks()
+        if got != BLOCKS_ABI_VERSION:
+            raise FemtoHipError(f"libfemtohip blocks ABI {got} != expected {BLOCKS_ABI_VERSION}: rebuild it")
+        for name, (restype, argtypes) in (SIGNATURES | BLOCK_SIGNATURES).items():
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes

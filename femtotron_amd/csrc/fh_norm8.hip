@@ -1,0 +1,218 @@
+// Activations kept in 8 bits (fh_pack8.hpp): pack and unpack, and the RMSNorm
+// kernels of fh_norm.hpp that pack what they read or read what was packed.
+//
+// All are HBM-bound streams.  Keeping x costs the forward's norm 1.03 bytes an
+// element more to write and no pass of its own; the backward's norms read 1.03
+// bytes where they read 2 (bf16), and the 16-bit tensor is never laid out.
+#include "femtohip_blocks.h"
+#include "fh_norm.hpp"
+
+namespace fh {
+namespace {
+
+// One thread = 8 elements.  Rows are counted in blocks of 32 (four threads), so
+// that a quad of lanes holds one block also where a row ends inside it: thread
+// -> (row, chunk of 8) over ceil(cols / 32) * 4 chunks a row.
+__device__ __forceinline__ void row_chunk(uint32_t idx, int cpr, const FastDiv& fd, int64_t& row, int& c) {
+  const uint32_t q = fd.div(idx);
+  row = q;
+  c = static_cast<int>(idx - q * static_cast<uint32_t>(cpr)) * 8;
+}
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, uint8_t* __restrict__ codes,
+                                               uint8_t* __restrict__ exps, int64_t rows, int cols, int cpr,
+                                               FastDiv fd) {
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  int64_t row;
+  int c;
+  row_chunk(idx, cpr, fd, row, c);
+  const bool in = row < rows && c < cols;
+  float v[8] = {};
+  if (in) Elem<T>::unpack(Elem<T>::ldraw_stream(x + row * cols + c), v);
+  pack8_store<FMT>(v, codes, exps, row, in ? cols : 0, c);
+}
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void k_unpack8(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
+                                                 T* __restrict__ x, int64_t rows, int cols, int cpr, FastDiv fd) {
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  int64_t row;
+  int c;
+  row_chunk(idx, cpr, fd, row, c);
+  if (row >= rows || c >= cols) return;
+  float v[8];
+  unpack8<FMT>(load8_codes(codes, exps, row, cols, c), v);
+  Elem<T>::store8(x + row * cols + c, v);
+}
+
+int check_fmt(fh_dtype dt, fh_fmt8 fmt, const char* what) {
+  if (dt != FH_BF16 && dt != FH_F32) return fail(FH_ERR_INVALID, std::string(what) + ": dtype must be FH_BF16 or FH_F32");
+  if (fmt != FH_INT8 && fmt != FH_E4M3) return fail(FH_ERR_INVALID, std::string(what) + ": format must be FH_INT8 or FH_E4M3");
+  return FH_OK;
+}
+
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+// A launch has fewer than 2^32 threads, and the forward takes a wave a row.
+int check_rows(fh_dtype dt, int64_t rows, int64_t cols) {
+  if (int e = validate_rows(dt, rows, cols)) return e;
+  FH_REQUIRE(rows < (int64_t(1) << 26), "rmsnorm: rows of a packed call must be < 2^26");
+  return FH_OK;
+}
+
+// f(element type tag, format) for a checked dtype and format.
+template <typename F>
+void with_types(fh_dtype dt, fh_fmt8 fmt, F&& f) {
+  auto go = [&](auto tag) {
+    if (fmt == FH_INT8) f(tag, std::integral_constant<int, kFmtInt8>{});
+    else f(tag, std::integral_constant<int, kFmtE4M3>{});
+  };
+  if (dt == FH_BF16) go(uint16_t{});
+  else go(float{});
+}
+
+// Grid of a pack or unpack: FH_ERR_INVALID where it would pass the largest.
+int stream_grid(int64_t rows, int64_t cols, const char* what, int64_t& threads) {
+  if (rows < 0 || cols <= 0 || cols % 8 || cols > (int64_t(1) << 30))
+    return fail(FH_ERR_INVALID, std::string(what) + ": rows must be >= 0 and cols a positive multiple of 8 (<= 2^30)");
+  const int64_t cpr = blocks8(cols) * 4;
+  // a launch has fewer than 2^32 threads
+  if (rows > ((int64_t(1) << 32) - 256) / cpr)
+    return fail(FH_ERR_INVALID, std::string(what) + ": too many elements for one call (2^35 or more)");
+  threads = rows * cpr;
+  return FH_OK;
+}
+
+}  // namespace
+}  // namespace fh
+
+using namespace fh;
+
+extern "C" int fh_blocks_abi_version(void) { return FH_BLOCKS_ABI_VERSION; }
+
+extern "C" int fh_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, void* codes, uint8_t* exps, int64_t rows, int64_t cols,
+                        hipStream_t stream) {
+  if (int e = check_fmt(dt, fmt, "pack8")) return e;
+  int64_t threads = 0;
+  if (int e = stream_grid(rows, cols, "pack8", threads)) return e;
+  if (rows == 0) return FH_OK;
+  FH_REQUIRE(x && codes && exps, "pack8: null pointer");
+  FH_REQUIRE(aligned16(x) && aligned8(codes), "pack8: x must be 16-byte and codes 8-byte aligned");
+  const int cpr = static_cast<int>(blocks8(cols) * 4);
+  const FastDiv fd(static_cast<uint32_t>(cpr));
+  with_types(dt, fmt, [&](auto tag, auto f) {
+    using T = decltype(tag);
+    hipLaunchKernelGGL((k_pack8<T, f()>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
+                       stream, static_cast<const T*>(x), static_cast<uint8_t*>(codes), exps, rows,
+                       static_cast<int>(cols), cpr, fd);
+  });
+  return check_launch("fh_pack8");
+}
+
+extern "C" int fh_unpack8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps, void* x, int64_t rows,
+                          int64_t cols, hipStream_t stream) {
+  if (int e = check_fmt(dt, fmt, "unpack8")) return e;
+  int64_t threads = 0;
+  if (int e = stream_grid(rows, cols, "unpack8", threads)) return e;
+  if (rows == 0) return FH_OK;
+  FH_REQUIRE(x && codes && exps, "unpack8: null pointer");
+  FH_REQUIRE(aligned16(x) && aligned8(codes), "unpack8: x must be 16-byte and codes 8-byte aligned");
+  const int cpr = static_cast<int>(blocks8(cols) * 4);
+  const FastDiv fd(static_cast<uint32_t>(cpr));
+  with_types(dt, fmt, [&](auto tag, auto f) {
+    using T = decltype(tag);
+    hipLaunchKernelGGL((k_unpack8<T, f()>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
+                       stream, static_cast<const uint8_t*>(codes), exps, static_cast<T*>(x), rows,
+                       static_cast<int>(cols), cpr, fd);
+  });
+  return check_launch("fh_unpack8");
+}
+
+extern "C" int fh_rmsnorm_fwd_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, const void* w, void* y, void* codes,
+                                    uint8_t* exps, float* rstd, int64_t rows, int64_t cols, float eps,
+                                    hipStream_t stream) {
+  if (int e = check_fmt(dt, fmt, "rmsnorm_fwd_pack8")) return e;
+  if (int e = check_rows(dt, rows, cols)) return e;
+  if (rows == 0) return FH_OK;
+  FH_REQUIRE(x && w && y && codes && exps, "rmsnorm_fwd_pack8: null pointer");
+  FH_REQUIRE(aligned16(x) && aligned16(w) && aligned16(y) && aligned8(codes),
+             "rmsnorm_fwd_pack8: pointers must be 16-byte aligned (codes 8-byte)");
+  const int c = static_cast<int>(cols);
+  with_types(dt, fmt, [&](auto tag, auto f) {
+    using T = decltype(tag);
+    dispatch_nv(c, [&](auto nv) {
+      launch_fwd<T, RowsT<T>, f(), nv()>(x, nullptr, w, nullptr, y, rstd, codes, exps, rows, c, eps, stream);
+      return 0;
+    });
+  });
+  return check_launch("fh_rmsnorm_fwd_pack8");
+}
+
+extern "C" int fh_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps, const void* w, void* y,
+                               float* rstd, int64_t rows, int64_t cols, float eps, hipStream_t stream) {
+  if (int e = check_fmt(dt, fmt, "rmsnorm_fwd8")) return e;
+  if (int e = check_rows(dt, rows, cols)) return e;
+  if (rows == 0) return FH_OK;
+  FH_REQUIRE(codes && exps && w && y, "rmsnorm_fwd8: null pointer");
+  FH_REQUIRE(aligned8(codes) && aligned16(w) && aligned16(y),
+             "rmsnorm_fwd8: pointers must be 16-byte aligned (codes 8-byte)");
+  const int c = static_cast<int>(cols);
+  with_types(dt, fmt, [&](auto tag, auto f) {
+    using T = decltype(tag);
+    dispatch_nv(c, [&](auto nv) {
+      launch_fwd<T, Rows8<f()>, kNoPack, nv()>(nullptr, nullptr, w, nullptr, y, rstd, codes, exps, rows, c, eps, stream);
+      return 0;
+    });
+  });
+  return check_launch("fh_rmsnorm_fwd8");
+}
+
+extern "C" int fh_add_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps, const void* a,
+                                   const void* w, void* h, void* y, float* rstd, int64_t rows, int64_t cols, float eps,
+                                   hipStream_t stream) {
+  if (int e = check_fmt(dt, fmt, "add_rmsnorm_fwd8")) return e;
+  if (int e = check_rows(dt, rows, cols)) return e;
+  if (rows == 0) return FH_OK;
+  FH_REQUIRE(codes && exps && a && w && h && y, "add_rmsnorm_fwd8: null pointer");
+  FH_REQUIRE(aligned8(codes) && aligned16(a) && aligned16(w) && aligned16(h) && aligned16(y),
+             "add_rmsnorm_fwd8: pointers must be 16-byte aligned (codes 8-byte)");
+  FH_REQUIRE(h != a, "add_rmsnorm_fwd8: h must not alias a");
+  const int c = static_cast<int>(cols);
+  with_types(dt, fmt, [&](auto tag, auto f) {
+    using T = decltype(tag);
+    dispatch_nv(c, [&](auto nv) {
+      launch_fwd<T, Rows8<f()>, kNoPack, nv()>(nullptr, a, w, h, y, rstd, codes, exps, rows, c, eps, stream);
+      return 0;
+    });
+  });
+  return check_launch("fh_add_rmsnorm_fwd8");
+}
+
+extern "C" size_t fh_rmsnorm_bwd8_workspace_size(int64_t rows, int64_t cols) {
+  return fh_rmsnorm_bwd_workspace_size(rows, cols);  // the same partial rows
+}
+
+extern "C" int fh_rmsnorm_bwd8(fh_dtype dt, fh_fmt8 fmt, const void* dy, const void* codes, const uint8_t* exps,
+                               const void* w, const float* rstd, const void* dres, void* dx, void* dw, void* workspace,
+                               int64_t rows, int64_t cols, float eps, hipStream_t stream) {
+  if (int e = check_fmt(dt, fmt, "rmsnorm_bwd8")) return e;
+  if (int e = check_rows(dt, rows, cols)) return e;
+  FH_REQUIRE(w && dw, "rmsnorm_bwd8: null pointer");
+  if (rows == 0)  // the weight gradient alone, zeros
+    return fh_rmsnorm_bwd(dt, nullptr, nullptr, w, nullptr, nullptr, nullptr, dw, nullptr, 0, cols, eps, stream);
+  FH_REQUIRE(dy && codes && exps && dx && workspace, "rmsnorm_bwd8: null pointer");
+  FH_REQUIRE(aligned16(dy) && aligned8(codes) && aligned16(w) && aligned16(dx) &&
+                 (dres == nullptr || aligned16(dres)) && aligned16(workspace),
+             "rmsnorm_bwd8: pointers (workspace included) must be 16-byte aligned (codes 8-byte)");
+  const int c = static_cast<int>(cols);
+  float* part = static_cast<float*>(workspace);
+  with_types(dt, fmt, [&](auto tag, auto f) {
+    using T = decltype(tag);
+    dispatch_nv(c, [&](auto nv) {
+      launch_bwd<T, Rows8<f()>, nv()>(dy, codes, exps, w, rstd, dres, dx, dw, part, rows, c, eps, stream);
+      return 0;
+    });
+  });
+  return check_launch("fh_rmsnorm_bwd8");
+}

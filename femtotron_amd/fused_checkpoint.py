@@ -15,6 +15,9 @@ all on the femtohip kernels.  Any other call is handed to
 ``torch.utils.checkpoint.checkpoint`` with the same arguments, i.e. it behaves
 exactly as the reference wrapper.
 
+``eight_bit_checkpoint(fmt)`` is such a ``checkpoint_fn`` whose fused calls keep
+their input in 8 bits (packed_checkpoint.py).
+
 On a HIP device the fused path never degrades silently: if ``libfemtohip.so`` is
 missing the call raises.
 """
@@ -26,9 +29,10 @@ from typing import Any
 import torch
 from torch.utils.checkpoint import checkpoint as _torch_checkpoint
 
-from . import _lib
+from . import _lib, ops
 from .fused_layer import FusedDecoderLayerFunction, LayerShape
 from .fused_parts import FusedMLPFunction, FusedRMSNormFunction
+from .packed_checkpoint import PackedDecoderLayerFunction, PackedMLPFunction, PackedRMSNormFunction
 
 _KNOWN_KWARGS = {"attention_mask", "position_embeddings", "position_ids", "past_key_values",
                  "use_cache", "cache_position"}
@@ -275,6 +279,32 @@ def fused_checkpoint(function, *args, use_reentrant: bool | None = None,
     only to format CheckpointError messages); ``preserve_rng_state`` is moot there
     because the fused layer draws no random numbers.  As in torch, reentrant mode
     together with ``debug`` raises ValueError (torch/utils/checkpoint.py:499-504)."""
+    return _checkpoint(None, function, args, kwargs, use_reentrant, preserve_rng_state, debug)
+
+
+_PACKED = {FusedDecoderLayerFunction: PackedDecoderLayerFunction, FusedMLPFunction: PackedMLPFunction,
+           FusedRMSNormFunction: PackedRMSNormFunction}
+
+
+def eight_bit_checkpoint(fmt: str = "int8"):
+    """A ``checkpoint_fn`` like ``fused_checkpoint`` that keeps the input of a fused
+    call in 8 bits from the forward to the backward: blocks of 32 elements with
+    one power-of-two exponent and codes in "int8" (the finer steps) or "e4m3"
+    (small elements beside a large one keep theirs), 8.25 bits an element.
+    Outputs are those of ``fused_checkpoint``; gradients are taken at the kept
+    value.  Calls that are not fused keep their input as it is."""
+    if fmt not in ops.FORMATS8:
+        raise ValueError(f"8-bit format must be one of {ops.FORMATS8}, got {fmt!r}")
+
+    def checkpoint_fn(function, *args, use_reentrant: bool | None = None,
+                      preserve_rng_state: bool = True, debug: bool = False, **kwargs):
+        return _checkpoint(fmt, function, args, kwargs, use_reentrant, preserve_rng_state, debug)
+
+    return checkpoint_fn
+
+
+def _checkpoint(fmt: str | None, function, args: tuple, kwargs: dict, use_reentrant, preserve_rng_state, debug):
+    """One checkpointed call; fmt: the 8-bit format its input is kept in, or None."""
     if use_reentrant and debug:
         raise ValueError("debug=True is only supported with use_reentrant=False")
     torch_only = {k: kwargs.pop(k) for k in ("context_fn", "determinism_check", "early_stop")
@@ -289,4 +319,6 @@ def fused_checkpoint(function, *args, use_reentrant: bool | None = None,
     _lib.lib()  # raises if the HIP library is not built: no silent fallback on GPU
     fn, fn_args = plan
     _bump("fused")
+    if fmt is not None and torch.is_grad_enabled():
+        return _PACKED[fn].apply(fmt, *fn_args)
     return fn.apply(*fn_args)

@@ -115,22 +115,28 @@ class _Acts:
     __slots__ = ("y1", "rstd1", "qkv", "o", "lse", "h", "rstd2", "z", "gu")
 
 
-def layer_forward(x2: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, shp: LayerShape,
-                  batch: int, seq: int, w: tuple, *, keep: bool):
-    """Run the layer on x2 [T, H].  keep=False returns the output [T, H];
+def layer_forward(x2: torch.Tensor | ops.Packed8, cos: torch.Tensor, sin: torch.Tensor, shp: LayerShape,
+                  batch: int, seq: int, w: tuple, *, keep: bool, pack: str | None = None):
+    """Run the layer on x2 [T, H] (kept in 8 bits or not).  keep=False returns the
+    output [T, H], and with `pack`, an 8-bit format, x2 packed beside it;
     keep=True (recompute) stops after the gate/up projection and returns _Acts
     (the backward's SwiGLU pass writes the product p itself)."""
     wq, wk, wv, wo, wg, wu, wd, w1, w2 = w
-    T, H = x2.shape
-    dev = x2.device
+    packed_in = isinstance(x2, ops.Packed8)
+    T, dev = (x2.codes if packed_in else x2).shape[0], w1.device
     acts = _Acts() if keep else None
     rstd1 = torch.empty(T, dtype=torch.float32, device=dev) if keep else None
-    y1 = ops.rmsnorm_fwd(x2, w1, shp.eps1, rstd=rstd1)
+    if packed_in:
+        y1 = ops.rmsnorm_fwd8(x2, w1, shp.eps1, rstd=rstd1)
+    elif pack is not None:
+        y1, kept = ops.rmsnorm_fwd_pack8(x2, w1, shp.eps1, pack, rstd=rstd1)
+    else:
+        y1 = ops.rmsnorm_fwd(x2, w1, shp.eps1, rstd=rstd1)
 
     qkv, o, lse = qkv_attention(y1, _cat_rows(wq, wk, wv), batch, seq, shp, cos, sin, keep=keep)
     a = linear(o, wo)
     rstd2 = torch.empty(T, dtype=torch.float32, device=dev) if keep else None
-    h, z = ops.add_rmsnorm_fwd(x2, a, w2, shp.eps2, rstd=rstd2)
+    h, z = (ops.add_rmsnorm_fwd8 if packed_in else ops.add_rmsnorm_fwd)(x2, a, w2, shp.eps2, rstd=rstd2)
     del a
     gu = linear(z, _cat_rows(wg, wu))
     F_ = shp.ffn
@@ -140,7 +146,8 @@ def layer_forward(x2: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, shp: L
         return acts
     p = ops.swiglu_fwd(gu[:, :F_], gu[:, F_:])
     del gu, qkv, o, y1, z
-    return linear_residual(p, wd, h)
+    out = linear_residual(p, wd, h)
+    return out if pack is None else (out, kept)
 
 
 _side_streams: dict[int, torch.cuda.Stream] = {}
@@ -276,7 +283,7 @@ def split_rows(dw: torch.Tensor | None, *rows: int) -> tuple:
     return tuple(out)
 
 
-def layer_backward(dout2: torch.Tensor, x2: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+def layer_backward(dout2: torch.Tensor, x2: torch.Tensor | ops.Packed8, cos: torch.Tensor, sin: torch.Tensor,
                    shp: LayerShape, batch: int, seq: int, w: tuple, acts: _Acts):
     """dx and the 9 weight gradients; a weight gradient accumulated into the
     parameter's existing .grad inside its GEMM (grad_target) comes back as None."""
@@ -318,7 +325,8 @@ def layer_backward(dout2: torch.Tensor, x2: torch.Tensor, cos: torch.Tensor, sin
     dy1 = linear_dgrad(dqkv, _cat_rows(wq, wk, wv))
     del dqkv
     acts.y1 = None
-    dx, dw1 = ops.rmsnorm_bwd(dy1, x2, w1, shp.eps1, rstd=acts.rstd1, dres=dh)
+    norm_bwd = ops.rmsnorm_bwd8 if isinstance(x2, ops.Packed8) else ops.rmsnorm_bwd
+    dx, dw1 = norm_bwd(dy1, x2, w1, shp.eps1, rstd=acts.rstd1, dres=dh)
     wg_stream.join()
     dwq, dwk, dwv = split_rows(dwqkv, shp.hq, shp.hkv, shp.hkv)
     dwg, dwu = split_rows(dwgu, F_, F_)

@@ -8,6 +8,7 @@ caching allocator); the library itself never allocates device memory.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -54,6 +55,16 @@ def _stream(t: torch.Tensor) -> int:
     """The current stream of t's device (the raw handle: building a
     torch.cuda.Stream object costs more than the launch's other host work)."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Calls an entry point on the current stream of t's device, with that device
+    the current one (the default stream's handle is 0 on every device)."""
+    if torch._C._cuda_getDevice() == t.device.index:
+        _lib.call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, _stream(t))
 
 
 def _ptr(t: torch.Tensor | None):
@@ -129,6 +140,137 @@ def rmsnorm_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: float, 
     ws = torch.empty(max(ws_bytes, 4) // 4, dtype=torch.float32, device=x.device)
     _lib.call("fh_rmsnorm_bwd", _dtype_code(x), _ptr(dy), _ptr(x), _ptr(w), _fptr(rstd),
               _ptr(dres), _ptr(dx), _ptr(dw), _ptr(ws), rows, cols, float(eps), _stream(x))
+    return dx, dw
+
+
+# ------------------------------------------------------- activations in 8 bits
+class Packed8(NamedTuple):
+    """An activation kept in 8 bits (include/femtohip_blocks.h): codes, int8 or
+    float8_e4m3fn of the activation's shape, and the exponent bytes, uint8 [...,
+    ceil(cols / 32)], of its blocks of 32 elements."""
+    codes: torch.Tensor
+    exps: torch.Tensor
+
+
+_FMT8 = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+FORMATS8 = tuple(_FMT8)
+_FMT8_CODE = {torch.int8: _lib.FH_INT8, torch.float8_e4m3fn: _lib.FH_E4M3}
+
+
+def _empty8(x: torch.Tensor, fmt: str) -> Packed8:
+    if fmt not in _FMT8:
+        raise ValueError(f"8-bit format must be one of {FORMATS8}, got {fmt!r}")
+    if x.dim() == 0 or x.size(-1) % 8:
+        raise ValueError(f"an activation's last dim must be a multiple of 8 to be packed, got shape {tuple(x.shape)}")
+    return Packed8(torch.empty(x.shape, dtype=_FMT8[fmt], device=x.device),
+                   torch.empty(*x.shape[:-1], -(-x.size(-1) // 32), dtype=torch.uint8, device=x.device))
+
+
+def _packed(name: str, p: Packed8) -> tuple[int, int, int]:
+    """(format code, rows, cols) of a packed activation, checked."""
+    codes, exps = p
+    _require_gpu(codes, exps)
+    if codes.dtype not in _FMT8_CODE or exps.dtype != torch.uint8:
+        raise TypeError(f"{name}: codes must be int8 or float8_e4m3fn and exps uint8, got {codes.dtype}, {exps.dtype}")
+    if codes.dim() == 0 or not codes.is_contiguous() or not exps.is_contiguous():
+        raise ValueError(f"{name}: codes and exps must be contiguous")
+    cols = codes.size(-1)
+    if exps.shape != (*codes.shape[:-1], -(-cols // 32)):
+        raise ValueError(f"{name}: exps {tuple(exps.shape)} are not those of codes {tuple(codes.shape)}")
+    return _FMT8_CODE[codes.dtype], codes.numel() // max(cols, 1), cols
+
+
+def pack8(x: torch.Tensor, fmt: str = "int8") -> Packed8:
+    """A contiguous x in 8.25 bits an element: blocks of 32 along the last dim with one
+    power-of-two exponent, codes "int8" or "e4m3" (fh_pack8)."""
+    _require_gpu(x)
+    dt = _dtype_code(x)
+    if not x.is_contiguous():
+        raise ValueError("pack8: x must be contiguous")
+    p = _empty8(x, fmt)
+    cols = x.size(-1)
+    if x.numel():
+        _launch("fh_pack8", x, dt, _FMT8_CODE[p.codes.dtype], _ptr(x), _ptr(p.codes), _ptr(p.exps), x.numel() // cols,
+                  cols)
+    return p
+
+
+def unpack8(p: Packed8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values a packed activation stands for; bf16 and fp32 hold them exactly (fh_unpack8)."""
+    fmt, rows, cols = _packed("unpack8", p)
+    x = torch.empty(p.codes.shape, dtype=dtype, device=p.codes.device)
+    dt = _dtype_code(x)
+    if x.numel():
+        _launch("fh_unpack8", x, dt, fmt, _ptr(p.codes), _ptr(p.exps), _ptr(x), rows, cols)
+    return x
+
+
+def _norm8_args(name: str, w: torch.Tensor, cols: int, rows: int, rstd: torch.Tensor | None) -> None:
+    if not w.is_contiguous() or w.numel() != cols:
+        raise ValueError(f"{name}: w must be contiguous, of the last dim's size")
+    if rstd is not None and (rstd.numel() != rows or not rstd.is_contiguous()):
+        raise ValueError(f"{name}: rstd must be contiguous with one entry per row")
+
+
+def rmsnorm_fwd_pack8(x: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "int8", *,
+                      rstd: torch.Tensor | None = None) -> tuple[torch.Tensor, Packed8]:
+    """(rmsnorm_fwd(x, w, eps), pack8(x, fmt)) in one pass over x."""
+    _require_gpu(x, w, rstd)
+    _same_dtype(x, w)
+    dt = _dtype_code(x)
+    if not x.is_contiguous():
+        raise ValueError("rmsnorm_fwd_pack8: x must be contiguous")
+    p = _empty8(x, fmt)
+    cols = x.size(-1)
+    rows = x.numel() // max(cols, 1)
+    _norm8_args("rmsnorm_fwd_pack8", w, cols, rows, rstd)
+    y = torch.empty_like(x)
+    _launch("fh_rmsnorm_fwd_pack8", x, dt, _FMT8_CODE[p.codes.dtype], _ptr(x), _ptr(w), _ptr(y), _ptr(p.codes),
+              _ptr(p.exps), _fptr(rstd), rows, cols, float(eps))
+    return y, p
+
+
+def rmsnorm_fwd8(p: Packed8, w: torch.Tensor, eps: float, *, rstd: torch.Tensor | None = None) -> torch.Tensor:
+    """rmsnorm_fwd of the packed x, in w's dtype: the bits of rmsnorm_fwd(unpack8(p), w, eps)."""
+    fmt, rows, cols = _packed("rmsnorm_fwd8", p)
+    _require_gpu(p.codes, w, rstd)
+    _norm8_args("rmsnorm_fwd8", w, cols, rows, rstd)
+    y = torch.empty(p.codes.shape, dtype=w.dtype, device=w.device)
+    _launch("fh_rmsnorm_fwd8", w, _dtype_code(w), fmt, _ptr(p.codes), _ptr(p.exps), _ptr(w), _ptr(y), _fptr(rstd), rows,
+              cols, float(eps))
+    return y
+
+
+def add_rmsnorm_fwd8(p: Packed8, a: torch.Tensor, w: torch.Tensor, eps: float, *,
+                     rstd: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """add_rmsnorm_fwd of the packed x and a: h = to_dtype(x + a); y = rmsnorm(h).  Returns (h, y)."""
+    fmt, rows, cols = _packed("add_rmsnorm_fwd8", p)
+    _require_gpu(p.codes, a, w, rstd)
+    _same_dtype(a, w)
+    if a.shape != p.codes.shape or not a.is_contiguous():
+        raise ValueError("add_rmsnorm_fwd8: a must be contiguous, of the packed x's shape")
+    _norm8_args("add_rmsnorm_fwd8", w, cols, rows, rstd)
+    h, y = torch.empty_like(a), torch.empty_like(a)
+    _launch("fh_add_rmsnorm_fwd8", a, _dtype_code(a), fmt, _ptr(p.codes), _ptr(p.exps), _ptr(a), _ptr(w), _ptr(h),
+              _ptr(y), _fptr(rstd), rows, cols, float(eps))
+    return h, y
+
+
+def rmsnorm_bwd8(dy: torch.Tensor, p: Packed8, w: torch.Tensor, eps: float, *, rstd: torch.Tensor | None = None,
+                 dres: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """rmsnorm_bwd with the packed x: returns (dx [+ dres], dw)."""
+    fmt, rows, cols = _packed("rmsnorm_bwd8", p)
+    _require_gpu(p.codes, dy, w, rstd, dres)
+    _same_dtype(dy, w, dres)
+    for t, n in ((dy, "dy"), (dres, "dres")):
+        if t is not None and (not t.is_contiguous() or t.shape != p.codes.shape):
+            raise ValueError(f"rmsnorm_bwd8: {n} must be contiguous, of the packed x's shape")
+    _norm8_args("rmsnorm_bwd8", w, cols, rows, rstd)
+    dx, dw = torch.empty_like(dy), torch.empty_like(w)
+    nbytes = _lib.lib().fh_rmsnorm_bwd8_workspace_size(rows, cols)
+    ws = torch.empty(max(nbytes, 4) // 4, dtype=torch.float32, device=dy.device)
+    _launch("fh_rmsnorm_bwd8", dy, _dtype_code(dy), fmt, _ptr(dy), _ptr(p.codes), _ptr(p.exps), _ptr(w), _fptr(rstd),
+              _ptr(dres), _ptr(dx), _ptr(dw), _ptr(ws), rows, cols, float(eps))
     return dx, dw
 
 

@@ -9,9 +9,12 @@ device then run on the hand-written gfx950 kernels of ``libfemtohip.so``.
 """
 from .fused_checkpoint import (dispatch_counts, eight_bit_checkpoint, fused_checkpoint, last_fallback_reason,
                                reset_dispatch_counts)
+from .block_norms import block_norms
 from .boundary_ops import fuse_boundary_ops
 from .fused_attention import fuse_attention
+from .rotary import apply_rotary, rotary_frequencies
 from .weight_packing import pack_layer_weights
 
 __all__ = ["fused_checkpoint", "dispatch_counts", "reset_dispatch_counts", "last_fallback_reason",
-           "pack_layer_weights", "fuse_boundary_ops", "fuse_attention", "eight_bit_checkpoint"]
+           "pack_layer_weights", "fuse_boundary_ops", "fuse_attention", "eight_bit_checkpoint",
+           "block_norms", "apply_rotary", "rotary_frequencies"]

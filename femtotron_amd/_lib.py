@@ -22,6 +22,9 @@ FH_F32 = 1
 FH_INT8 = 0
 FH_E4M3 = 1
 
+FH_ROTARY_HALF = 0
+FH_ROTARY_INTERLEAVED = 1
+
 FH_OK = 0
 
 FH_GEMM_NT = 0
@@ -117,6 +120,15 @@ BLOCK_SIGNATURES: dict[str, tuple] = {
     "fh_add_rmsnorm_fwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, _V, POINTER(c_float), _I64, _I64, _F, _V]),
     "fh_rmsnorm_bwd8_workspace_size": (c_size_t, [_I64, _I64]),
     "fh_rmsnorm_bwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, POINTER(c_float), _V, _V, _V, _V, _I64, _I64, _F, _V]),
+    "fh_block_norms_fwd": (c_int, [c_int, _V, _V, _V, _V, _V, c_int, _F, _V, _V, POINTER(c_float), POINTER(c_float),
+                                   _I64, _I64, _F, _V]),
+    "fh_block_norms_bwd_workspace_size": (c_size_t, [_I64, _I64]),
+    "fh_block_norms_bwd": (c_int, [c_int, _V, _V, _V, _V, _V, _V, _V, c_int, _F, POINTER(c_float), POINTER(c_float),
+                                   _V, _V, _V, _V, _V, _V, _I64, _I64, _V]),
+    "fh_rotary_fwd": (c_int, [c_int, _V, _I64, _I64, _V, _I64, _I64, _V, _I64, _V, _I64, _I64, _I64, _I64, _I64, c_int,
+                              _V, _I64, _V, _F, _V]),
+    "fh_rotary_bwd": (c_int, [c_int, _V, _I64, _I64, _V, _I64, _I64, _V, _I64, _V, _I64, _I64, _I64, _I64, _I64, c_int,
+                              _V, _I64, _V, _F, _V]),
 }
 
 _lock = threading.Lock()

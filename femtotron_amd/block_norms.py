@@ -1,0 +1,74 @@
+"""The norms after and before a block, with the block's gate and residual scale, as one
+differentiable call.
+
+A stock Llama layer adds a block's output to the residual stream and norms the sum for
+the next block (transformers 5.15.0, models/llama/modeling_llama.py:284-325;
+``ops.add_rmsnorm_fwd``).  Layers that also norm the block's output, gate it or scale it
+before the add need
+
+    h = x + scale * gate * RMSNorm(a; w_post)      y = RMSNorm(h; w_pre)
+
+whose forward and backward each run in one pass here (fh_block_norms_fwd / _bwd).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ops
+
+
+def _aligned(t: torch.Tensor | None) -> torch.Tensor | None:
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class BlockNormsFunction(torch.autograd.Function):
+    """Saved: a, h, the vectors and the gate, and two fp32 values a row."""
+
+    @staticmethod
+    def forward(ctx, x, a, w_post, w_pre, gate, scale, eps):
+        rows = x.numel() // max(x.size(-1), 1)
+        rstd_post = None if w_post is None else torch.empty(rows, dtype=torch.float32, device=x.device)
+        rstd_pre = None if w_pre is None else torch.empty(rows, dtype=torch.float32, device=x.device)
+        h, y = ops.block_norms_fwd(x, a, w_post, w_pre, eps, gate=gate, scale=scale, rstd_post=rstd_post,
+                                   rstd_pre=rstd_pre)
+        ctx.save_for_backward(a if w_post is not None or gate is not None else None, None if w_pre is None else h, w_post,
+                              w_pre, gate, rstd_post, rstd_pre)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return h, y
+
+    @staticmethod
+    def backward(ctx, dh, dy):
+        a, h, w_post, w_pre, gate, rstd_post, rstd_pre = ctx.saved_tensors
+        if dh is None and dy is None:
+            return (None,) * 7
+        with torch.no_grad():
+            dh, dy = _aligned(dh), _aligned(dy)
+            if dh is None:
+                dh = torch.zeros_like(dy)
+            if dy is None and w_pre is not None:
+                dy = torch.zeros_like(dh)
+            grads = ops.block_norms_bwd(dh, dy, h, a, w_post, w_pre, gate=gate, scale=ctx.scale, rstd_post=rstd_post,
+                                        rstd_pre=rstd_pre)
+        dx, da, dw_post, dw_pre, dgate = grads
+        return dx, da, dw_post, dw_pre, dgate, None, None
+
+
+def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = None,
+                w_pre: torch.Tensor | None = None, *, gate: torch.Tensor | None = None, scale: float = 1.0,
+                eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(h, y) = (x + scale * gate * RMSNorm(a; w_post), RMSNorm(h; w_pre)) over the last
+    dim of x and a (one shape, bf16 or fp32, on a HIP device), differentiable in every
+    tensor.
+
+    ``w_post`` None: a enters without a norm; ``w_pre`` None: y is None (one of the
+    two is given).  ``gate``: one value a channel ([hidden], or with leading ones), one an
+    element (x's shape: expand a gate that is shared along some dims), or None.
+    y is the norm of h in x's dtype, as returned."""
+    if gate is not None and gate.shape != x.shape and gate.numel() == x.shape[-1] == gate.shape[-1]:
+        gate = gate.reshape(-1)
+    return BlockNormsFunction.apply(_aligned(x), _aligned(a), _aligned(w_post), _aligned(w_pre), _aligned(gate),
+                                    float(scale), float(eps))

@@ -318,6 +318,149 @@ def rope_bwd_(dqk: torch.Tensor, n_heads: int, head_dim: int, seq_len: int, cos:
     return dqk
 
 
+# --------------------------------------------------- norms around a block
+def _block_norms_args(name: str, like: torch.Tensor, w_post, w_pre, gate) -> tuple[int, int, int, int]:
+    """(dtype code, gate_per_token, rows, cols) of block norms over `like`'s rows, checked."""
+    cols = like.size(-1) if like.dim() else 0
+    rows = like.numel() // max(cols, 1)
+    if w_post is None and w_pre is None:
+        raise ValueError(f"{name}: at least one of w_post and w_pre is needed")
+    for w, n in ((w_post, "w_post"), (w_pre, "w_pre")):
+        if w is not None and (w.shape != (cols,) or not w.is_contiguous()):
+            raise ValueError(f"{name}: {n} must be a contiguous [{cols}] tensor, got {tuple(w.shape)}")
+    per_token = 0
+    if gate is not None:
+        per_token = int(gate.shape != (cols,))
+        if (per_token and gate.shape != like.shape) or not gate.is_contiguous():
+            raise ValueError(f"{name}: gate must be contiguous, of shape [{cols}] or {tuple(like.shape)}, got "
+                             f"{tuple(gate.shape)}")
+    return _dtype_code(like), per_token, rows, cols
+
+
+def block_norms_fwd(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None, w_pre: torch.Tensor | None, eps: float,
+                    *, gate: torch.Tensor | None = None, scale: float = 1.0, rstd_post: torch.Tensor | None = None,
+                    rstd_pre: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """h = to_dtype(x + scale * gate * rmsnorm(a; w_post)) and y = rmsnorm(h; w_pre), in
+    fp32 between those roundings (fh_block_norms_fwd).  w_post None: a enters as it is;
+    w_pre None: no y; gate [cols], of x's shape, or None.  Returns (h, y or None);
+    rstd_post and rstd_pre (fp32, one a row) receive what block_norms_bwd reads."""
+    _require_gpu(x, a, w_post, w_pre, gate, rstd_post, rstd_pre)
+    _same_dtype(x, a, w_post, w_pre, gate)
+    dt, per_token, rows, cols = _block_norms_args("block_norms_fwd", x, w_post, w_pre, gate)
+    if not x.is_contiguous() or not a.is_contiguous() or a.shape != x.shape:
+        raise ValueError("block_norms_fwd: x and a must be contiguous, of one shape")
+    for r, n in ((rstd_post, "rstd_post"), (rstd_pre, "rstd_pre")):
+        if r is not None and (r.numel() != rows or not r.is_contiguous()):
+            raise ValueError(f"block_norms_fwd: {n} must be contiguous with one entry per row")
+    h = torch.empty_like(x)
+    y = None if w_pre is None else torch.empty_like(x)
+    _launch("fh_block_norms_fwd", x, dt, _ptr(x), _ptr(a), _ptr(w_post), _ptr(w_pre), _ptr(gate), per_token, float(scale),
+            _ptr(h), _ptr(y), _fptr(rstd_post), _fptr(rstd_pre), rows, cols, float(eps))
+    return h, y
+
+
+def block_norms_bwd(dh: torch.Tensor, dy: torch.Tensor | None, h: torch.Tensor | None, a: torch.Tensor | None,
+                    w_post: torch.Tensor | None, w_pre: torch.Tensor | None, *, gate: torch.Tensor | None = None,
+                    scale: float = 1.0, rstd_post: torch.Tensor | None = None, rstd_pre: torch.Tensor | None = None):
+    """Gradients of block_norms_fwd: (dx, da, dw_post, dw_pre, dgate), None for what it
+    did not have.  dy, h and rstd_pre go with w_pre, rstd_post with w_post, a with
+    w_post or a gate."""
+    _require_gpu(dh, dy, h, a, w_post, w_pre, gate, rstd_post, rstd_pre)
+    _same_dtype(dh, dy, h, a, w_post, w_pre, gate)
+    dt, per_token, rows, cols = _block_norms_args("block_norms_bwd", dh, w_post, w_pre, gate)
+    if w_pre is not None and (dy is None or h is None or rstd_pre is None):
+        raise ValueError("block_norms_bwd: w_pre needs dy, h and rstd_pre")
+    if w_post is not None and rstd_post is None:
+        raise ValueError("block_norms_bwd: w_post needs rstd_post")
+    if a is None and (w_post is not None or gate is not None):
+        raise ValueError("block_norms_bwd: w_post and a gate need a")
+    for t, n in ((dh, "dh"), (dy, "dy"), (h, "h"), (a, "a")):
+        if t is not None and (not t.is_contiguous() or t.shape != dh.shape):
+            raise ValueError(f"block_norms_bwd: {n} must be contiguous, of dh's shape")
+    for r, n in ((rstd_post, "rstd_post"), (rstd_pre, "rstd_pre")):
+        if r is not None and (r.numel() != rows or not r.is_contiguous()):
+            raise ValueError(f"block_norms_bwd: {n} must be contiguous with one entry per row")
+    dx, da = torch.empty_like(dh), torch.empty_like(dh)
+    dw_post, dw_pre, dgate = (None if t is None else torch.empty_like(t) for t in (w_post, w_pre, gate))
+    nbytes = _lib.lib().fh_block_norms_bwd_workspace_size(rows, cols)
+    ws = torch.empty(max(nbytes, 4) // 4, dtype=torch.float32, device=dh.device)
+    _launch("fh_block_norms_bwd", dh, dt, _ptr(dh), _ptr(dy), _ptr(h), _ptr(a), _ptr(w_post), _ptr(w_pre), _ptr(gate),
+            per_token, float(scale), _fptr(rstd_post), _fptr(rstd_pre), _ptr(dx), _ptr(da), _ptr(dw_post), _ptr(dw_pre),
+            _ptr(dgate), _ptr(ws), rows, cols)
+    return dx, da, dw_post, dw_pre, dgate
+
+
+# ------------------------------------------------------- rotary positions
+_ROTARY_LAYOUTS = {"half": _lib.FH_ROTARY_HALF, "interleaved": _lib.FH_ROTARY_INTERLEAVED}
+
+
+def _rotary(name: str, q, k, positions: torch.Tensor, inv_freq: torch.Tensor, head_dim: int, rot_dim: int | None,
+            offset: int, layout: str, factor: float, out):
+    first = q if q is not None else k
+    if first is None:
+        raise ValueError(f"{name}: one of q and k is needed")
+    qo, ko = (None, None) if out is None else out
+    _require_gpu(first, q, k, positions, inv_freq, qo, ko)
+    _same_dtype(first, q, k, qo, ko)
+    dt, T = _dtype_code(first), first.size(0)
+    if layout not in _ROTARY_LAYOUTS:
+        raise ValueError(f"{name}: layout must be one of {tuple(_ROTARY_LAYOUTS)}, got {layout!r}")
+    if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+        raise TypeError(f"{name}: inv_freq must be contiguous float64")
+    rot = 2 * inv_freq.numel() if rot_dim is None else rot_dim
+    if inv_freq.dim() != 1 or rot != 2 * inv_freq.numel():
+        raise ValueError(f"{name}: inv_freq must hold rot_dim / 2 values, got {tuple(inv_freq.shape)} for {rot}")
+    if positions.dtype != torch.int64 or not positions.is_contiguous():
+        raise TypeError(f"{name}: positions must be contiguous int64")
+    side = []
+    for t, o, n in ((q, qo, "q"), (k, ko, "k")):
+        if t is None:
+            if o is not None:
+                raise ValueError(f"{name}: an output for {n} without {n}")
+            side.append((None, 0, 0, None, 0, None))
+            continue
+        ld = _rowmajor(t, f"{name}.{n}")
+        if t.size(0) != T or t.size(1) % head_dim:
+            raise ValueError(f"{name}: {n} must be [{T}, heads * {head_dim}], got {tuple(t.shape)}")
+        if o is None:
+            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        elif o.shape != t.shape:
+            raise ValueError(f"{name}: {n}'s output must have its shape")
+        lo = _rowmajor(o, f"{name}.{n} out")
+        # a single row's stride says nothing: the width stands for it
+        width = t.size(1)
+        side.append((t, ld if T > 1 else max(ld, width), width // head_dim, o, lo if T > 1 else max(lo, width), o))
+    if T and (positions.numel() == 0 or T % positions.numel()):
+        raise ValueError(f"{name}: {T} tokens are no multiple of {positions.numel()} positions")
+    (qt, ldq, nq, qp, ldqo, qo), (kt, ldk, nk, kp, ldko, ko) = side
+    if qt is not None and T == 1 and qt.data_ptr() == qp.data_ptr():
+        ldq = ldqo
+    if kt is not None and T == 1 and kt.data_ptr() == kp.data_ptr():
+        ldk = ldko
+    _launch(name, first, dt, _ptr(qt), ldq, nq, _ptr(kt), ldk, nk, _ptr(qp), ldqo, _ptr(kp), ldko, T, head_dim, rot,
+            offset, _ROTARY_LAYOUTS[layout], _ptr(positions), positions.numel(), _ptr(inv_freq), float(factor))
+    return qo, ko
+
+
+def rotary_fwd(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+               head_dim: int, rot_dim: int | None = None, offset: int = 0, layout: str = "half", factor: float = 1.0,
+               out: tuple | None = None) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """Turns the heads of the token-major views q and k [T, heads * head_dim] (either may
+    be None) by positions * inv_freq in dims [offset, offset + rot_dim) of each head,
+    pairs in the "half" or "interleaved" layout, cos and sin times factor; the other
+    dims pass (fh_rotary_fwd).  positions: int64, one a token or one a position of
+    sequences of equal length; inv_freq: float64 [rot_dim / 2].  `out`: (q, k) to
+    write to, which may be the inputs.  Returns (q, k)."""
+    return _rotary("fh_rotary_fwd", q, k, positions, inv_freq, head_dim, rot_dim, offset, layout, factor, out)
+
+
+def rotary_bwd(dq: torch.Tensor | None, dk: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
+               head_dim: int, rot_dim: int | None = None, offset: int = 0, layout: str = "half", factor: float = 1.0,
+               out: tuple | None = None) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """The gradients of rotary_fwd's inputs from those of its outputs: the turn back."""
+    return _rotary("fh_rotary_bwd", dq, dk, positions, inv_freq, head_dim, rot_dim, offset, layout, factor, out)
+
+
 # ------------------------------------------------------------------- SwiGLU
 def swiglu_fwd(g: torch.Tensor, u: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """p = to_dtype(to_dtype(silu(g)) * u) for 2-D row-major views g, u (same row stride)."""

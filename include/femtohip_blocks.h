@@ -68,6 +68,70 @@ int fh_rmsnorm_bwd8(fh_dtype dt, fh_fmt8 fmt, const void* dy, const void* codes,
                     void* dx, void* dw, void* workspace, int64_t rows, int64_t cols, float eps,
                     hipStream_t stream);
 
+/* ------------------------------------- norms after and before a block
+ * A block's output a enters the residual stream x through a norm, a gate and a
+ * residual scale, and the next block reads the stream through its norm:
+ *   n = a rsqrt(mean(a^2) + eps) w_post          (n = a without w_post)
+ *   h = to_dtype(x + scale * gate * n)           (gate 1 without one)
+ *   y = to_dtype(h rsqrt(mean(h^2) + eps) w_pre) (no y without w_pre)
+ * in fp32 between the roundings written; y is the norm of h as stored.  The
+ * residual adds and norms of modeling_llama.py:284-325 are the case without
+ * w_post, gate and scale (fh_add_rmsnorm_fwd, which rounds the normalised value
+ * as LlamaRMSNorm does).  At least one of w_post and w_pre is given.
+ * x, a, h, y: [rows, cols]; w_post, w_pre: [cols]; gate: [cols], or with
+ * gate_per_token [rows, cols]; rstd_post, rstd_pre (nullable): fp32 [rows], the
+ * reciprocal roots, which the backward reads.  cols % 8 == 0, cols <= 8192, all
+ * tensors 16-byte aligned, h none of x, a and gate.
+ */
+int fh_block_norms_fwd(fh_dtype dt, const void* x, const void* a, const void* w_post,
+                       const void* w_pre, const void* gate, int gate_per_token, float scale, void* h,
+                       void* y, float* rstd_post, float* rstd_pre, int64_t rows, int64_t cols,
+                       float eps, hipStream_t stream);
+
+/* Gradients of fh_block_norms_fwd for dh and dy (dy with w_pre only): dx and da
+ * [rows, cols]; dw_post, dw_pre [cols]; dgate of the gate's shape.  h and rstd_pre
+ * are read with w_pre, rstd_post with w_post, a with w_post or a gate; the others
+ * may be null.  The sums over rows are fp32, in a fixed order.  workspace:
+ * fh_block_norms_bwd_workspace_size bytes, 16-byte aligned. */
+size_t fh_block_norms_bwd_workspace_size(int64_t rows, int64_t cols);
+int fh_block_norms_bwd(fh_dtype dt, const void* dh, const void* dy, const void* h, const void* a,
+                       const void* w_post, const void* w_pre, const void* gate, int gate_per_token,
+                       float scale, const float* rstd_post, const float* rstd_pre, void* dx,
+                       void* da, void* dw_post, void* dw_pre, void* dgate, void* workspace,
+                       int64_t rows, int64_t cols, hipStream_t stream);
+
+/* --------------------------------------------------- rotary positions
+ * Rotary embedding of q and k from positions and frequencies, for part of a head
+ * or all of it.  Pair i of the rot_dim rotated dims (from `offset` on) of a head is
+ *   FH_ROTARY_HALF         dims (offset + i, offset + rot_dim / 2 + i)
+ *   FH_ROTARY_INTERLEAVED  dims (offset + 2i, offset + 2i + 1)
+ * and is turned by position * inv_freq[i] radians, cos and sin times `factor`;
+ * the other dims pass.  (fh_rope_fwd, apply_rotary_pos_emb of modeling_llama.py:
+ * 130-160, is the half layout over the whole head from tables in the model's
+ * dtype.)  Angles are computed in fp64, the turn in fp32, rounded once.
+ * Token-major: head h of q at columns h * head_dim of its row, row strides in
+ * elements; n_q or n_k may be 0, q and k then null.  Outputs may be their inputs
+ * (same stride) and overlap nothing else.  positions: int64 [n_positions] on the
+ * device, token t at positions[t % n_positions] (tokens a multiple);
+ * inv_freq: fp64 [rot_dim / 2] on the device.  (n_q + n_k) * head_dim <= 2^20,
+ * head_dim <= 1024.  The backward takes and gives gradients: the turn back.
+ */
+typedef enum fh_rotary_layout {
+  FH_ROTARY_HALF = 0,
+  FH_ROTARY_INTERLEAVED = 1
+} fh_rotary_layout;
+
+int fh_rotary_fwd(fh_dtype dt, const void* q, int64_t ldq, int64_t n_q, const void* k, int64_t ldk,
+                  int64_t n_k, void* q_out, int64_t ldqo, void* k_out, int64_t ldko, int64_t tokens,
+                  int64_t head_dim, int64_t rot_dim, int64_t offset, fh_rotary_layout layout,
+                  const int64_t* positions, int64_t n_positions, const double* inv_freq,
+                  float factor, hipStream_t stream);
+int fh_rotary_bwd(fh_dtype dt, const void* dq, int64_t lddq, int64_t n_q, const void* dk,
+                  int64_t lddk, int64_t n_k, void* dq_out, int64_t lddqo, void* dk_out,
+                  int64_t lddko, int64_t tokens, int64_t head_dim, int64_t rot_dim, int64_t offset,
+                  fh_rotary_layout layout, const int64_t* positions, int64_t n_positions,
+                  const double* inv_freq, float factor, hipStream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -54,3 +54,50 @@ def rmsnorm_bwd(dy: np.ndarray, x: np.ndarray, w: np.ndarray, eps: float):
     dx = r * (g - n * (g * n).mean(-1, keepdims=True))
     terms = r * (np.abs(g) + np.abs(n) * np.abs(g * n).mean(-1, keepdims=True))
     return dx, (dy * n).sum(0), terms
+
+
+def block_norms(x, a, w_post, w_pre, gate, scale, eps, h=None):
+    """(h, y or None); with h given (as stored), y is its norm."""
+    n = a if w_post is None else rmsnorm(a, w_post, eps)
+    s = x + scale * (1.0 if gate is None else gate) * n
+    return s, None if w_pre is None else rmsnorm(s if h is None else h, w_pre, eps)
+
+
+def block_norms_bwd(dh, dy, h, a, w_post, w_pre, gate, scale, eps):
+    """{name: (gradient, what fp32 roundings act on)} of block_norms at the stored h: the
+    second of each pair sums the magnitudes that its fp32 arithmetic adds up."""
+    g = 1.0 if gate is None else gate
+    D, mag, out = dh, np.abs(dh), {}
+    if w_pre is not None:
+        dn, _, terms = rmsnorm_bwd(dy, h, w_pre, eps)
+        D, mag = D + dn, mag + terms
+        n = rmsnorm(h, 1.0, eps)
+        out["dw_pre"] = (dy * n).sum(0), np.abs(dy * n).sum(0)
+    out["dx"] = D, mag
+    P, pmag = scale * g * D, np.abs(scale * g) * mag
+    n = a if w_post is None else rmsnorm(a, 1.0, eps)
+    nw = n if w_post is None else n * w_post
+    if w_post is not None:
+        out["dw_post"] = (P * n).sum(0), (pmag * np.abs(n)).sum(0)
+        out["da"] = rmsnorm_bwd(P, a, w_post, eps)[0], rmsnorm_bwd(pmag, np.abs(a), np.abs(w_post), eps)[2]
+    else:
+        out["da"] = P, pmag
+    if gate is not None:
+        dg, gmag = scale * D * nw, np.abs(scale * nw) * mag
+        out["dgate"] = (dg, gmag) if gate.ndim > 1 else (dg.sum(0), gmag.sum(0))
+    return out
+
+
+def rotary(x, pos, inv_freq, head_dim, offset, layout, factor, back=False):
+    """(x [T, heads * head_dim] turned, the magnitudes its roundings act on)."""
+    T, n = x.shape[0], len(inv_freq)
+    i = np.arange(n)
+    u, v = (offset + i, offset + n + i) if layout == "half" else (offset + 2 * i, offset + 2 * i + 1)
+    angle = np.resize(pos, T).astype(np.float64)[:, None] * inv_freq
+    c, s = factor * np.cos(angle)[:, None], factor * np.sin(-angle if back else angle)[:, None]
+    y = x.reshape(T, -1, head_dim).copy()
+    mag = np.zeros_like(y)
+    x0, x1 = y[..., u].copy(), y[..., v].copy()
+    y[..., u], y[..., v] = x0 * c - x1 * s, x1 * c + x0 * s
+    mag[..., u] = mag[..., v] = abs(factor) * (np.abs(x0) + np.abs(x1))
+    return y.reshape(T, -1), mag.reshape(T, -1)

@@ -10,45 +10,65 @@
 // remainder goes to [-pi/4, pi/4] in fp64 and to fp32 there, where Taylor's
 // polynomials of sin (to x^9) and cos (to x^10) are off by less than 2^-27.
 //
-// HBM-bound: q and k are read and written once and the angles, n a token, are
-// computed by each block once into LDS for all its heads (1/80 to 1/20 of the
-// elements), so no table is read.
+// HBM-bound: q and k are read and written once.  The angles, n a token, are
+// computed by each block into LDS for the heads it has of a token, so no table is
+// read.
 #include "femtohip_blocks.h"
 #include "fh_common.hpp"
 
 namespace fh {
 namespace {
 
-// V consecutive elements between memory and fp32 registers in one access
-// (fp32 of 8: two).
+// V consecutive elements, moved in one access (fp32 of 8: two) and kept as loaded.
 template <typename T, int V>
-struct Vec {
-  __device__ __forceinline__ static void load(const T* p, float v[V]) {
-    if constexpr (V == 8) {
-      Elem<T>::load8(p, v);
-    } else if constexpr (V == 4 && sizeof(T) == 2) {
-      const uint2 q = *reinterpret_cast<const uint2*>(p);
-      v[0] = __uint_as_float(q.x << 16);
-      v[1] = __uint_as_float(q.x & 0xffff0000u);
-      v[2] = __uint_as_float(q.y << 16);
-      v[3] = __uint_as_float(q.y & 0xffff0000u);
-    } else if constexpr (V == 4) {
-      const float4 q = *reinterpret_cast<const float4*>(p);
-      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else {
-      v[0] = Elem<T>::ld1(p);
-    }
+struct Vec;
+
+template <typename T>
+struct Vec<T, 8> {
+  using Raw = typename Elem<T>::Raw;
+  __device__ __forceinline__ static Raw load(const T* p) { return Elem<T>::ldraw(p); }
+  __device__ __forceinline__ static void store(T* p, const Raw& q) { Elem<T>::straw(p, q); }
+  __device__ __forceinline__ static void unpack(const Raw& q, float* v) { Elem<T>::unpack(q, v); }
+  __device__ __forceinline__ static Raw pack(const float* v) { return Elem<T>::pack(v); }
+};
+
+template <>
+struct Vec<uint16_t, 4> {
+  using Raw = uint2;
+  __device__ __forceinline__ static Raw load(const uint16_t* p) { return *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ static void store(uint16_t* p, const Raw& q) { *reinterpret_cast<uint2*>(p) = q; }
+  __device__ __forceinline__ static void unpack(const Raw& q, float* v) {
+    v[0] = __uint_as_float(q.x << 16);
+    v[1] = __uint_as_float(q.x & 0xffff0000u);
+    v[2] = __uint_as_float(q.y << 16);
+    v[3] = __uint_as_float(q.y & 0xffff0000u);
   }
-  __device__ __forceinline__ static void store(T* p, const float v[V]) {
-    if constexpr (V == 8) {
-      Elem<T>::store8(p, v);
-    } else if constexpr (V == 4 && sizeof(T) == 2) {
-      *reinterpret_cast<uint2*>(p) = make_uint2(pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]));
-    } else if constexpr (V == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      Elem<T>::st1(p, v[0]);
-    }
+  __device__ __forceinline__ static Raw pack(const float* v) {
+    return make_uint2(pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]));
+  }
+};
+
+template <>
+struct Vec<float, 4> {
+  using Raw = float4;
+  __device__ __forceinline__ static Raw load(const float* p) { return *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ static void store(float* p, const Raw& q) { *reinterpret_cast<float4*>(p) = q; }
+  __device__ __forceinline__ static void unpack(const Raw& q, float* v) {
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  }
+  __device__ __forceinline__ static Raw pack(const float* v) { return make_float4(v[0], v[1], v[2], v[3]); }
+};
+
+template <typename T>
+struct Vec<T, 1> {
+  using Raw = T;
+  __device__ __forceinline__ static Raw load(const T* p) { return *p; }
+  __device__ __forceinline__ static void store(T* p, const Raw& q) { *p = q; }
+  __device__ __forceinline__ static void unpack(const Raw& q, float* v) { v[0] = Elem<T>::ld1(&q); }
+  __device__ __forceinline__ static Raw pack(const float* v) {
+    Raw q;
+    Elem<T>::st1(&q, v[0]);
+    return q;
   }
 };
 
@@ -75,73 +95,86 @@ struct RotaryArgs {
   int64_t ldq, ldk, ldqo, ldko;  // row strides in elements
   const int64_t* pos;
   const double* inv_freq;
-  int64_t tokens, npos;
   float factor;
-  int nq, heads, head_dim, n, off;  // heads: q's and k's; n = rot_dim / 2
-  int rot_items, items, tpb;        // items a head (the first rot_items turn), tokens a block
-  int inplace;
-  FastDiv per_head, per_token;
+  uint32_t total;                         // items of the call
+  int nq, head_dim, n, off;               // n = rot_dim / 2
+  int rot_items, items;                   // items a head (the first rot_items turn)
+  FastDiv per_head, per_token;            // items of a head and of a token
+  FastDiv pairs, positions;               // n, and the number of positions
 };
 
-constexpr int kItemsPerBlock = 1024;
-constexpr int kMaxPairs = 2048;  // angles of a block, 16 KB
+constexpr int kMaxPairs = 2048 + 2 * 512;  // angles of a block: 256 items of at most 8 pairs, and two cut tokens
 
-// An item is V pairs of one head of one token, or 2V of its passing elements.
-// blockIdx.x: tokens tpb at a time; blockIdx.y: kItemsPerBlock of their items.
+// An item is V pairs of one head of one token, or 2V of its passing elements: two
+// accesses of V elements each way.  A thread has one, of the call's items token by
+// token, and has its loads under way before the block computes the angles of the
+// tokens it touches.  (More items a thread, or blocks of whole tokens, measured
+// slower: 16384 tokens of 36 heads of 64, forward and backward, 55 us with one
+// item, 60, 63 and 69 with two, four and eight; 86 with the loads behind the
+// angles.)
 template <typename T, int V, bool INTER, bool BWD>
 __global__ __launch_bounds__(256) void k_rotary(RotaryArgs p) {
   __shared__ __align__(16) float cs[kMaxPairs], sn[kMaxPairs];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tpb;
-  const int nt = static_cast<int>(min(static_cast<int64_t>(p.tpb), p.tokens - t0));
-  for (int i = threadIdx.x; i < nt * p.n; i += 256) {
-    const int tt = i / p.n;
-    const int64_t t = t0 + tt;
-    float s, c;
-    sincos_of(p.pos[t < p.npos ? t : t % p.npos], p.inv_freq[i - tt * p.n], s, c);
-    cs[i] = c * p.factor;
-    sn[i] = BWD ? -s * p.factor : s * p.factor;
-  }
-  __syncthreads();
-  const int all = nt * p.heads * p.items;
-  const int end = min(all, static_cast<int>(blockIdx.y + 1) * kItemsPerBlock);
-  for (int i = blockIdx.y * kItemsPerBlock + threadIdx.x; i < end; i += 256) {
-    const int tt = static_cast<int>(p.per_token.div(i));
-    const int in_token = i - tt * p.heads * p.items;
+  const uint32_t base = blockIdx.x * 256u, last = min(base + 255u, p.total - 1);
+  const uint32_t t0 = p.per_token.div(base), nt = p.per_token.div(last) - t0 + 1;
+  const uint32_t i = base + threadIdx.x;
+  const bool mine = i <= last;
+  typename Vec<T, V>::Raw u, v;
+  T *du = nullptr, *dv = nullptr;
+  int angle = -1;  // where the item's angles start; -1: it passes
+  if (mine) {
+    const uint32_t t = p.per_token.div(i);
+    const int in_token = static_cast<int>(i - t * p.per_token.d);
     const int head = static_cast<int>(p.per_head.div(in_token));
     const int item = in_token - head * p.items;
     const bool is_q = head < p.nq;
-    const int64_t t = t0 + tt;
     const int hd = (is_q ? head : head - p.nq) * p.head_dim;
-    const T* src = static_cast<const T*>(is_q ? p.q : p.k) + t * (is_q ? p.ldq : p.ldk) + hd;
-    T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + t * (is_q ? p.ldqo : p.ldko) + hd;
+    int d0, d1;
     if (item < p.rot_items) {
-      const int d0 = p.off + (INTER ? 2 : 1) * item * V, d1 = INTER ? d0 + V : d0 + p.n;
-      float u[2 * V], o[2 * V];
-      Vec<T, V>::load(src + d0, u);
-      Vec<T, V>::load(src + d1, u + V);
-      const float* cb = cs + tt * p.n + item * V;
-      const float* sb = sn + tt * p.n + item * V;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int a = INTER ? 2 * j : j, b = INTER ? 2 * j + 1 : j + V;
-        o[a] = u[a] * cb[j] - u[b] * sb[j];
-        o[b] = u[b] * cb[j] + u[a] * sb[j];
-      }
-      Vec<T, V>::store(dst + d0, o);
-      Vec<T, V>::store(dst + d1, o + V);
+      d0 = p.off + (INTER ? 2 : 1) * item * V;
+      d1 = INTER ? d0 + V : d0 + p.n;
+      angle = static_cast<int>(t - t0) * p.n + item * V;
     } else {
       const int pass = p.head_dim - 2 * p.n;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        int d = (2 * (item - p.rot_items) + m) * V;
-        if (d >= pass) break;
-        if (d >= p.off) d += 2 * p.n;
-        float u[V];
-        Vec<T, V>::load(src + d, u);
-        Vec<T, V>::store(dst + d, u);
-      }
+      d0 = 2 * (item - p.rot_items) * V;
+      d1 = d0 + V < pass ? d0 + V : d0;  // an odd last one twice
+      if (d0 >= p.off) d0 += 2 * p.n;
+      if (d1 >= p.off) d1 += 2 * p.n;
     }
+    const int64_t row = t;
+    const T* src = static_cast<const T*>(is_q ? p.q : p.k) + row * (is_q ? p.ldq : p.ldk) + hd;
+    T* dst = static_cast<T*>(is_q ? p.qo : p.ko) + row * (is_q ? p.ldqo : p.ldko) + hd;
+    u = Vec<T, V>::load(src + d0);
+    v = Vec<T, V>::load(src + d1);
+    du = dst + d0;
+    dv = dst + d1;
   }
+  for (uint32_t a = threadIdx.x; a < nt * p.n; a += 256) {
+    const uint32_t tt = p.pairs.div(a), t = t0 + tt;
+    float s, c;
+    sincos_of(p.pos[t - p.positions.div(t) * p.positions.d], p.inv_freq[a - tt * p.n], s, c);
+    cs[a] = c * p.factor;
+    sn[a] = BWD ? -s * p.factor : s * p.factor;
+  }
+  __syncthreads();
+  if (!mine) return;
+  if (angle >= 0) {
+    float x[2 * V], o[2 * V], c[V], s[V];
+    Vec<T, V>::unpack(u, x);
+    Vec<T, V>::unpack(v, x + V);
+    Vec<float, V>::unpack(Vec<float, V>::load(cs + angle), c);
+    Vec<float, V>::unpack(Vec<float, V>::load(sn + angle), s);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int a = INTER ? 2 * j : j, b = INTER ? 2 * j + 1 : j + V;
+      o[a] = x[a] * c[j] - x[b] * s[j];
+      o[b] = x[b] * c[j] + x[a] * s[j];
+    }
+    u = Vec<T, V>::pack(o);
+    v = Vec<T, V>::pack(o + V);
+  }
+  Vec<T, V>::store(du, u);
+  Vec<T, V>::store(dv, v);
 }
 
 template <bool BWD>
@@ -152,10 +185,11 @@ int rotary_impl(fh_dtype dt, const void* q, int64_t ldq, int64_t n_q, const void
   FH_REQUIRE(dt == FH_BF16 || dt == FH_F32, "rotary: dtype must be FH_BF16 or FH_F32");
   FH_REQUIRE(layout == FH_ROTARY_HALF || layout == FH_ROTARY_INTERLEAVED,
              "rotary: layout must be FH_ROTARY_HALF or FH_ROTARY_INTERLEAVED");
-  FH_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 24) * 256, "rotary: tokens must be >= 0 and < 2^32");
-  FH_REQUIRE(n_q >= 0 && n_k >= 0, "rotary: negative number of heads");
+  FH_REQUIRE(tokens >= 0, "rotary: tokens must be >= 0");
+  FH_REQUIRE(n_q >= 0 && n_k >= 0 && n_q <= (1 << 20) && n_k <= (1 << 20),
+             "rotary: a number of heads is negative or over 2^20");
   FH_REQUIRE(head_dim > 0 && head_dim <= 1024, "rotary: head_dim must be 1 to 1024");
-  FH_REQUIRE(rot_dim > 0 && rot_dim % 2 == 0 && offset >= 0 && offset + rot_dim <= head_dim,
+  FH_REQUIRE(rot_dim > 0 && rot_dim % 2 == 0 && rot_dim <= head_dim && offset >= 0 && offset <= head_dim - rot_dim,
              "rotary: rot_dim must be even and positive, and offset + rot_dim within the head");
   FH_REQUIRE((n_q + n_k) * head_dim <= (int64_t(1) << 20), "rotary: (n_q + n_k) * head_dim must be <= 2^20");
   FH_REQUIRE(ldq >= n_q * head_dim && ldqo >= n_q * head_dim && ldk >= n_k * head_dim && ldko >= n_k * head_dim,
@@ -166,8 +200,6 @@ int rotary_impl(fh_dtype dt, const void* q, int64_t ldq, int64_t n_q, const void
   const size_t size = dt == FH_BF16 ? 2 : 4;
   FH_REQUIRE((!n_q || q != qo || ldq == ldqo) && (!n_k || k != ko || ldk == ldko),
              "rotary: in place, input and output share their row stride");
-  RotaryArgs p{};
-  p.inplace = (n_q == 0 || q == qo) && (n_k == 0 || k == ko);
   // Accesses of 8 elements where every part of a head is whole in them and every
   // row aligned, else of 4, else single ones.
   const int64_t n = rot_dim / 2;
@@ -180,33 +212,32 @@ int rotary_impl(fh_dtype dt, const void* q, int64_t ldq, int64_t n_q, const void
   };
   const int v = fits(8) ? 8 : fits(4) ? 4 : 1;
   FH_REQUIRE(reinterpret_cast<uintptr_t>(q) % size == 0 && reinterpret_cast<uintptr_t>(k) % size == 0 &&
-                 reinterpret_cast<uintptr_t>(qo) % size == 0 && reinterpret_cast<uintptr_t>(ko) % size == 0,
+                 reinterpret_cast<uintptr_t>(qo) % size == 0 && reinterpret_cast<uintptr_t>(ko) % size == 0 && reinterpret_cast<uintptr_t>(positions) % 8 == 0 &&
+                 reinterpret_cast<uintptr_t>(inv_freq) % 8 == 0,
              "rotary: pointers must be aligned to their elements");
+  const bool inplace = (n_q == 0 || q == qo) && (n_k == 0 || k == ko);  // passing dims stay where they are
+  const int64_t pass = inplace ? 0 : head_dim - rot_dim;
+  const int64_t items = n / v + (pass + 2 * v - 1) / (2 * v), per_token = (n_q + n_k) * items;
+  FH_REQUIRE(tokens <= ((int64_t(1) << 32) - 256) / per_token,
+             "rotary: too many elements for one call (2^32 items of 16 elements, or fewer where rows are not aligned)");
+  RotaryArgs p{};
   p.q = q; p.k = k; p.qo = qo; p.ko = ko;
   p.ldq = ldq; p.ldk = ldk; p.ldqo = ldqo; p.ldko = ldko;
   p.pos = positions;
   p.inv_freq = inv_freq;
-  p.tokens = tokens;
-  p.npos = n_positions;
   p.factor = factor;
+  p.total = static_cast<uint32_t>(tokens * per_token);
   p.nq = static_cast<int>(n_q);
-  p.heads = static_cast<int>(n_q + n_k);
   p.head_dim = static_cast<int>(head_dim);
   p.n = static_cast<int>(n);
   p.off = static_cast<int>(offset);
-  p.rot_items = static_cast<int>(n) / v;
-  const int64_t pass = p.inplace ? 0 : head_dim - rot_dim;
-  p.items = p.rot_items + static_cast<int>((pass + 2 * v - 1) / (2 * v));
-  const int per_token = p.heads * p.items;
-  p.per_head = FastDiv(static_cast<uint32_t>(p.items));
+  p.rot_items = static_cast<int>(n / v);
+  p.items = static_cast<int>(items);
+  p.per_head = FastDiv(static_cast<uint32_t>(items));
   p.per_token = FastDiv(static_cast<uint32_t>(per_token));
-  int64_t tpb = kItemsPerBlock / per_token;
-  if (tpb * n > kMaxPairs) tpb = kMaxPairs / n;
-  p.tpb = static_cast<int>(tpb < 1 ? 1 : tpb > tokens ? tokens : tpb);
-  const int64_t gx = (tokens + p.tpb - 1) / p.tpb;
-  const int64_t gy = (static_cast<int64_t>(p.tpb) * per_token + kItemsPerBlock - 1) / kItemsPerBlock;
-  FH_REQUIRE(gx < (int64_t(1) << 24), "rotary: too many tokens for one call");  // fewer than 2^32 threads
-  const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
+  p.pairs = FastDiv(static_cast<uint32_t>(n));
+  p.positions = FastDiv(static_cast<uint32_t>(n_positions));
+  const dim3 grid(static_cast<unsigned>((p.total + 255ll) / 256));
   auto go = [&](auto tag, auto vec) {
     using T = decltype(tag);
     if (layout == FH_ROTARY_HALF) hipLaunchKernelGGL((k_rotary<T, vec(), false, BWD>), grid, dim3(256), 0, s, p);

@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -102,13 +103,12 @@ class RotaryFunction(torch.autograd.Function):
         return _turn(ops.rotary_fwd, q, k, positions, inv_freq, how)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         if dq is None and dk is None:
             return (None,) * 5
-        with torch.no_grad():
-            dq, dk = _turn(ops.rotary_bwd, dq, dk, positions, inv_freq, ctx.how)
-        return dq, dk, None, None, None
+        return (*_turn(ops.rotary_bwd, dq, dk, positions, inv_freq, ctx.how), None, None, None)
 
 
 def _turn(op, q, k, positions, inv_freq, how):
@@ -129,4 +129,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     length (any shape of that many); inv_freq, factor: ``rotary_frequencies``; layout:
     pairs (i, i + rot_dim / 2), "half", or (2i, 2i + 1), "interleaved"."""
     how = dict(head_dim=head_dim, rot_dim=rot_dim, offset=offset, layout=layout, factor=factor)
-    return RotaryFunction.apply(q, k, positions.contiguous(), inv_freq.contiguous(), how)
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+        return RotaryFunction.apply(q, k, positions, inv_freq, how)
+    return _turn(ops.rotary_fwd, q, k, positions, inv_freq, how)

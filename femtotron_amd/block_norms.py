@@ -13,6 +13,7 @@ whose forward and backward each run in one pass here (fh_block_norms_fwd / _bwd)
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -41,20 +42,18 @@ class BlockNormsFunction(torch.autograd.Function):
         return h, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dh, dy):
         a, h, w_post, w_pre, gate, rstd_post, rstd_pre = ctx.saved_tensors
         if dh is None and dy is None:
             return (None,) * 7
-        with torch.no_grad():
-            dh, dy = _aligned(dh), _aligned(dy)
-            if dh is None:
-                dh = torch.zeros_like(dy)
-            if dy is None and w_pre is not None:
-                dy = torch.zeros_like(dh)
-            grads = ops.block_norms_bwd(dh, dy, h, a, w_post, w_pre, gate=gate, scale=ctx.scale, rstd_post=rstd_post,
-                                        rstd_pre=rstd_pre)
-        dx, da, dw_post, dw_pre, dgate = grads
-        return dx, da, dw_post, dw_pre, dgate, None, None
+        dh, dy = _aligned(dh), _aligned(dy)
+        if dh is None:
+            dh = torch.zeros_like(dy)
+        if dy is None and w_pre is not None:
+            dy = torch.zeros_like(dh)
+        return (*ops.block_norms_bwd(dh, dy, h, a, w_post, w_pre, gate=gate, scale=ctx.scale, rstd_post=rstd_post,
+                                     rstd_pre=rstd_pre), None, None)
 
 
 def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = None,
@@ -70,5 +69,8 @@ def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = 
     y is the norm of h in x's dtype, as returned."""
     if gate is not None and gate.shape != x.shape and gate.numel() == x.shape[-1] == gate.shape[-1]:
         gate = gate.reshape(-1)
-    return BlockNormsFunction.apply(_aligned(x), _aligned(a), _aligned(w_post), _aligned(w_pre), _aligned(gate),
-                                    float(scale), float(eps))
+    tensors = tuple(map(_aligned, (x, a, w_post, w_pre, gate)))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return BlockNormsFunction.apply(*tensors, float(scale), float(eps))
+    x, a, w_post, w_pre, gate = tensors
+    return ops.block_norms_fwd(x, a, w_post, w_pre, float(eps), gate=gate, scale=float(scale))

@@ -40,6 +40,15 @@ __device__ __forceinline__ float row_sum(float v, float* red, int wave, int lane
   return s;
 }
 
+// 8 elements of a row, with STREAM as non-temporal loads: data read once.  16384 x
+// 2048, us: backward 86.6 -> 81.4, forward with a per-token gate (8192 x 4096) 62.1
+// -> 56.7; the forward's two rows without one 45.9 against 47.1, so not there.
+template <typename T, bool STREAM>
+__device__ __forceinline__ typename Elem<T>::Raw load_once(const T* p) {
+  if constexpr (STREAM) return Elem<T>::ldraw_stream(p);
+  else return Elem<T>::ldraw(p);
+}
+
 // A block takes kWaves / WPR rows a step; its barriers are reached by every wave
 // (the step loop is uniform, rows behind the last one are computed on zeros).
 template <typename T, int NVW, int WPR, int GATE, bool POST, bool PRE>
@@ -75,9 +84,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_fwd(
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
       if (!in(i)) continue;
-      ar[i] = E::ldraw(a + base + col(i));
-      xr[i] = E::ldraw(x + base + col(i));
-      if constexpr (GATE == kTokenGate) gr[i] = E::ldraw(gate + base + col(i));
+      ar[i] = load_once<T, GATE == kTokenGate>(a + base + col(i));
+      xr[i] = load_once<T, GATE == kTokenGate>(x + base + col(i));
+      if constexpr (GATE == kTokenGate) gr[i] = load_once<T, GATE == kTokenGate>(gate + base + col(i));
     }
     float ra = 1.f;
     if constexpr (POST) {
@@ -188,12 +197,12 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_bwd(
     for (int i = 0; i < NVW; ++i) {
       if (!in(i)) continue;
       if constexpr (PRE) {
-        dyr[i] = E::ldraw(dy + base + col(i));
-        hr[i] = E::ldraw(h + base + col(i));
+        dyr[i] = load_once<T, true>(dy + base + col(i));
+        hr[i] = load_once<T, true>(h + base + col(i));
       }
-      dhr[i] = E::ldraw(dh + base + col(i));
-      if constexpr (A) ar[i] = E::ldraw(a + base + col(i));
-      if constexpr (GATE == kTokenGate) gr[i] = E::ldraw(gate + base + col(i));
+      dhr[i] = load_once<T, true>(dh + base + col(i));
+      if constexpr (A) ar[i] = load_once<T, true>(a + base + col(i));
+      if constexpr (GATE == kTokenGate) gr[i] = load_once<T, true>(gate + base + col(i));
     }
     float D[NVW][8];
     float dot = 0.f, rh = 0.f;
@@ -347,24 +356,32 @@ __global__ __launch_bounds__(256) void k_block_norms_sums(const float* __restric
   }
 }
 
-constexpr int kMaxBlocks = 512;  // two blocks a CU; each leaves a partial row
+// Largest grids: the forward two blocks a CU; the backward one, since each leaves
+// partial rows (512 blocks 92.6 us and 384 98, 256 86.6 at 16384 x 2048).  Loading
+// the next step's rows ahead gained nothing (82.7 against 81.4).
+constexpr int kMaxBlocks[2] = {512, 256};
 
-// Waves a row and 8-element chunks a lane.
+// Waves a row: at most two chunks of 8 a lane (one: 91.6 us; four spill).
+constexpr int waves_per_row(int64_t cols) { return cols <= 1024 ? 1 : cols <= 2048 ? 2 : cols <= 4096 ? 4 : 8; }
+
+// f(chunks of 8 a lane, waves a row).
 template <typename F>
 void dispatch_cols(int cols, F&& f) {
   using std::integral_constant;
-  if (cols <= 512) f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  else if (cols <= 1024) f(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-  else if (cols <= 2048) f(integral_constant<int, 2>{}, integral_constant<int, 2>{});
-  else if (cols <= 4096) f(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-  else f(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+  auto go = [&](auto c) {
+    constexpr int wpr = waves_per_row(c());
+    f(integral_constant<int, c() / 512 / wpr>{}, integral_constant<int, wpr>{});
+  };
+  if (cols <= 512) go(integral_constant<int, 512>{});
+  else if (cols <= 1024) go(integral_constant<int, 1024>{});
+  else if (cols <= 2048) go(integral_constant<int, 2048>{});
+  else if (cols <= 4096) go(integral_constant<int, 4096>{});
+  else go(integral_constant<int, 8192>{});
 }
 
-int waves_per_row(int64_t cols) { return cols <= 1024 ? 1 : cols <= 2048 ? 2 : cols <= 4096 ? 4 : 8; }
-
-int grid_of(int64_t rows, int64_t cols) {
+int grid_of(int64_t rows, int64_t cols, bool bwd) {
   const int64_t rpb = kWaves / waves_per_row(cols), need = (rows + rpb - 1) / rpb;
-  return static_cast<int>(need < kMaxBlocks ? need : kMaxBlocks);
+  return static_cast<int>(need < kMaxBlocks[bwd] ? need : kMaxBlocks[bwd]);
 }
 
 // f(element tag, gate mode, has w_post, has w_pre); one of the norms is there.
@@ -411,7 +428,7 @@ extern "C" int fh_block_norms_fwd(fh_dtype dt, const void* x, const void* a, con
   FH_REQUIRE(x && a && h && (y || !w_pre), "block_norms_fwd: null pointer");
   FH_REQUIRE(all_aligned(x, a, w_post, w_pre, gate, h, y), "block_norms_fwd: pointers must be 16-byte aligned");
   FH_REQUIRE(h != x && h != a && h != gate, "block_norms_fwd: h must not alias x, a or the gate");
-  const int c = static_cast<int>(cols), blocks = grid_of(rows, cols);
+  const int c = static_cast<int>(cols), blocks = grid_of(rows, cols, false);
   dispatch_mode(dt, gate != nullptr, gate_per_token != 0, w_post != nullptr, w_pre != nullptr,
                 [&](auto tag, auto gm, auto post, auto pre) {
     using T = decltype(tag);
@@ -427,7 +444,7 @@ extern "C" int fh_block_norms_fwd(fh_dtype dt, const void* x, const void* a, con
 
 extern "C" size_t fh_block_norms_bwd_workspace_size(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return static_cast<size_t>(grid_of(rows, cols)) * 2 * static_cast<size_t>(cols) * sizeof(float);
+  return static_cast<size_t>(grid_of(rows, cols, true)) * 2 * static_cast<size_t>(cols) * sizeof(float);
 }
 
 extern "C" int fh_block_norms_bwd(fh_dtype dt, const void* dh, const void* dy, const void* h, const void* a,
@@ -449,7 +466,7 @@ extern "C" int fh_block_norms_bwd(fh_dtype dt, const void* dh, const void* dy, c
     FH_REQUIRE(!token || dgate, "block_norms_bwd: null pointer (dgate with a gate)");
     FH_REQUIRE(all_aligned(dh, dy, h, a, w_post, w_pre, gate, dx, da, dgate, workspace),
                "block_norms_bwd: pointers (workspace included) must be 16-byte aligned");
-    blocks = grid_of(rows, cols);
+    blocks = grid_of(rows, cols, true);
     dispatch_mode(dt, gate != nullptr, token, w_post != nullptr, w_pre != nullptr,
                   [&](auto tag, auto gm, auto post, auto pre) {
       using T = decltype(tag);

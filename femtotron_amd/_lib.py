@@ -115,15 +115,15 @@ BLOCK_SIGNATURES: dict[str, tuple] = {
     "fh_blocks_abi_version": (c_int, []),
     "fh_pack8": (c_int, [c_int, c_int, _V, _V, _V, _I64, _I64, _V]),
     "fh_unpack8": (c_int, [c_int, c_int, _V, _V, _V, _I64, _I64, _V]),
-    "fh_rmsnorm_fwd_pack8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, POINTER(c_float), _I64, _I64, _F, _V]),
-    "fh_rmsnorm_fwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, POINTER(c_float), _I64, _I64, _F, _V]),
-    "fh_add_rmsnorm_fwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, _V, POINTER(c_float), _I64, _I64, _F, _V]),
+    "fh_rmsnorm_fwd_pack8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, _V, _I64, _I64, _F, c_int, _V]),
+    "fh_rmsnorm_fwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, _I64, _I64, _F, c_int, _V]),
+    "fh_add_rmsnorm_fwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, _V, _V, _I64, _I64, _F, c_int, _V]),
     "fh_rmsnorm_bwd8_workspace_size": (c_size_t, [_I64, _I64]),
-    "fh_rmsnorm_bwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, POINTER(c_float), _V, _V, _V, _V, _I64, _I64, _F, _V]),
-    "fh_block_norms_fwd": (c_int, [c_int, _V, _V, _V, _V, _V, c_int, _F, _V, _V, POINTER(c_float), POINTER(c_float),
+    "fh_rmsnorm_bwd8": (c_int, [c_int, c_int, _V, _V, _V, _V, _V, _V, _V, _V, _V, _I64, _I64, _F, c_int, _V]),
+    "fh_block_norms_fwd": (c_int, [c_int, _V, _V, _V, _V, _V, c_int, _F, _V, _V, _V, _V,
                                    _I64, _I64, _F, _V]),
     "fh_block_norms_bwd_workspace_size": (c_size_t, [_I64, _I64]),
-    "fh_block_norms_bwd": (c_int, [c_int, _V, _V, _V, _V, _V, _V, _V, c_int, _F, POINTER(c_float), POINTER(c_float),
+    "fh_block_norms_bwd": (c_int, [c_int, _V, _V, _V, _V, _V, _V, _V, c_int, _F, _V, _V,
                                    _V, _V, _V, _V, _V, _V, _I64, _I64, _V]),
     "fh_rotary_fwd": (c_int, [c_int, _V, _I64, _I64, _V, _I64, _I64, _V, _I64, _V, _I64, _I64, _I64, _I64, _I64, c_int,
                               _V, _I64, _V, _F, _V]),

@@ -43,7 +43,7 @@ extern "C" size_t fh_rmsnorm_bwd_workspace_size(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
   // one fp32 partial row per backward block (4 rows per block, 2 above 2048
   // columns)
-  const int64_t nrows = bwd_blocks(rows, cols > 2048 ? 2 : 4);
+  const int64_t nrows = bwd_blocks(rows, cols > 2048 ? 2 : 4, kMaxBwdBlocks);
   return static_cast<size_t>(nrows) * static_cast<size_t>(cols) * sizeof(float);
 }
 

@@ -14,7 +14,8 @@
 //
 // XS (RowsT or Rows8) is how x is read; an x kept in 8 bits unpacks to values
 // that T holds exactly, so every result equals, bit for bit, that of the
-// unpacked tensor.
+// unpacked tensor.  RND: the normalised value and dy * w are rounded to T, as
+// LlamaRMSNorm's tensors are; without it only what is stored is rounded.
 #pragma once
 
 #include "fh_common.hpp"
@@ -47,6 +48,19 @@ struct Rows8 {
   __device__ __forceinline__ static void unpack(const Raw& q, float v[8]) { unpack8<FMT>(q, v); }
 };
 
+template <typename T, bool RND>
+__device__ __forceinline__ float rnd_if(float f) {
+  if constexpr (RND) return Elem<T>::rnd(f);
+  else return f;
+}
+
+// 8 elements, with STREAM as a non-temporal load: data read once.
+template <typename T, bool STREAM>
+__device__ __forceinline__ typename Elem<T>::Raw load_if(const T* p) {
+  if constexpr (STREAM) return Elem<T>::ldraw_stream(p);
+  else return Elem<T>::ldraw(p);
+}
+
 constexpr int kWavesPerBlock = 4;  // 256 threads
 
 // Forward: each wave takes rows row, row + stride, ... (stride = 4 x grid).
@@ -56,7 +70,7 @@ constexpr int kWavesPerBlock = 4;  // 256 threads
 // (two input rows): 45.2 -> 43.1 us at T = 16384, H = 2048 and 50.5 -> 48.8 us
 // at T = 8192, H = 4096; the one-input form measured no gain from it.
 // PACK: x also goes out in 8 bits (a format of fh_pack8.hpp; kNoPack: it does not).
-template <typename T, typename XS, int NV, bool ADD, bool PIPE, int PACK>
+template <typename T, typename XS, int NV, bool ADD, bool PIPE, int PACK, bool RND>
 __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
     const typename XS::Item* __restrict__ x, const uint8_t* __restrict__ xe, const T* __restrict__ a,
     const T* __restrict__ w, T* __restrict__ h, T* __restrict__ y, float* __restrict__ rstd,
@@ -126,7 +140,7 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
         else XS::unpack(xr[i], v);
         Elem<T>::unpack(wr[i], wv);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = Elem<T>::rnd(wv[j] * Elem<T>::rnd(v[j] * r));
+        for (int j = 0; j < 8; ++j) o[j] = Elem<T>::rnd(wv[j] * rnd_if<T, RND>(v[j] * r));
         Elem<T>::store8(y + base + c, o);
       }
     }
@@ -167,7 +181,8 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
 // gradient at T=16384, H=2048; with it (3 input rows) at that width the extra
 // registers cost a wave of occupancy and it gained nothing (60.8 vs 62.3 us);
 // BwdSplit chooses it per width.
-template <typename T, typename XS, int NVW, int WPR, int NWB, bool RES, bool HAVE_RSTD, bool PF>
+template <typename T, typename XS, int NVW, int WPR, int NWB, bool RES, bool HAVE_RSTD, bool PF, bool RND,
+          bool STREAM>
 __global__ __launch_bounds__(64 * NWB) void k_rmsnorm_bwd(
     const T* __restrict__ dy, const typename XS::Item* __restrict__ x, const uint8_t* __restrict__ xe,
     const T* __restrict__ w, const float* __restrict__ rstd, const T* __restrict__ dres,
@@ -208,8 +223,8 @@ __global__ __launch_bounds__(64 * NWB) void k_rmsnorm_bwd(
       const int c = col(i);
       if (c < cols) {
         xn[i] = XS::load(x, xe, row, cols, c);
-        gn[i] = Elem<T>::ldraw(dy + base + c);
-        if constexpr (RES) rn[i] = Elem<T>::ldraw(dres + base + c);
+        gn[i] = load_if<T, STREAM>(dy + base + c);
+        if constexpr (RES) rn[i] = load_if<T, STREAM>(dres + base + c);
       }
     }
   };
@@ -266,8 +281,8 @@ __global__ __launch_bounds__(64 * NWB) void k_rmsnorm_bwd(
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float n = xv[j] * r;
-          dot = fmaf(Elem<T>::rnd(gv[j] * wv[j]), n, dot);
-          acc[i][j] = fmaf(gv[j], Elem<T>::rnd(n), acc[i][j]);
+          dot = fmaf(rnd_if<T, RND>(gv[j] * wv[j]), n, dot);
+          acc[i][j] = fmaf(gv[j], rnd_if<T, RND>(n), acc[i][j]);
         }
       }
     }
@@ -289,7 +304,7 @@ __global__ __launch_bounds__(64 * NWB) void k_rmsnorm_bwd(
         XS::unpack(xr[i], xv);
         Elem<T>::unpack(gr[i], gv);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = r * (Elem<T>::rnd(gv[j] * wv[j]) - xv[j] * r * dot);
+        for (int j = 0; j < 8; ++j) o[j] = r * (rnd_if<T, RND>(gv[j] * wv[j]) - xv[j] * r * dot);
         if constexpr (RES) {
           float rv[8];
           Elem<T>::unpack(rr[i], rv);
@@ -387,9 +402,11 @@ constexpr int kMaxBwdBlocks = FH_NORM_BWD_BLOCKS;
 constexpr int64_t kFwdPipeBlocks = 768;
 // Grid cap of the pipelined one-input forward (2049-4096 bf16 columns).
 constexpr int64_t kFwdPipeBlocks1 = 512;
+// Grid cap of the pipelined forward of a packed x (1025-2048 bf16 columns).
+constexpr int64_t kFwdPipeBlocks8 = 1024;
 
 // codes, exps: the kept x that is read (XS = Rows8; x is then null) or written (PACK).
-template <typename T, typename XS, int PACK, int NV>
+template <typename T, typename XS, int PACK, int NV, bool RND = true>
 void launch_fwd(const void* x, const void* a, const void* w, void* h, void* y, float* rstd, const void* codes,
                 const uint8_t* exps, int64_t rows, int cols, float eps, hipStream_t s) {
   using Item = typename XS::Item;
@@ -399,7 +416,7 @@ void launch_fwd(const void* x, const void* a, const void* w, void* h, void* y, f
   auto* const eo = const_cast<uint8_t*>(exps);
   auto go = [&](auto add, auto pipe, int64_t blocks) {
     if constexpr (PACK == kNoPack || !add())
-      hipLaunchKernelGGL((k_rmsnorm_fwd<T, XS, NV, add(), pipe(), PACK>), dim3(static_cast<unsigned>(blocks)),
+      hipLaunchKernelGGL((k_rmsnorm_fwd<T, XS, NV, add(), pipe(), PACK, RND>), dim3(static_cast<unsigned>(blocks)),
                          dim3(256), 0, s, xp, exps, static_cast<const T*>(a), static_cast<const T*>(w),
                          static_cast<T*>(h), static_cast<T*>(y), rstd, co, eo, rows, cols, eps);
   };
@@ -410,6 +427,10 @@ void launch_fwd(const void* x, const void* a, const void* w, void* h, void* y, f
     // in flight fit the registers (bf16 up to 4096 columns, fp32 up to 2048)
     constexpr bool kPipe = NV * sizeof(typename Elem<T>::Raw) <= 128;
     go(yes, std::bool_constant<kPipe>{}, kPipe && need > kFwdPipeBlocks ? kFwdPipeBlocks : need);
+  } else if (XS::kPacked && NV == 4 && sizeof(typename Elem<T>::Raw) == 16 && need > kFwdPipeBlocks8) {
+    // packed x, 1025-2048 bf16 columns: 19.2 -> 17.1 us at T = 16384, H = 2048
+    // (half the loads of a bf16 row in flight a wave; at 1024 columns no gain)
+    go(no, yes, kFwdPipeBlocks8);
   } else if (NV == 8 && sizeof(typename Elem<T>::Raw) == 16 && need > kFwdPipeBlocks1) {
     // one input, 2049-4096 bf16 columns: pipelined over a capped grid (kernel
     // time 15.3 -> 14.1 us at T = 4096, 26.1 -> 23.7 us at 8192, H = 4096)
@@ -435,39 +456,61 @@ struct BwdSplit {
   static constexpr int NVW = NV / WPR;
   static constexpr int NWB = kWide || (NV == 4 && RES) ? 8 : 4;
   static constexpr int RPB = NWB / WPR;
-  static constexpr bool PF = !RES || kWide;
+  static constexpr bool PF = !RES || kWide, STREAM = false;
+  static constexpr int kBlocks = kMaxBwdBlocks;
 };
 
-// Blocks of the backward: one per RPB rows, at most kMaxBwdBlocks (each
-// writes one fp32 partial row of dw).
-int bwd_blocks(int64_t rows, int rpb) {
+// The split of a backward of a packed x that does not have to give
+// fh_rmsnorm_bwd's bits (RND false): two chunks a lane whatever the width, the next
+// row prefetched, one block of 8 waves a CU (256 partial rows), non-temporal loads.
+// Kernel and reduction against BwdSplit's, without and with the residual gradient:
+// 16384 x 2048 34.6 and 42.5 us against 36.0 and 44.9, 8192 x 4096 33.7 and 42.4
+// against 36.5 and 45.4, 4096 x 8192 35.3 and 43.6 against 57.8 and 94.8.  Without
+// the prefetch 43.7 and 51.2 (16384 x 2048), 512 blocks 34.3 and 45.6, four chunks a
+// lane 36.5 and 45.5.
+template <int NV, bool RES>
+struct Bwd8Split {
+  static constexpr int NVW = NV < 2 ? NV : 2;
+  static constexpr int WPR = NV / NVW;
+  static constexpr int NWB = 8;
+  static constexpr int RPB = NWB / WPR;
+  static constexpr bool PF = true, STREAM = true;
+  static constexpr int kBlocks = 256;
+};
+
+// Blocks of the backward: one per RPB rows, at most `most` (each writes one fp32
+// partial row of dw).
+inline int bwd_blocks(int64_t rows, int rpb, int most) {
   const int64_t need = (rows + rpb - 1) / rpb;
-  return static_cast<int>(need < kMaxBwdBlocks ? need : kMaxBwdBlocks);
+  return static_cast<int>(need < most ? need : most);
 }
 
-template <typename T, typename XS, int NV, bool RES, bool HR>
+template <typename T, typename XS, typename SP, bool RES, bool HR, bool RND>
 void launch_bwd_k(const void* dy, const void* x, const uint8_t* xe, const void* w, const float* rstd,
                   const void* dres, void* dx, float* part, int64_t rows, int cols, float eps,
                   int blocks, hipStream_t s) {
-  using SP = BwdSplit<NV, RES>;
-  hipLaunchKernelGGL((k_rmsnorm_bwd<T, XS, SP::NVW, SP::WPR, SP::NWB, RES, HR, SP::PF>), dim3(blocks), dim3(64 * SP::NWB),
-                     static_cast<size_t>(cols) * sizeof(float), s, static_cast<const T*>(dy),
+  hipLaunchKernelGGL((k_rmsnorm_bwd<T, XS, SP::NVW, SP::WPR, SP::NWB, RES, HR, SP::PF, RND, SP::STREAM>), dim3(blocks),
+                     dim3(64 * SP::NWB), static_cast<size_t>(cols) * sizeof(float), s, static_cast<const T*>(dy),
                      static_cast<const typename XS::Item*>(x), xe, static_cast<const T*>(w), rstd,
                      static_cast<const T*>(dres), static_cast<T*>(dx), part, rows, cols, eps);
 }
 
-template <typename T, typename XS, int NV>
+template <typename T, typename XS, int NV, bool RND = true>
 void launch_bwd(const void* dy, const void* x, const uint8_t* xe, const void* w, const float* rstd,
                 const void* dres, void* dx, void* dw, float* part, int64_t rows, int cols,
                 float eps, hipStream_t s) {
-  const bool res = dres != nullptr, hr = rstd != nullptr;
-  const int blocks = bwd_blocks(rows, res ? BwdSplit<NV, true>::RPB : BwdSplit<NV, false>::RPB);
-  if (res && hr) launch_bwd_k<T, XS, NV, true, true>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);
-  else if (res) launch_bwd_k<T, XS, NV, true, false>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);
-  else if (hr) launch_bwd_k<T, XS, NV, false, true>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);
-  else launch_bwd_k<T, XS, NV, false, false>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);
-  hipLaunchKernelGGL((k_reduce_parts<T>), dim3((cols + 15) / 16), dim3(256), 0, s, part, blocks, cols,
-                     static_cast<T*>(dw));
+  auto go = [&](auto res) {
+    // The rows' sums are added in the split's order: where a call promises
+    // fh_rmsnorm_bwd's bits it takes fh_rmsnorm_bwd's split.
+    using SP = std::conditional_t<RND, BwdSplit<NV, res()>, Bwd8Split<NV, res()>>;
+    const int blocks = bwd_blocks(rows, SP::RPB, SP::kBlocks);
+    if (rstd != nullptr) launch_bwd_k<T, XS, SP, res(), true, RND>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);
+    else launch_bwd_k<T, XS, SP, res(), false, RND>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);
+    hipLaunchKernelGGL((k_reduce_parts<T>), dim3((cols + 15) / 16), dim3(256), 0, s, part, blocks, cols,
+                       static_cast<T*>(dw));
+  };
+  if (dres != nullptr) go(std::true_type{});
+  else go(std::false_type{});
 }
 
 // Chunks of 8 per lane: cols <= 512*NV.

@@ -61,15 +61,17 @@ int check_rows(fh_dtype dt, int64_t rows, int64_t cols) {
   return FH_OK;
 }
 
-// f(element type tag, format) for a checked dtype and format.
+// f(element type tag, format) for a checked dtype and format; with `rounding`,
+// f(tag, format, whether the normalised value is rounded: in fp32 it is either way).
 template <typename F>
-void with_types(fh_dtype dt, fh_fmt8 fmt, F&& f) {
-  auto go = [&](auto tag) {
-    if (fmt == FH_INT8) f(tag, std::integral_constant<int, kFmtInt8>{});
-    else f(tag, std::integral_constant<int, kFmtE4M3>{});
+void with_types(fh_dtype dt, fh_fmt8 fmt, bool rounding, F&& f) {
+  auto go = [&](auto tag, auto rnd) {
+    if (fmt == FH_INT8) f(tag, std::integral_constant<int, kFmtInt8>{}, rnd);
+    else f(tag, std::integral_constant<int, kFmtE4M3>{}, rnd);
   };
-  if (dt == FH_BF16) go(uint16_t{});
-  else go(float{});
+  if (dt != FH_BF16) go(float{}, std::true_type{});
+  else if (rounding) go(uint16_t{}, std::true_type{});
+  else go(uint16_t{}, std::false_type{});
 }
 
 // Grid of a pack or unpack: FH_ERR_INVALID where it would pass the largest.
@@ -101,7 +103,7 @@ extern "C" int fh_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, void* codes, ui
   FH_REQUIRE(aligned16(x) && aligned8(codes), "pack8: x must be 16-byte and codes 8-byte aligned");
   const int cpr = static_cast<int>(blocks8(cols) * 4);
   const FastDiv fd(static_cast<uint32_t>(cpr));
-  with_types(dt, fmt, [&](auto tag, auto f) {
+  with_types(dt, fmt, true, [&](auto tag, auto f, auto) {
     using T = decltype(tag);
     hipLaunchKernelGGL((k_pack8<T, f()>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
                        stream, static_cast<const T*>(x), static_cast<uint8_t*>(codes), exps, rows,
@@ -120,7 +122,7 @@ extern "C" int fh_unpack8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uin
   FH_REQUIRE(aligned16(x) && aligned8(codes), "unpack8: x must be 16-byte and codes 8-byte aligned");
   const int cpr = static_cast<int>(blocks8(cols) * 4);
   const FastDiv fd(static_cast<uint32_t>(cpr));
-  with_types(dt, fmt, [&](auto tag, auto f) {
+  with_types(dt, fmt, true, [&](auto tag, auto f, auto) {
     using T = decltype(tag);
     hipLaunchKernelGGL((k_unpack8<T, f()>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
                        stream, static_cast<const uint8_t*>(codes), exps, static_cast<T*>(x), rows,
@@ -131,7 +133,7 @@ extern "C" int fh_unpack8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uin
 
 extern "C" int fh_rmsnorm_fwd_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, const void* w, void* y, void* codes,
                                     uint8_t* exps, float* rstd, int64_t rows, int64_t cols, float eps,
-                                    hipStream_t stream) {
+                                    int llama_rounding, hipStream_t stream) {
   if (int e = check_fmt(dt, fmt, "rmsnorm_fwd_pack8")) return e;
   if (int e = check_rows(dt, rows, cols)) return e;
   if (rows == 0) return FH_OK;
@@ -139,10 +141,10 @@ extern "C" int fh_rmsnorm_fwd_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, con
   FH_REQUIRE(aligned16(x) && aligned16(w) && aligned16(y) && aligned8(codes),
              "rmsnorm_fwd_pack8: pointers must be 16-byte aligned (codes 8-byte)");
   const int c = static_cast<int>(cols);
-  with_types(dt, fmt, [&](auto tag, auto f) {
+  with_types(dt, fmt, llama_rounding != 0, [&](auto tag, auto f, auto rnd) {
     using T = decltype(tag);
     dispatch_nv(c, [&](auto nv) {
-      launch_fwd<T, RowsT<T>, f(), nv()>(x, nullptr, w, nullptr, y, rstd, codes, exps, rows, c, eps, stream);
+      launch_fwd<T, RowsT<T>, f(), nv(), rnd()>(x, nullptr, w, nullptr, y, rstd, codes, exps, rows, c, eps, stream);
       return 0;
     });
   });
@@ -150,7 +152,8 @@ extern "C" int fh_rmsnorm_fwd_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, con
 }
 
 extern "C" int fh_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps, const void* w, void* y,
-                               float* rstd, int64_t rows, int64_t cols, float eps, hipStream_t stream) {
+                               float* rstd, int64_t rows, int64_t cols, float eps,
+                               int llama_rounding, hipStream_t stream) {
   if (int e = check_fmt(dt, fmt, "rmsnorm_fwd8")) return e;
   if (int e = check_rows(dt, rows, cols)) return e;
   if (rows == 0) return FH_OK;
@@ -158,10 +161,10 @@ extern "C" int fh_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, cons
   FH_REQUIRE(aligned8(codes) && aligned16(w) && aligned16(y),
              "rmsnorm_fwd8: pointers must be 16-byte aligned (codes 8-byte)");
   const int c = static_cast<int>(cols);
-  with_types(dt, fmt, [&](auto tag, auto f) {
+  with_types(dt, fmt, llama_rounding != 0, [&](auto tag, auto f, auto rnd) {
     using T = decltype(tag);
     dispatch_nv(c, [&](auto nv) {
-      launch_fwd<T, Rows8<f()>, kNoPack, nv()>(nullptr, nullptr, w, nullptr, y, rstd, codes, exps, rows, c, eps, stream);
+      launch_fwd<T, Rows8<f()>, kNoPack, nv(), rnd()>(nullptr, nullptr, w, nullptr, y, rstd, codes, exps, rows, c, eps, stream);
       return 0;
     });
   });
@@ -170,7 +173,7 @@ extern "C" int fh_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, cons
 
 extern "C" int fh_add_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps, const void* a,
                                    const void* w, void* h, void* y, float* rstd, int64_t rows, int64_t cols, float eps,
-                                   hipStream_t stream) {
+                                   int llama_rounding, hipStream_t stream) {
   if (int e = check_fmt(dt, fmt, "add_rmsnorm_fwd8")) return e;
   if (int e = check_rows(dt, rows, cols)) return e;
   if (rows == 0) return FH_OK;
@@ -179,10 +182,10 @@ extern "C" int fh_add_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, 
              "add_rmsnorm_fwd8: pointers must be 16-byte aligned (codes 8-byte)");
   FH_REQUIRE(h != a, "add_rmsnorm_fwd8: h must not alias a");
   const int c = static_cast<int>(cols);
-  with_types(dt, fmt, [&](auto tag, auto f) {
+  with_types(dt, fmt, llama_rounding != 0, [&](auto tag, auto f, auto rnd) {
     using T = decltype(tag);
     dispatch_nv(c, [&](auto nv) {
-      launch_fwd<T, Rows8<f()>, kNoPack, nv()>(nullptr, a, w, h, y, rstd, codes, exps, rows, c, eps, stream);
+      launch_fwd<T, Rows8<f()>, kNoPack, nv(), rnd()>(nullptr, a, w, h, y, rstd, codes, exps, rows, c, eps, stream);
       return 0;
     });
   });
@@ -190,12 +193,22 @@ extern "C" int fh_add_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, 
 }
 
 extern "C" size_t fh_rmsnorm_bwd8_workspace_size(int64_t rows, int64_t cols) {
-  return fh_rmsnorm_bwd_workspace_size(rows, cols);  // the same partial rows
+  if (rows <= 0 || cols <= 0 || cols > 8192) return 0;
+  // the partial rows of the split that a call takes: fh_rmsnorm_bwd's, or its own
+  size_t blocks = 0;
+  dispatch_nv(static_cast<int>(cols), [&](auto nv) {
+    using SP = Bwd8Split<nv(), false>;
+    blocks = static_cast<size_t>(bwd_blocks(rows, SP::RPB, SP::kBlocks));
+    return 0;
+  });
+  const size_t own = blocks * static_cast<size_t>(cols) * sizeof(float), other = fh_rmsnorm_bwd_workspace_size(rows, cols);
+  return own > other ? own : other;
 }
 
 extern "C" int fh_rmsnorm_bwd8(fh_dtype dt, fh_fmt8 fmt, const void* dy, const void* codes, const uint8_t* exps,
                                const void* w, const float* rstd, const void* dres, void* dx, void* dw, void* workspace,
-                               int64_t rows, int64_t cols, float eps, hipStream_t stream) {
+                               int64_t rows, int64_t cols, float eps,
+                               int llama_rounding, hipStream_t stream) {
   if (int e = check_fmt(dt, fmt, "rmsnorm_bwd8")) return e;
   if (int e = check_rows(dt, rows, cols)) return e;
   FH_REQUIRE(w && dw, "rmsnorm_bwd8: null pointer");
@@ -207,10 +220,10 @@ extern "C" int fh_rmsnorm_bwd8(fh_dtype dt, fh_fmt8 fmt, const void* dy, const v
              "rmsnorm_bwd8: pointers (workspace included) must be 16-byte aligned (codes 8-byte)");
   const int c = static_cast<int>(cols);
   float* part = static_cast<float*>(workspace);
-  with_types(dt, fmt, [&](auto tag, auto f) {
+  with_types(dt, fmt, llama_rounding != 0, [&](auto tag, auto f, auto rnd) {
     using T = decltype(tag);
     dispatch_nv(c, [&](auto nv) {
-      launch_bwd<T, Rows8<f()>, nv()>(dy, codes, exps, w, rstd, dres, dx, dw, part, rows, c, eps, stream);
+      launch_bwd<T, Rows8<f()>, nv(), rnd()>(dy, codes, exps, w, rstd, dres, dx, dw, part, rows, c, eps, stream);
       return 0;
     });
   });

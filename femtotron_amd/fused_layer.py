@@ -127,16 +127,19 @@ def layer_forward(x2: torch.Tensor | ops.Packed8, cos: torch.Tensor, sin: torch.
     acts = _Acts() if keep else None
     rstd1 = torch.empty(T, dtype=torch.float32, device=dev) if keep else None
     if packed_in:
-        y1 = ops.rmsnorm_fwd8(x2, w1, shp.eps1, rstd=rstd1)
+        y1 = ops.rmsnorm_fwd8(x2, w1, shp.eps1, rstd=rstd1, llama_rounding=True)
     elif pack is not None:
-        y1, kept = ops.rmsnorm_fwd_pack8(x2, w1, shp.eps1, pack, rstd=rstd1)
+        y1, kept = ops.rmsnorm_fwd_pack8(x2, w1, shp.eps1, pack, rstd=rstd1, llama_rounding=True)
     else:
         y1 = ops.rmsnorm_fwd(x2, w1, shp.eps1, rstd=rstd1)
 
     qkv, o, lse = qkv_attention(y1, _cat_rows(wq, wk, wv), batch, seq, shp, cos, sin, keep=keep)
     a = linear(o, wo)
     rstd2 = torch.empty(T, dtype=torch.float32, device=dev) if keep else None
-    h, z = (ops.add_rmsnorm_fwd8 if packed_in else ops.add_rmsnorm_fwd)(x2, a, w2, shp.eps2, rstd=rstd2)
+    if packed_in:
+        h, z = ops.add_rmsnorm_fwd8(x2, a, w2, shp.eps2, rstd=rstd2, llama_rounding=True)
+    else:
+        h, z = ops.add_rmsnorm_fwd(x2, a, w2, shp.eps2, rstd=rstd2)
     del a
     gu = linear(z, _cat_rows(wg, wu))
     F_ = shp.ffn
@@ -325,8 +328,10 @@ def layer_backward(dout2: torch.Tensor, x2: torch.Tensor | ops.Packed8, cos: tor
     dy1 = linear_dgrad(dqkv, _cat_rows(wq, wk, wv))
     del dqkv
     acts.y1 = None
-    norm_bwd = ops.rmsnorm_bwd8 if isinstance(x2, ops.Packed8) else ops.rmsnorm_bwd
-    dx, dw1 = norm_bwd(dy1, x2, w1, shp.eps1, rstd=acts.rstd1, dres=dh)
+    if isinstance(x2, ops.Packed8):
+        dx, dw1 = ops.rmsnorm_bwd8(dy1, x2, w1, shp.eps1, rstd=acts.rstd1, dres=dh, llama_rounding=True)
+    else:
+        dx, dw1 = ops.rmsnorm_bwd(dy1, x2, w1, shp.eps1, rstd=acts.rstd1, dres=dh)
     wg_stream.join()
     dwq, dwk, dwv = split_rows(dwqkv, shp.hq, shp.hkv, shp.hkv)
     dwg, dwu = split_rows(dwgu, F_, F_)

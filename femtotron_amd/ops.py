@@ -43,6 +43,31 @@ def _same_dtype(ref: torch.Tensor, *ts: torch.Tensor) -> None:
             raise TypeError(f"dtype mismatch: {t.dtype} vs {ref.dtype}")
 
 
+def _alike(ref: torch.Tensor, *ts: torch.Tensor | None) -> None:
+    """Every tensor on ref's HIP device and of its dtype (_require_gpu and _same_dtype in one pass)."""
+    dev, dt = ref.get_device(), ref.dtype
+    if dev < 0:
+        raise ValueError("femtohip ops take HIP device tensors only")
+    for t in ts:
+        if t is None:
+            continue
+        if t.get_device() != dev:
+            _require_gpu(ref, t)
+        if t.dtype != dt:
+            raise TypeError(f"dtype mismatch: {t.dtype} vs {dt}")
+
+
+def _row_stats(name: str, like: torch.Tensor, rows: int, *rs: torch.Tensor | None) -> None:
+    """Per-row fp32 statistics (rstd): on like's device, contiguous, one entry a row."""
+    for r in rs:
+        if r is None:
+            continue
+        if r.get_device() != like.get_device():
+            _require_gpu(like, r)
+        if r.dtype != torch.float32 or r.numel() != rows or not r.is_contiguous():
+            raise ValueError(f"{name}: rstd must be contiguous fp32 with one entry per row")
+
+
 def _rowmajor(t: torch.Tensor, name: str) -> int:
     """Row stride of a 2-D view whose last dim is contiguous."""
     if t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1):
@@ -60,11 +85,12 @@ def _stream(t: torch.Tensor) -> int:
 def _launch(name: str, t: torch.Tensor, *args) -> None:
     """Calls an entry point on the current stream of t's device, with that device
     the current one (the default stream's handle is 0 on every device)."""
-    if torch._C._cuda_getDevice() == t.device.index:
-        _lib.call(name, *args, _stream(t))
+    index = t.get_device()
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, _stream(t))
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _ptr(t: torch.Tensor | None):
@@ -169,29 +195,31 @@ def _empty8(x: torch.Tensor, fmt: str) -> Packed8:
 def _packed(name: str, p: Packed8) -> tuple[int, int, int]:
     """(format code, rows, cols) of a packed activation, checked."""
     codes, exps = p
-    _require_gpu(codes, exps)
-    if codes.dtype not in _FMT8_CODE or exps.dtype != torch.uint8:
+    fmt = _FMT8_CODE.get(codes.dtype)
+    if fmt is None or exps.dtype != torch.uint8:
         raise TypeError(f"{name}: codes must be int8 or float8_e4m3fn and exps uint8, got {codes.dtype}, {exps.dtype}")
-    if codes.dim() == 0 or not codes.is_contiguous() or not exps.is_contiguous():
+    if codes.get_device() < 0 or codes.get_device() != exps.get_device():
+        _require_gpu(codes, exps)
+    shape = codes.shape
+    if not shape or not codes.is_contiguous() or not exps.is_contiguous():
         raise ValueError(f"{name}: codes and exps must be contiguous")
-    cols = codes.size(-1)
-    if exps.shape != (*codes.shape[:-1], -(-cols // 32)):
-        raise ValueError(f"{name}: exps {tuple(exps.shape)} are not those of codes {tuple(codes.shape)}")
-    return _FMT8_CODE[codes.dtype], codes.numel() // max(cols, 1), cols
+    cols = shape[-1]
+    if exps.shape != (*shape[:-1], -(-cols // 32)):
+        raise ValueError(f"{name}: exps {tuple(exps.shape)} are not those of codes {tuple(shape)}")
+    return fmt, codes.numel() // max(cols, 1), cols
 
 
 def pack8(x: torch.Tensor, fmt: str = "int8") -> Packed8:
     """A contiguous x in 8.25 bits an element: blocks of 32 along the last dim with one
     power-of-two exponent, codes "int8" or "e4m3" (fh_pack8)."""
-    _require_gpu(x)
+    _alike(x)
     dt = _dtype_code(x)
     if not x.is_contiguous():
         raise ValueError("pack8: x must be contiguous")
-    p = _empty8(x, fmt)
+    codes, exps = p = _empty8(x, fmt)
     cols = x.size(-1)
     if x.numel():
-        _launch("fh_pack8", x, dt, _FMT8_CODE[p.codes.dtype], _ptr(x), _ptr(p.codes), _ptr(p.exps), x.numel() // cols,
-                  cols)
+        _launch("fh_pack8", x, dt, _FMT8_CODE[codes.dtype], _ptr(x), _ptr(codes), _ptr(exps), x.numel() // cols, cols)
     return p
 
 
@@ -205,72 +233,76 @@ def unpack8(p: Packed8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return x
 
 
-def _norm8_args(name: str, w: torch.Tensor, cols: int, rows: int, rstd: torch.Tensor | None) -> None:
-    if not w.is_contiguous() or w.numel() != cols:
+def _norm8_args(name: str, codes: torch.Tensor, w: torch.Tensor, cols: int, rows: int, rstd: torch.Tensor | None) -> int:
+    """The dtype code of w, checked to be the weight of a norm over the rows of codes."""
+    if w.get_device() != codes.get_device():
+        _require_gpu(codes, w)
+    if w.numel() != cols or not w.is_contiguous():
         raise ValueError(f"{name}: w must be contiguous, of the last dim's size")
-    if rstd is not None and (rstd.numel() != rows or not rstd.is_contiguous()):
-        raise ValueError(f"{name}: rstd must be contiguous with one entry per row")
+    if rstd is not None:
+        _row_stats(name, w, rows, rstd)
+    return _dtype_code(w)
 
 
 def rmsnorm_fwd_pack8(x: torch.Tensor, w: torch.Tensor, eps: float, fmt: str = "int8", *,
-                      rstd: torch.Tensor | None = None) -> tuple[torch.Tensor, Packed8]:
-    """(rmsnorm_fwd(x, w, eps), pack8(x, fmt)) in one pass over x."""
-    _require_gpu(x, w, rstd)
-    _same_dtype(x, w)
-    dt = _dtype_code(x)
+                      rstd: torch.Tensor | None = None, llama_rounding: bool = False) -> tuple[torch.Tensor, Packed8]:
+    """RMSNorm of x, and pack8(x, fmt), in one pass over x.  Rounded once; with
+    llama_rounding as rmsnorm_fwd is, the normalised value before its product with w."""
+    _alike(x, w)
     if not x.is_contiguous():
         raise ValueError("rmsnorm_fwd_pack8: x must be contiguous")
-    p = _empty8(x, fmt)
+    codes, exps = p = _empty8(x, fmt)
     cols = x.size(-1)
     rows = x.numel() // max(cols, 1)
-    _norm8_args("rmsnorm_fwd_pack8", w, cols, rows, rstd)
+    dt = _norm8_args("rmsnorm_fwd_pack8", x, w, cols, rows, rstd)
     y = torch.empty_like(x)
-    _launch("fh_rmsnorm_fwd_pack8", x, dt, _FMT8_CODE[p.codes.dtype], _ptr(x), _ptr(w), _ptr(y), _ptr(p.codes),
-              _ptr(p.exps), _fptr(rstd), rows, cols, float(eps))
+    _launch("fh_rmsnorm_fwd_pack8", x, dt, _FMT8_CODE[codes.dtype], _ptr(x), _ptr(w), _ptr(y), _ptr(codes), _ptr(exps),
+            _ptr(rstd), rows, cols, eps, llama_rounding)
     return y, p
 
 
-def rmsnorm_fwd8(p: Packed8, w: torch.Tensor, eps: float, *, rstd: torch.Tensor | None = None) -> torch.Tensor:
-    """rmsnorm_fwd of the packed x, in w's dtype: the bits of rmsnorm_fwd(unpack8(p), w, eps)."""
+def rmsnorm_fwd8(p: Packed8, w: torch.Tensor, eps: float, *, rstd: torch.Tensor | None = None,
+                 llama_rounding: bool = False) -> torch.Tensor:
+    """RMSNorm of the packed x, in w's dtype; with llama_rounding the bits of
+    rmsnorm_fwd(unpack8(p), w, eps)."""
     fmt, rows, cols = _packed("rmsnorm_fwd8", p)
-    _require_gpu(p.codes, w, rstd)
-    _norm8_args("rmsnorm_fwd8", w, cols, rows, rstd)
+    dt = _norm8_args("rmsnorm_fwd8", p.codes, w, cols, rows, rstd)
     y = torch.empty(p.codes.shape, dtype=w.dtype, device=w.device)
-    _launch("fh_rmsnorm_fwd8", w, _dtype_code(w), fmt, _ptr(p.codes), _ptr(p.exps), _ptr(w), _ptr(y), _fptr(rstd), rows,
-              cols, float(eps))
+    _launch("fh_rmsnorm_fwd8", w, dt, fmt, _ptr(p.codes), _ptr(p.exps), _ptr(w), _ptr(y), _ptr(rstd), rows, cols, eps,
+            llama_rounding)
     return y
 
 
-def add_rmsnorm_fwd8(p: Packed8, a: torch.Tensor, w: torch.Tensor, eps: float, *,
-                     rstd: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """add_rmsnorm_fwd of the packed x and a: h = to_dtype(x + a); y = rmsnorm(h).  Returns (h, y)."""
+def add_rmsnorm_fwd8(p: Packed8, a: torch.Tensor, w: torch.Tensor, eps: float, *, rstd: torch.Tensor | None = None,
+                     llama_rounding: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """h = to_dtype(x + a) of the packed x, and y = RMSNorm(h); with llama_rounding the bits
+    of add_rmsnorm_fwd.  Returns (h, y)."""
     fmt, rows, cols = _packed("add_rmsnorm_fwd8", p)
-    _require_gpu(p.codes, a, w, rstd)
-    _same_dtype(a, w)
+    _alike(a, w)
     if a.shape != p.codes.shape or not a.is_contiguous():
         raise ValueError("add_rmsnorm_fwd8: a must be contiguous, of the packed x's shape")
-    _norm8_args("add_rmsnorm_fwd8", w, cols, rows, rstd)
+    dt = _norm8_args("add_rmsnorm_fwd8", p.codes, w, cols, rows, rstd)
     h, y = torch.empty_like(a), torch.empty_like(a)
-    _launch("fh_add_rmsnorm_fwd8", a, _dtype_code(a), fmt, _ptr(p.codes), _ptr(p.exps), _ptr(a), _ptr(w), _ptr(h),
-              _ptr(y), _fptr(rstd), rows, cols, float(eps))
+    _launch("fh_add_rmsnorm_fwd8", a, dt, fmt, _ptr(p.codes), _ptr(p.exps), _ptr(a), _ptr(w), _ptr(h), _ptr(y),
+            _ptr(rstd), rows, cols, eps, llama_rounding)
     return h, y
 
 
 def rmsnorm_bwd8(dy: torch.Tensor, p: Packed8, w: torch.Tensor, eps: float, *, rstd: torch.Tensor | None = None,
-                 dres: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """rmsnorm_bwd with the packed x: returns (dx [+ dres], dw)."""
+                 dres: torch.Tensor | None = None, llama_rounding: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradients of RMSNorm at the packed x: (dx [+ dres], dw); with llama_rounding the bits
+    of rmsnorm_bwd."""
     fmt, rows, cols = _packed("rmsnorm_bwd8", p)
-    _require_gpu(p.codes, dy, w, rstd, dres)
-    _same_dtype(dy, w, dres)
+    _alike(dy, w, dres)
     for t, n in ((dy, "dy"), (dres, "dres")):
-        if t is not None and (not t.is_contiguous() or t.shape != p.codes.shape):
+        if t is not None and (t.shape != p.codes.shape or not t.is_contiguous()):
             raise ValueError(f"rmsnorm_bwd8: {n} must be contiguous, of the packed x's shape")
-    _norm8_args("rmsnorm_bwd8", w, cols, rows, rstd)
+    dt = _norm8_args("rmsnorm_bwd8", p.codes, w, cols, rows, rstd)
     dx, dw = torch.empty_like(dy), torch.empty_like(w)
     nbytes = _lib.lib().fh_rmsnorm_bwd8_workspace_size(rows, cols)
-    ws = torch.empty(max(nbytes, 4) // 4, dtype=torch.float32, device=dy.device)
-    _launch("fh_rmsnorm_bwd8", dy, _dtype_code(dy), fmt, _ptr(dy), _ptr(p.codes), _ptr(p.exps), _ptr(w), _fptr(rstd),
-              _ptr(dres), _ptr(dx), _ptr(dw), _ptr(ws), rows, cols, float(eps))
+    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=dy.device)
+    _launch("fh_rmsnorm_bwd8", dy, dt, fmt, _ptr(dy), _ptr(p.codes), _ptr(p.exps), _ptr(w), _ptr(rstd), _ptr(dres),
+            _ptr(dx), _ptr(dw), _ptr(ws), rows, cols, eps, llama_rounding)
     return dx, dw
 
 
@@ -344,18 +376,15 @@ def block_norms_fwd(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | Non
     fp32 between those roundings (fh_block_norms_fwd).  w_post None: a enters as it is;
     w_pre None: no y; gate [cols], of x's shape, or None.  Returns (h, y or None);
     rstd_post and rstd_pre (fp32, one a row) receive what block_norms_bwd reads."""
-    _require_gpu(x, a, w_post, w_pre, gate, rstd_post, rstd_pre)
-    _same_dtype(x, a, w_post, w_pre, gate)
+    _alike(x, a, w_post, w_pre, gate)
     dt, per_token, rows, cols = _block_norms_args("block_norms_fwd", x, w_post, w_pre, gate)
     if not x.is_contiguous() or not a.is_contiguous() or a.shape != x.shape:
         raise ValueError("block_norms_fwd: x and a must be contiguous, of one shape")
-    for r, n in ((rstd_post, "rstd_post"), (rstd_pre, "rstd_pre")):
-        if r is not None and (r.numel() != rows or not r.is_contiguous()):
-            raise ValueError(f"block_norms_fwd: {n} must be contiguous with one entry per row")
+    _row_stats("block_norms_fwd", x, rows, rstd_post, rstd_pre)
     h = torch.empty_like(x)
     y = None if w_pre is None else torch.empty_like(x)
-    _launch("fh_block_norms_fwd", x, dt, _ptr(x), _ptr(a), _ptr(w_post), _ptr(w_pre), _ptr(gate), per_token, float(scale),
-            _ptr(h), _ptr(y), _fptr(rstd_post), _fptr(rstd_pre), rows, cols, float(eps))
+    _launch("fh_block_norms_fwd", x, dt, _ptr(x), _ptr(a), _ptr(w_post), _ptr(w_pre), _ptr(gate), per_token, scale, _ptr(h),
+            _ptr(y), _ptr(rstd_post), _ptr(rstd_pre), rows, cols, eps)
     return h, y
 
 
@@ -365,8 +394,7 @@ def block_norms_bwd(dh: torch.Tensor, dy: torch.Tensor | None, h: torch.Tensor |
     """Gradients of block_norms_fwd: (dx, da, dw_post, dw_pre, dgate), None for what it
     did not have.  dy, h and rstd_pre go with w_pre, rstd_post with w_post, a with
     w_post or a gate."""
-    _require_gpu(dh, dy, h, a, w_post, w_pre, gate, rstd_post, rstd_pre)
-    _same_dtype(dh, dy, h, a, w_post, w_pre, gate)
+    _alike(dh, dy, h, a, w_post, w_pre, gate)
     dt, per_token, rows, cols = _block_norms_args("block_norms_bwd", dh, w_post, w_pre, gate)
     if w_pre is not None and (dy is None or h is None or rstd_pre is None):
         raise ValueError("block_norms_bwd: w_pre needs dy, h and rstd_pre")
@@ -377,15 +405,13 @@ def block_norms_bwd(dh: torch.Tensor, dy: torch.Tensor | None, h: torch.Tensor |
     for t, n in ((dh, "dh"), (dy, "dy"), (h, "h"), (a, "a")):
         if t is not None and (not t.is_contiguous() or t.shape != dh.shape):
             raise ValueError(f"block_norms_bwd: {n} must be contiguous, of dh's shape")
-    for r, n in ((rstd_post, "rstd_post"), (rstd_pre, "rstd_pre")):
-        if r is not None and (r.numel() != rows or not r.is_contiguous()):
-            raise ValueError(f"block_norms_bwd: {n} must be contiguous with one entry per row")
+    _row_stats("block_norms_bwd", dh, rows, rstd_post, rstd_pre)
     dx, da = torch.empty_like(dh), torch.empty_like(dh)
     dw_post, dw_pre, dgate = (None if t is None else torch.empty_like(t) for t in (w_post, w_pre, gate))
     nbytes = _lib.lib().fh_block_norms_bwd_workspace_size(rows, cols)
-    ws = torch.empty(max(nbytes, 4) // 4, dtype=torch.float32, device=dh.device)
+    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=dh.device)
     _launch("fh_block_norms_bwd", dh, dt, _ptr(dh), _ptr(dy), _ptr(h), _ptr(a), _ptr(w_post), _ptr(w_pre), _ptr(gate),
-            per_token, float(scale), _fptr(rstd_post), _fptr(rstd_pre), _ptr(dx), _ptr(da), _ptr(dw_post), _ptr(dw_pre),
+            per_token, scale, _ptr(rstd_post), _ptr(rstd_pre), _ptr(dx), _ptr(da), _ptr(dw_post), _ptr(dw_pre),
             _ptr(dgate), _ptr(ws), rows, cols)
     return dx, da, dw_post, dw_pre, dgate
 
@@ -400,8 +426,8 @@ def _rotary(name: str, q, k, positions: torch.Tensor, inv_freq: torch.Tensor, he
     if first is None:
         raise ValueError(f"{name}: one of q and k is needed")
     qo, ko = (None, None) if out is None else out
-    _require_gpu(first, q, k, positions, inv_freq, qo, ko)
-    _same_dtype(first, q, k, qo, ko)
+    _alike(first, q, k, qo, ko)
+    _require_gpu(first, positions, inv_freq)
     dt, T = _dtype_code(first), first.size(0)
     if layout not in _ROTARY_LAYOUTS:
         raise ValueError(f"{name}: layout must be one of {tuple(_ROTARY_LAYOUTS)}, got {layout!r}")
@@ -438,7 +464,7 @@ def _rotary(name: str, q, k, positions: torch.Tensor, inv_freq: torch.Tensor, he
     if kt is not None and T == 1 and kt.data_ptr() == kp.data_ptr():
         ldk = ldko
     _launch(name, first, dt, _ptr(qt), ldq, nq, _ptr(kt), ldk, nk, _ptr(qp), ldqo, _ptr(kp), ldko, T, head_dim, rot,
-            offset, _ROTARY_LAYOUTS[layout], _ptr(positions), positions.numel(), _ptr(inv_freq), float(factor))
+            offset, _ROTARY_LAYOUTS[layout], _ptr(positions), positions.numel(), _ptr(inv_freq), factor)
     return qo, ko
 
 

@@ -20,6 +20,7 @@ in "int8", 2^-4 |x| in "e4m3"), again bit for bit.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .fused_layer import _one_call, _one_call_backward, layer_backward, layer_forward
@@ -47,14 +48,14 @@ class PackedDecoderLayerFunction(torch.autograd.Function):
         return out.view(B, S, H)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         codes, exps, cos, sin, *w = ctx.saved_tensors
         kept, w, shp, B = ops.Packed8(codes, exps), tuple(w), ctx.shp, ctx.batch
         T, H = codes.shape
         S = T // B
         dout = dout.contiguous()
-        with torch.no_grad():
-            dx, dws = _backward(dout, kept, cos, sin, shp, B, S, w)
+        dx, dws = _backward(dout, kept, cos, sin, shp, B, S, w)
         return (None, dx.view(B, S, H), None, None, None, *dws)
 
 
@@ -80,12 +81,12 @@ class PackedMLPFunction(torch.autograd.Function):
         return m.view(z.shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dm):
         codes, exps, wg, wu, wd = ctx.saved_tensors
-        with torch.no_grad():
-            z2 = ops.unpack8(ops.Packed8(codes, exps), dm.dtype)
-            dz, dwg, dwu, dwd = mlp_backward(dm.contiguous().view(-1, z2.shape[-1]), z2, wg, wu, wd,
-                                             mlp_forward(z2, wg, wu, wd, keep=True))
+        z2 = ops.unpack8(ops.Packed8(codes, exps), dm.dtype)
+        dz, dwg, dwu, dwd = mlp_backward(dm.contiguous().view(-1, z2.shape[-1]), z2, wg, wu, wd,
+                                         mlp_forward(z2, wg, wu, wd, keep=True))
         return None, dz.view(dm.shape), dwg, dwu, dwd
 
 
@@ -94,14 +95,14 @@ class PackedRMSNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, fmt, x, w, eps):
-        y, kept = ops.rmsnorm_fwd_pack8(x, w, eps, fmt)
+        y, kept = ops.rmsnorm_fwd_pack8(x, w, eps, fmt, llama_rounding=True)
         ctx.save_for_backward(*kept, w)
         ctx.eps = eps
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         codes, exps, w = ctx.saved_tensors
-        with torch.no_grad():
-            dx, dw = ops.rmsnorm_bwd8(dy.contiguous(), ops.Packed8(codes, exps), w, ctx.eps)
+        dx, dw = ops.rmsnorm_bwd8(dy.contiguous(), ops.Packed8(codes, exps), w, ctx.eps, llama_rounding=True)
         return None, dx, dw, None

@@ -47,26 +47,30 @@ int fh_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, void* codes, uint8_t* exps
 int fh_unpack8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps, void* x,
                int64_t rows, int64_t cols, hipStream_t stream);
 
-/* fh_rmsnorm_fwd that also packs the x it reads: fh_rmsnorm_fwd and fh_pack8 in
- * one pass, bit for bit.  cols <= 8192, as in every norm here. */
+/* fh_rmsnorm_fwd that also packs the x it reads (as fh_pack8 does), in one pass.
+ * llama_rounding != 0: the normalised value is rounded to dt before its product
+ * with w, as LlamaRMSNorm does, and y is fh_rmsnorm_fwd's bit for bit; 0: it is
+ * not, and y is rounded once.  cols <= 8192, as in every norm here. */
 int fh_rmsnorm_fwd_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, const void* w, void* y,
                          void* codes, uint8_t* exps, float* rstd, int64_t rows, int64_t cols,
-                         float eps, hipStream_t stream);
+                         float eps, int llama_rounding, hipStream_t stream);
 
 /* fh_rmsnorm_fwd, fh_add_rmsnorm_fwd (h = to_dtype(x + a); y = rmsnorm(h)) and
- * fh_rmsnorm_bwd of a packed x: each equals, bit for bit, the call on the tensor
- * that fh_unpack8 gives.  dt is the dtype of every tensor but the packed one. */
+ * fh_rmsnorm_bwd of a packed x, read as the values that fh_unpack8 gives.  With
+ * llama_rounding each equals, bit for bit, the call on the unpacked tensor; without
+ * it the normalised value and dy * w stay in fp32.  dt is the dtype of every tensor
+ * but the packed one. */
 int fh_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps,
                     const void* w, void* y, float* rstd, int64_t rows, int64_t cols, float eps,
-                    hipStream_t stream);
+                    int llama_rounding, hipStream_t stream);
 int fh_add_rmsnorm_fwd8(fh_dtype dt, fh_fmt8 fmt, const void* codes, const uint8_t* exps,
                         const void* a, const void* w, void* h, void* y, float* rstd, int64_t rows,
-                        int64_t cols, float eps, hipStream_t stream);
+                        int64_t cols, float eps, int llama_rounding, hipStream_t stream);
 size_t fh_rmsnorm_bwd8_workspace_size(int64_t rows, int64_t cols);
 int fh_rmsnorm_bwd8(fh_dtype dt, fh_fmt8 fmt, const void* dy, const void* codes,
                     const uint8_t* exps, const void* w, const float* rstd, const void* dres,
                     void* dx, void* dw, void* workspace, int64_t rows, int64_t cols, float eps,
-                    hipStream_t stream);
+                    int llama_rounding, hipStream_t stream);
 
 /* ------------------------------------- norms after and before a block
  * A block's output a enters the residual stream x through a norm, a gate and a

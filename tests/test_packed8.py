@@ -49,13 +49,13 @@ def test_packed_calls_are_refused_on_the_host():
         ("fh_pack8", (0, 0, off, p, p, 4, 64, None), b"aligned"),
         ("fh_unpack8", (0, 0, off, p, p, 4, 64, None), b"aligned"),
         ("fh_unpack8", (0, -1, p, p, p, 4, 64, None), b"format"),
-        ("fh_rmsnorm_fwd_pack8", (0, 0, p, p, p, p, p, None, 4, 8200, 1e-5, None), b"8192"),
-        ("fh_rmsnorm_fwd_pack8", (0, 0, p, p, p, off, p, None, 4, 64, 1e-5, None), b"aligned"),
-        ("fh_rmsnorm_fwd8", (0, 1, p, None, p, p, None, 4, 64, 1e-5, None), b"null"),
-        ("fh_rmsnorm_fwd8", (0, 1, p, p, p, p, None, 1 << 26, 64, 1e-5, None), b"2^26"),
-        ("fh_add_rmsnorm_fwd8", (0, 1, p, p, p, p, p, p, None, 4, 64, 1e-5, None), b"alias"),
-        ("fh_rmsnorm_bwd8", (0, 1, p, p, p, p, None, None, p, p, None, 4, 64, 1e-5, None), b"null"),
-        ("fh_rmsnorm_bwd8", (0, 1, p, p, p, p, None, off, p, p, p, 4, 64, 1e-5, None), b"aligned"),
+        ("fh_rmsnorm_fwd_pack8", (0, 0, p, p, p, p, p, None, 4, 8200, 1e-5, 0, None), b"8192"),
+        ("fh_rmsnorm_fwd_pack8", (0, 0, p, p, p, off, p, None, 4, 64, 1e-5, 0, None), b"aligned"),
+        ("fh_rmsnorm_fwd8", (0, 1, p, None, p, p, None, 4, 64, 1e-5, 0, None), b"null"),
+        ("fh_rmsnorm_fwd8", (0, 1, p, p, p, p, None, 1 << 26, 64, 1e-5, 0, None), b"2^26"),
+        ("fh_add_rmsnorm_fwd8", (0, 1, p, p, p, p, p, p, None, 4, 64, 1e-5, 0, None), b"alias"),
+        ("fh_rmsnorm_bwd8", (0, 1, p, p, p, p, None, None, p, p, None, 4, 64, 1e-5, 0, None), b"null"),
+        ("fh_rmsnorm_bwd8", (0, 1, p, p, p, p, None, off, p, p, p, 4, 64, 1e-5, 0, None), b"aligned"),
     ]
     for name, args, word in bad:
         assert getattr(L, name)(*args) == 1, name
@@ -101,7 +101,7 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
 
     @contextmanager
     def device(d):
-        current[0], old = d.index, current[0]
+        current[0], old = d, current[0]
         yield
         current[0] = old
 
@@ -112,7 +112,7 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
 
     class T:
         def __init__(self, i):
-            self.device = torch.device("cuda", i)
+            self.get_device = lambda: i
 
     ops._launch("fh_x", T(0), 1)
     ops._launch("fh_x", T(3), 2)

@@ -126,19 +126,19 @@ def test_norms_equal_those_of_the_unpacked_tensor(rows, cols, fmt, dtype):
     a, dy, dres = (randn((rows, cols), s).to(dtype).to(DEV) for s in (6, 7, 8))
     w = (1 + randn((cols,), 9, 0.1)).to(dtype).to(DEV)
     r0, r1, r2 = (torch.empty(rows, device=DEV) for _ in range(3))
-    y, p = ops.rmsnorm_fwd_pack8(x, w, EPS, fmt, rstd=r0)
+    y, p = ops.rmsnorm_fwd_pack8(x, w, EPS, fmt, rstd=r0, llama_rounding=True)
     assert torch.equal(y, ops.rmsnorm_fwd(x, w, EPS, rstd=r1)) and torch.equal(r0, r1)
     q = ops.pack8(x, fmt)
     assert torch.equal(p.codes.view(torch.uint8), q.codes.view(torch.uint8)) and torch.equal(p.exps, q.exps)
     kept = ops.unpack8(p, dtype)
-    assert torch.equal(ops.rmsnorm_fwd8(p, w, EPS, rstd=r1), ops.rmsnorm_fwd(kept, w, EPS, rstd=r2)) and torch.equal(r1, r2)
-    for got, ref in zip(ops.add_rmsnorm_fwd8(p, a, w, EPS, rstd=r1), ops.add_rmsnorm_fwd(kept, a, w, EPS, rstd=r2)):
+    assert torch.equal(ops.rmsnorm_fwd8(p, w, EPS, rstd=r1, llama_rounding=True), ops.rmsnorm_fwd(kept, w, EPS, rstd=r2)) and torch.equal(r1, r2)
+    for got, ref in zip(ops.add_rmsnorm_fwd8(p, a, w, EPS, rstd=r1, llama_rounding=True), ops.add_rmsnorm_fwd(kept, a, w, EPS, rstd=r2)):
         assert torch.equal(got, ref)
     assert torch.equal(r1, r2)
-    ops.rmsnorm_fwd8(p, w, EPS, rstd=r1)
+    ops.rmsnorm_fwd8(p, w, EPS, rstd=r1, llama_rounding=True)
     for rstd in (None, r1):
         for res in (None, dres):
-            for got, ref in zip(ops.rmsnorm_bwd8(dy, p, w, EPS, rstd=rstd, dres=res),
+            for got, ref in zip(ops.rmsnorm_bwd8(dy, p, w, EPS, rstd=rstd, dres=res, llama_rounding=True),
                                 ops.rmsnorm_bwd(dy, kept, w, EPS, rstd=rstd, dres=res)):
                 assert torch.equal(got, ref)
 
@@ -154,25 +154,29 @@ def test_norms_against_fp64(rows, cols, fmt, dtype):
     xd, ad, dyd, dresd, wd = (t.to(DEV) for t in (x, a, dy, dres, w))
     half = HALF[dtype]
     kept = ob.unpack8(*ob.pack8(_f64(x), fmt))
-    y, p = ops.rmsnorm_fwd_pack8(xd, wd, EPS, fmt)
-    # y = to(w * to(x r)): two roundings
-    ref = ob.rmsnorm(_f64(x), _f64(w), EPS)
-    assert (np.abs(_f64(y) - ref) <= (2 * half + half * half + FUZZ) * np.abs(ref)).all()
-    ref = ob.rmsnorm(kept, _f64(w), EPS)
-    assert (np.abs(_f64(ops.rmsnorm_fwd8(p, wd, EPS)) - ref) <= (2 * half + half * half + FUZZ) * np.abs(ref)).all()
-    h, z = ops.add_rmsnorm_fwd8(p, ad, wd, EPS)
-    s = kept + _f64(a)
-    assert (np.abs(_f64(h) - s) <= (half + 2.0 ** -24) * np.abs(s)).all()
-    ref = ob.rmsnorm(_f64(h), _f64(w), EPS)
-    assert (np.abs(_f64(z) - ref) <= (2 * half + half * half + FUZZ) * np.abs(ref)).all()
-    dx, dw = ops.rmsnorm_bwd8(dyd, p, wd, EPS, dres=dresd)
-    rdx, rdw, terms = ob.rmsnorm_bwd(_f64(dy), kept, _f64(w), EPS)
-    rdx = rdx + _f64(dres)
-    # dy w is rounded, in dx's own term and in the mean; the sum is rounded once more
-    assert (np.abs(_f64(dx) - rdx) <= (half + 3 * FUZZ) * (terms + np.abs(rdx)) + 2.0 ** -23 * np.abs(_f64(dres))).all()
-    # the normalised value is rounded before the sum, and the sum once
-    n = np.abs(_f64(dy) * ob.rmsnorm(kept, 1.0, EPS)).sum(0)
-    assert (np.abs(_f64(dw) - rdw) <= half * np.abs(rdw) + (half + FUZZ + (rows + 128) * 2.0 ** -24) * n).all()
+    for llama in (False, True):
+        # y is rounded once; with llama_rounding its normalised value was rounded too
+        inner = half if llama else 0.0
+        tol = half + inner * (1 + half) + FUZZ
+        y, p = ops.rmsnorm_fwd_pack8(xd, wd, EPS, fmt, llama_rounding=llama)
+        ref = ob.rmsnorm(_f64(x), _f64(w), EPS)
+        assert (np.abs(_f64(y) - ref) <= tol * np.abs(ref)).all()
+        ref = ob.rmsnorm(kept, _f64(w), EPS)
+        assert (np.abs(_f64(ops.rmsnorm_fwd8(p, wd, EPS, llama_rounding=llama)) - ref) <= tol * np.abs(ref)).all()
+        h, z = ops.add_rmsnorm_fwd8(p, ad, wd, EPS, llama_rounding=llama)
+        s = kept + _f64(a)
+        assert (np.abs(_f64(h) - s) <= (half + 2.0 ** -24) * np.abs(s)).all()
+        ref = ob.rmsnorm(_f64(h), _f64(w), EPS)
+        assert (np.abs(_f64(z) - ref) <= tol * np.abs(ref)).all()
+        dx, dw = ops.rmsnorm_bwd8(dyd, p, wd, EPS, dres=dresd, llama_rounding=llama)
+        rdx, rdw, terms = ob.rmsnorm_bwd(_f64(dy), kept, _f64(w), EPS)
+        rdx = rdx + _f64(dres)
+        # with llama_rounding dy w is rounded, in dx's own term and in the mean; the sum is rounded once
+        lim = (half + 3 * FUZZ) * np.abs(rdx) + (inner + 3 * FUZZ) * terms + 2.0 ** -23 * np.abs(_f64(dres))
+        assert (np.abs(_f64(dx) - rdx) <= lim).all()
+        # and the normalised value before the sum over rows, which is rounded once
+        n = np.abs(_f64(dy) * ob.rmsnorm(kept, 1.0, EPS)).sum(0)
+        assert (np.abs(_f64(dw) - rdw) <= half * np.abs(rdw) + (inner + FUZZ + (rows + 128) * 2.0 ** -24) * n).all()
 
 
 def test_gradient_is_the_slope_of_the_norm_at_the_kept_value():

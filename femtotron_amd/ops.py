@@ -420,6 +420,14 @@ def block_norms_bwd(dh: torch.Tensor, dy: torch.Tensor | None, h: torch.Tensor |
 _ROTARY_LAYOUTS = {"half": _lib.FH_ROTARY_HALF, "interleaved": _lib.FH_ROTARY_INTERLEAVED}
 
 
+def _rotary_rows(name: str, t: torch.Tensor, T: int, head_dim: int) -> int:
+    """The row stride of a [T, heads * head_dim] view (of one row, which has none, its width)."""
+    ld, shape = _rowmajor(t, name), t.shape
+    if shape[0] != T or shape[1] % head_dim:
+        raise ValueError(f"{name} must be [{T}, heads * {head_dim}], got {tuple(shape)}")
+    return ld if T > 1 else shape[1]
+
+
 def _rotary(name: str, q, k, positions: torch.Tensor, inv_freq: torch.Tensor, head_dim: int, rot_dim: int | None,
             offset: int, layout: str, factor: float, out):
     first = q if q is not None else k
@@ -427,7 +435,8 @@ def _rotary(name: str, q, k, positions: torch.Tensor, inv_freq: torch.Tensor, he
         raise ValueError(f"{name}: one of q and k is needed")
     qo, ko = (None, None) if out is None else out
     _alike(first, q, k, qo, ko)
-    _require_gpu(first, positions, inv_freq)
+    if positions.get_device() != first.get_device() or inv_freq.get_device() != first.get_device():
+        _require_gpu(first, positions, inv_freq)
     dt, T = _dtype_code(first), first.size(0)
     if layout not in _ROTARY_LAYOUTS:
         raise ValueError(f"{name}: layout must be one of {tuple(_ROTARY_LAYOUTS)}, got {layout!r}")
@@ -438,34 +447,31 @@ def _rotary(name: str, q, k, positions: torch.Tensor, inv_freq: torch.Tensor, he
         raise ValueError(f"{name}: inv_freq must hold rot_dim / 2 values, got {tuple(inv_freq.shape)} for {rot}")
     if positions.dtype != torch.int64 or not positions.is_contiguous():
         raise TypeError(f"{name}: positions must be contiguous int64")
-    side = []
+    args = []
+    outs = []
     for t, o, n in ((q, qo, "q"), (k, ko, "k")):
         if t is None:
             if o is not None:
                 raise ValueError(f"{name}: an output for {n} without {n}")
-            side.append((None, 0, 0, None, 0, None))
-            continue
-        ld = _rowmajor(t, f"{name}.{n}")
-        if t.size(0) != T or t.size(1) % head_dim:
-            raise ValueError(f"{name}: {n} must be [{T}, heads * {head_dim}], got {tuple(t.shape)}")
-        if o is None:
-            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        elif o.shape != t.shape:
-            raise ValueError(f"{name}: {n}'s output must have its shape")
-        lo = _rowmajor(o, f"{name}.{n} out")
-        # a single row's stride says nothing: the width stands for it
-        width = t.size(1)
-        side.append((t, ld if T > 1 else max(ld, width), width // head_dim, o, lo if T > 1 else max(lo, width), o))
-    if T and (positions.numel() == 0 or T % positions.numel()):
-        raise ValueError(f"{name}: {T} tokens are no multiple of {positions.numel()} positions")
-    (qt, ldq, nq, qp, ldqo, qo), (kt, ldk, nk, kp, ldko, ko) = side
-    if qt is not None and T == 1 and qt.data_ptr() == qp.data_ptr():
-        ldq = ldqo
-    if kt is not None and T == 1 and kt.data_ptr() == kp.data_ptr():
-        ldk = ldko
-    _launch(name, first, dt, _ptr(qt), ldq, nq, _ptr(kt), ldk, nk, _ptr(qp), ldqo, _ptr(kp), ldko, T, head_dim, rot,
-            offset, _ROTARY_LAYOUTS[layout], _ptr(positions), positions.numel(), _ptr(inv_freq), factor)
-    return qo, ko
+            args.append((None, 0, 0, None, 0))
+        else:
+            ld = _rotary_rows(f"{name}: {n}", t, T, head_dim)
+            if o is None:
+                o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                lo = t.shape[1]
+            elif o.shape != t.shape:
+                raise ValueError(f"{name}: {n}'s output must have its shape")
+            else:
+                lo = _rotary_rows(f"{name}: {n}'s output", o, T, head_dim)
+            args.append((t.data_ptr(), ld, t.shape[1] // head_dim, o.data_ptr(), lo))
+        outs.append(o)
+    n_positions = positions.numel()
+    if T and (n_positions == 0 or T % n_positions):
+        raise ValueError(f"{name}: {T} tokens are no multiple of {n_positions} positions")
+    (qp, ldq, nq, qop, ldqo), (kp, ldk, nk, kop, ldko) = args
+    _launch(name, first, dt, qp, ldq, nq, kp, ldk, nk, qop, ldqo, kop, ldko, T, head_dim, rot, offset,
+            _ROTARY_LAYOUTS[layout], positions.data_ptr(), n_positions, inv_freq.data_ptr(), factor)
+    return tuple(outs)
 
 
 def rotary_fwd(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,

@@ -111,12 +111,20 @@ class RotaryFunction(torch.autograd.Function):
         return (*_turn(ops.rotary_bwd, dq, dk, positions, inv_freq, ctx.how), None, None, None)
 
 
+def _rows(t: torch.Tensor | None) -> torch.Tensor | None:
+    """t as token rows: a view where it is one, laid out first where it is none (a
+    transposed or an expanded gradient)."""
+    if t is None:
+        return None
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 and t.stride(0) >= t.size(1) else t.contiguous()
+
+
 def _turn(op, q, k, positions, inv_freq, how):
-    rows = [None if t is None else t.reshape(-1, t.shape[-1]) for t in (q, k)]
-    # what is no view of rows (a transposed or an expanded gradient) is laid out first
-    rows = [t if t is None or (t.stride(1) == 1 and t.stride(0) >= t.size(1)) else t.contiguous() for t in rows]
-    outs = op(*rows, positions, inv_freq, **how)
-    return tuple(None if t is None else o.view(t.shape) for t, o in zip((q, k), outs))
+    qo, ko = op(_rows(q), _rows(k), positions, inv_freq, **how)
+    return (qo if q is None or q.dim() == 2 else qo.view(q.shape),
+            ko if k is None or k.dim() == 2 else ko.view(k.shape))
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,

@@ -18,21 +18,14 @@ from torch.autograd.function import once_differentiable
 from . import ops
 
 
-def _aligned(t: torch.Tensor | None) -> torch.Tensor | None:
-    if t is None:
-        return None
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 class BlockNormsFunction(torch.autograd.Function):
     """Saved: a, h, the vectors and the gate, and two fp32 values a row."""
 
     @staticmethod
     def forward(ctx, x, a, w_post, w_pre, gate, scale, eps):
         rows = x.numel() // max(x.size(-1), 1)
-        rstd_post = None if w_post is None else torch.empty(rows, dtype=torch.float32, device=x.device)
-        rstd_pre = None if w_pre is None else torch.empty(rows, dtype=torch.float32, device=x.device)
+        rstd_post = None if w_post is None else x.new_empty(rows, dtype=torch.float32)
+        rstd_pre = None if w_pre is None else x.new_empty(rows, dtype=torch.float32)
         h, y = ops.block_norms_fwd(x, a, w_post, w_pre, eps, gate=gate, scale=scale, rstd_post=rstd_post,
                                    rstd_pre=rstd_pre)
         ctx.save_for_backward(a if w_post is not None or gate is not None else None, None if w_pre is None else h, w_post,
@@ -47,7 +40,7 @@ class BlockNormsFunction(torch.autograd.Function):
         a, h, w_post, w_pre, gate, rstd_post, rstd_pre = ctx.saved_tensors
         if dh is None and dy is None:
             return (None,) * 7
-        dh, dy = _aligned(dh), _aligned(dy)
+        dh, dy = ops.aligned(dh), ops.aligned(dy)
         if dh is None:
             dh = torch.zeros_like(dy)
         if dy is None and w_pre is not None:
@@ -69,7 +62,7 @@ def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = 
     y is the norm of h in x's dtype, as returned."""
     if gate is not None and gate.shape != x.shape and gate.numel() == x.shape[-1] == gate.shape[-1]:
         gate = gate.reshape(-1)
-    tensors = tuple(map(_aligned, (x, a, w_post, w_pre, gate)))
+    tensors = tuple(map(ops.aligned, (x, a, w_post, w_pre, gate)))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         return BlockNormsFunction.apply(*tensors, float(scale), float(eps))
     x, a, w_post, w_pre, gate = tensors

@@ -93,6 +93,14 @@ def _launch(name: str, t: torch.Tensor, *args) -> None:
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def aligned(t: torch.Tensor | None) -> torch.Tensor | None:
+    """t contiguous and 16-byte aligned, as the kernels take it: itself, or a copy."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
@@ -188,8 +196,7 @@ def _empty8(x: torch.Tensor, fmt: str) -> Packed8:
         raise ValueError(f"8-bit format must be one of {FORMATS8}, got {fmt!r}")
     if x.dim() == 0 or x.size(-1) % 8:
         raise ValueError(f"an activation's last dim must be a multiple of 8 to be packed, got shape {tuple(x.shape)}")
-    return Packed8(torch.empty(x.shape, dtype=_FMT8[fmt], device=x.device),
-                   torch.empty(*x.shape[:-1], -(-x.size(-1) // 32), dtype=torch.uint8, device=x.device))
+    return Packed8(torch.empty_like(x, dtype=_FMT8[fmt]), x.new_empty((*x.shape[:-1], -(-x.size(-1) // 32)), dtype=torch.uint8))
 
 
 def _packed(name: str, p: Packed8) -> tuple[int, int, int]:
@@ -226,7 +233,7 @@ def pack8(x: torch.Tensor, fmt: str = "int8") -> Packed8:
 def unpack8(p: Packed8, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values a packed activation stands for; bf16 and fp32 hold them exactly (fh_unpack8)."""
     fmt, rows, cols = _packed("unpack8", p)
-    x = torch.empty(p.codes.shape, dtype=dtype, device=p.codes.device)
+    x = torch.empty_like(p.codes, dtype=dtype)
     dt = _dtype_code(x)
     if x.numel():
         _launch("fh_unpack8", x, dt, fmt, _ptr(p.codes), _ptr(p.exps), _ptr(x), rows, cols)
@@ -267,7 +274,7 @@ def rmsnorm_fwd8(p: Packed8, w: torch.Tensor, eps: float, *, rstd: torch.Tensor 
     rmsnorm_fwd(unpack8(p), w, eps)."""
     fmt, rows, cols = _packed("rmsnorm_fwd8", p)
     dt = _norm8_args("rmsnorm_fwd8", p.codes, w, cols, rows, rstd)
-    y = torch.empty(p.codes.shape, dtype=w.dtype, device=w.device)
+    y = torch.empty_like(p.codes, dtype=w.dtype)
     _launch("fh_rmsnorm_fwd8", w, dt, fmt, _ptr(p.codes), _ptr(p.exps), _ptr(w), _ptr(y), _ptr(rstd), rows, cols, eps,
             llama_rounding)
     return y
@@ -300,7 +307,7 @@ def rmsnorm_bwd8(dy: torch.Tensor, p: Packed8, w: torch.Tensor, eps: float, *, r
     dt = _norm8_args("rmsnorm_bwd8", p.codes, w, cols, rows, rstd)
     dx, dw = torch.empty_like(dy), torch.empty_like(w)
     nbytes = _lib.lib().fh_rmsnorm_bwd8_workspace_size(rows, cols)
-    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=dy.device)
+    ws = dy.new_empty(max(nbytes, 4), dtype=torch.uint8)
     _launch("fh_rmsnorm_bwd8", dy, dt, fmt, _ptr(dy), _ptr(p.codes), _ptr(p.exps), _ptr(w), _ptr(rstd), _ptr(dres),
             _ptr(dx), _ptr(dw), _ptr(ws), rows, cols, eps, llama_rounding)
     return dx, dw
@@ -409,7 +416,7 @@ def block_norms_bwd(dh: torch.Tensor, dy: torch.Tensor | None, h: torch.Tensor |
     dx, da = torch.empty_like(dh), torch.empty_like(dh)
     dw_post, dw_pre, dgate = (None if t is None else torch.empty_like(t) for t in (w_post, w_pre, gate))
     nbytes = _lib.lib().fh_block_norms_bwd_workspace_size(rows, cols)
-    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=dh.device)
+    ws = dh.new_empty(max(nbytes, 4), dtype=torch.uint8)
     _launch("fh_block_norms_bwd", dh, dt, _ptr(dh), _ptr(dy), _ptr(h), _ptr(a), _ptr(w_post), _ptr(w_pre), _ptr(gate),
             per_token, scale, _ptr(rstd_post), _ptr(rstd_pre), _ptr(dx), _ptr(da), _ptr(dw_post), _ptr(dw_pre),
             _ptr(dgate), _ptr(ws), rows, cols)
@@ -457,7 +464,7 @@ def _rotary(name: str, q, k, positions: torch.Tensor, inv_freq: torch.Tensor, he
         else:
             ld = _rotary_rows(f"{name}: {n}", t, T, head_dim)
             if o is None:
-                o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                o = torch.empty_like(t, memory_format=torch.contiguous_format)
                 lo = t.shape[1]
             elif o.shape != t.shape:
                 raise ValueError(f"{name}: {n}'s output must have its shape")

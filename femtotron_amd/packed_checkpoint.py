@@ -44,19 +44,16 @@ class PackedDecoderLayerFunction(torch.autograd.Function):
         else:
             out, kept = layer_forward(x2, cos, sin, shp, B, S, w, keep=False, pack=fmt)
         ctx.save_for_backward(*kept, cos, sin, *w)
-        ctx.shp, ctx.batch = shp, B
+        ctx.shp, ctx.batch, ctx.seq = shp, B, S
         return out.view(B, S, H)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         codes, exps, cos, sin, *w = ctx.saved_tensors
-        kept, w, shp, B = ops.Packed8(codes, exps), tuple(w), ctx.shp, ctx.batch
-        T, H = codes.shape
-        S = T // B
-        dout = dout.contiguous()
-        dx, dws = _backward(dout, kept, cos, sin, shp, B, S, w)
-        return (None, dx.view(B, S, H), None, None, None, *dws)
+        B, S = ctx.batch, ctx.seq
+        dx, dws = _backward(ops.aligned(dout), ops.Packed8(codes, exps), cos, sin, ctx.shp, B, S, tuple(w))
+        return (None, dx.view(B, S, codes.shape[-1]), None, None, None, *dws)
 
 
 def _backward(dout, kept, cos, sin, shp, B, S, w):
@@ -85,7 +82,7 @@ class PackedMLPFunction(torch.autograd.Function):
     def backward(ctx, dm):
         codes, exps, wg, wu, wd = ctx.saved_tensors
         z2 = ops.unpack8(ops.Packed8(codes, exps), dm.dtype)
-        dz, dwg, dwu, dwd = mlp_backward(dm.contiguous().view(-1, z2.shape[-1]), z2, wg, wu, wd,
+        dz, dwg, dwu, dwd = mlp_backward(ops.aligned(dm).view(-1, z2.shape[-1]), z2, wg, wu, wd,
                                          mlp_forward(z2, wg, wu, wd, keep=True))
         return None, dz.view(dm.shape), dwg, dwu, dwd
 
@@ -104,5 +101,5 @@ class PackedRMSNormFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         codes, exps, w = ctx.saved_tensors
-        dx, dw = ops.rmsnorm_bwd8(dy.contiguous(), ops.Packed8(codes, exps), w, ctx.eps, llama_rounding=True)
+        dx, dw = ops.rmsnorm_bwd8(ops.aligned(dy), ops.Packed8(codes, exps), w, ctx.eps, llama_rounding=True)
         return None, dx, dw, None

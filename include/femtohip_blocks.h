@@ -4,7 +4,8 @@
  * block, and rotary positions.  Same library and conventions as femtohip.h
  * (device pointers owned by the caller, workspaces passed in, asynchronous on
  * `stream`, int status with fh_last_error(), thread-safe: no state of its own);
- * versioned by itself.
+ * versioned by itself.  Outputs and workspaces overlap no operand of their call
+ * unless its comment allows it.
  */
 #ifndef FEMTOHIP_BLOCKS_H_
 #define FEMTOHIP_BLOCKS_H_
@@ -115,10 +116,10 @@ int fh_block_norms_bwd(fh_dtype dt, const void* dh, const void* dy, const void* 
  * dtype.)  Angles are computed in fp64, the turn in fp32, rounded once.
  * Token-major: head h of q at columns h * head_dim of its row, row strides in
  * elements; n_q or n_k may be 0, q and k then null.  Outputs may be their inputs
- * (same stride) and overlap nothing else.  positions: int64 [n_positions] on the
+ * (same stride) and overlap nothing else (refused).  positions: int64 [n_positions] on the
  * device, token t at positions[t % n_positions] (tokens a multiple);
  * inv_freq: fp64 [rot_dim / 2] on the device.  (n_q + n_k) * head_dim <= 2^20,
- * head_dim <= 1024.  The backward takes and gives gradients: the turn back.
+ * head_dim <= 1024, row strides <= 2^28.  The backward takes and gives gradients: the turn back.
  */
 typedef enum fh_rotary_layout {
   FH_ROTARY_HALF = 0,

@@ -235,3 +235,65 @@ def test_another_stream_and_a_replayed_graph():
         torch.cuda.synchronize()
         kept = [o.clone() for o in outs]
         assert all(torch.equal(p, q) for p, q in zip(kept, step())), k
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 elements: the last rows equal those of a call on them alone."""
+    ops = _ops()
+    rows, cols = (1 << 19) + 3, 8192
+    w = (1 + randn((cols,), 91, 0.1)).bfloat16().to(DEV)
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = randn((3, cols), 92).bfloat16().to(DEV)
+    tail = x[-3:].clone()
+    r1, r2, s1, s2 = (torch.empty(n, device=DEV) for n in (rows, rows, 3, 3))
+    h, y = ops.block_norms_fwd(x, x, w, w, EPS, rstd_post=r1, rstd_pre=r2)
+    ht, yt = ops.block_norms_fwd(tail, tail, w, w, EPS, rstd_post=s1, rstd_pre=s2)
+    assert torch.equal(h[-3:], ht) and torch.equal(y[-3:], yt) and torch.equal(r1[-3:], s1) and torch.equal(r2[-3:], s2)
+    del y
+    dx, da, *_ = ops.block_norms_bwd(x, x, h, x, w, w, rstd_post=r1, rstd_pre=r2)
+    dxt, dat, *_ = ops.block_norms_bwd(tail, tail, ht, tail, w, w, rstd_post=s1, rstd_pre=s2)
+    assert torch.equal(dx[-3:], dxt) and torch.equal(da[-3:], dat)
+
+
+def test_a_second_derivative_is_refused():
+    from femtotron_amd import block_norms
+    x, g = (randn((4, 64), s).to(DEV).requires_grad_(True) for s in (93, 94))
+    h, _ = block_norms(x, x, torch.ones(64, device=DEV))
+    (dx,) = torch.autograd.grad(h, [x], g, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+def test_a_step_with_its_backward_in_a_graph():
+    """block_norms and its gradients captured together, on leaves that no eager graph holds."""
+    from femtotron_amd import block_norms
+    t = _inputs(300, 688, torch.bfloat16, True, True, "token", seed=101)
+    names = ["x", "a", "w_post", "w_pre", "gate"]
+
+    def step(leaves):
+        h, y = block_norms(leaves["x"], leaves["a"], leaves["w_post"], leaves["w_pre"], gate=leaves["gate"], scale=0.5)
+        return [h.detach(), y.detach(), *torch.autograd.grad((h, y), [leaves[n] for n in names], (t["dh"], t["dy"]))]
+
+    def fresh():
+        return {n: t[n].clone().requires_grad_(True) for n in names}
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(fresh())
+    torch.cuda.current_stream().wait_stream(side)
+    held = fresh()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step(held)
+    for k in range(4):
+        new = _inputs(300, 688, torch.bfloat16, True, True, "token", seed=110 + k)
+        with torch.no_grad():
+            for n, v in new.items():
+                t[n].copy_(v)
+            for n in names:
+                held[n].copy_(t[n])
+        g.replay()
+        torch.cuda.synchronize()
+        kept = [o.clone() for o in outs]
+        assert all(torch.equal(p, q) for p, q in zip(kept, step(fresh()))), k

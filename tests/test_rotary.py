@@ -54,8 +54,8 @@ def test_calls_are_refused_on_the_host():
     if not _lib.LIB_PATH.exists():
         pytest.skip("libfemtohip.so not built")
     L = _lib.lib()
-    p = ctypes.c_void_p(1 << 20)  # never read: every call below is refused before a launch
-    ok = dict(dt=0, q=p, ldq=256, nq=4, k=p, ldk=128, nk=2, qo=p, ldqo=256, ko=p, ldko=128, tokens=6, hd=64, rot=64,
+    p, r = ctypes.c_void_p(1 << 20), ctypes.c_void_p(1 << 24)  # never read: every call below is refused before a launch
+    ok = dict(dt=0, q=p, ldq=256, nq=4, k=r, ldk=128, nk=2, qo=p, ldqo=256, ko=r, ldko=128, tokens=6, hd=64, rot=64,
               off=0, layout=0, pos=p, npos=6, f=p, factor=1.0, stream=None)
     for change, word in ((dict(dt=5), b"dtype"), (dict(layout=2), b"layout"), (dict(tokens=-1), b"tokens"),
                          (dict(nq=-1), b"heads"), (dict(hd=0), b"head_dim"), (dict(hd=2048, rot=64), b"head_dim"),
@@ -63,7 +63,12 @@ def test_calls_are_refused_on_the_host():
                          (dict(ldq=255), b"stride"), (dict(ldko=64), b"stride"), (dict(k=None), b"null"),
                          (dict(pos=None), b"null"), (dict(f=None), b"null"), (dict(npos=4), b"n_positions"),
                          (dict(npos=0), b"n_positions"), (dict(ldqo=512), b"in place"), (dict(nq=1 << 20, ldq=1 << 30, ldqo=1 << 30), b"2^20"),
-                         (dict(q=ctypes.c_void_p((1 << 20) + 1)), b"aligned")):
+                         (dict(ldq=1 << 29, ldqo=1 << 29), b"2^28"),
+                         (dict(q=ctypes.c_void_p((1 << 22) + 1)), b"aligned"), (dict(qo=r), b"overlap"),
+                         (dict(ko=ctypes.c_void_p((1 << 20) + 2 * 255)), b"overlap"),
+                         (dict(qo=ctypes.c_void_p((1 << 20) + 2)), b"overlap"), (dict(nq=1 << 30), b"heads"),
+                         (dict(pos=ctypes.c_void_p((1 << 20) + 4)), b"aligned"), (dict(off=1 << 62), b"rot_dim"),
+                         (dict(tokens=1 << 40, npos=1 << 20), b"too many")):
         for name in ("fh_rotary_fwd", "fh_rotary_bwd"):
             assert getattr(L, name)(*{**ok, **change}.values()) == 1, change
             assert word in L.fh_last_error(), (change, L.fh_last_error())

@@ -177,6 +177,38 @@ def test_refusals():
     from femtotron_amd._lib import FemtoHipError
     with pytest.raises(FemtoHipError, match="within the head"):
         apply_rotary(q, None, pos, f, head_dim=64, offset=8)
+    k = torch.zeros_like(q)
+    for out in ((k, q), (k, k), (q, q)):  # another operand's, or one for both
+        with pytest.raises(FemtoHipError, match="overlap"):
+            ops.rotary_fwd(q, k, pos, f, head_dim=64, out=out)
+    both = torch.zeros(6, 256, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(FemtoHipError, match="overlap"):  # shifted by half a head
+        ops.rotary_fwd(both[:, :128], None, pos, f, head_dim=64, out=(both[:, 32:160], None))
+    ops.rotary_fwd(both[:, :128], None, pos, f, head_dim=64, out=(both[:, 128:], None))  # beside it
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 elements: the last rows equal those turned alone."""
+    ops = _ops()
+    T, hd = (1 << 20) + 5, 64
+    f, pos = _freq(hd), torch.arange(T, device=DEV)
+    q = torch.empty(T, 65 * hd, dtype=torch.bfloat16, device=DEV)
+    q[-5:] = randn((5, 65 * hd), 15).bfloat16().to(DEV)
+    ref, _ = ops.rotary_fwd(q[-5:].clone(), None, pos[-5:].clone(), f, head_dim=hd)
+    got, _ = ops.rotary_fwd(q, None, pos, f, head_dim=hd)
+    assert torch.equal(got[-5:], ref)
+    ops.rotary_fwd(q, None, pos, f, head_dim=hd, out=(q, None))
+    assert torch.equal(q[-5:], ref)
+
+
+def test_a_second_derivative_is_refused():
+    from femtotron_amd import apply_rotary
+    q = randn((4, 64), 16).to(DEV).requires_grad_(True)
+    g = randn((4, 64), 17).to(DEV).requires_grad_(True)
+    o, _ = apply_rotary(q, None, torch.arange(4, device=DEV), _freq(64), head_dim=64)
+    (dq,) = torch.autograd.grad(o, [q], g, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.sum().backward()
 
 
 def test_another_stream_and_a_replayed_graph():

@@ -34,6 +34,35 @@ def test_library_exports_every_symbol_of_the_blocks_header():
     assert lib.lib().fh_blocks_abi_version() == lib.BLOCKS_ABI_VERSION
 
 
+# As ABI_DECLARATIONS of test_api.py: the declarations of a version of this header.
+BLOCKS_DECLARATIONS = (1, "1b65722b168f7dcb")
+
+
+def test_blocks_version_is_raised_with_the_declarations():
+    from femtotron_amd import _lib
+    text = _header()
+    version = int(re.search(r"#define FH_BLOCKS_ABI_VERSION (\d+)", text).group(1))
+    text = re.sub(r"#define FH_BLOCKS_ABI_VERSION \d+", "", text)
+    digest = hashlib.sha256(re.sub(r"\s+", "", text).encode()).hexdigest()[:16]
+    assert (version, digest) == BLOCKS_DECLARATIONS, "declarations changed: raise FH_BLOCKS_ABI_VERSION and record both"
+    assert _lib.BLOCKS_ABI_VERSION == version
+
+
+def test_a_library_without_the_block_operators_is_refused(tmp_path, monkeypatch):
+    """One built before them (its own version right) says to rebuild, and is not bound."""
+    import subprocess
+
+    lib = _lib()
+    src = tmp_path / "old.c"
+    src.write_text("int fh_abi_version(void) { return %d; }" % lib.ABI_VERSION)
+    so = tmp_path / "old.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(so)], check=True)
+    monkeypatch.setattr(lib, "LIB_PATH", so)
+    monkeypatch.setattr(lib, "_lib", None)
+    with pytest.raises(lib.FemtoHipError, match="rebuild"):
+        lib.lib()
+
+
 def test_packed_calls_are_refused_on_the_host():
     lib = _lib()
     L = lib.lib()

@@ -130,13 +130,26 @@ def _turn(op, q, k, positions, inv_freq, how):
 def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
                  head_dim: int, rot_dim: int | None = None, offset: int = 0, layout: str = "half",
                  factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """q and k [..., heads * head_dim] (k may be None, their head counts may differ; column
-    views of a packed projection are read in place) with dims [offset, offset + rot_dim) of
-    each head turned by positions * inv_freq, cos and sin times factor; differentiable in q
-    and k.  positions: int64, one a token in order, or one a position of sequences of equal
-    length (any shape of that many); inv_freq, factor: ``rotary_frequencies``; layout:
-    pairs (i, i + rot_dim / 2), "half", or (2i, 2i + 1), "interleaved"."""
-    how = dict(head_dim=head_dim, rot_dim=rot_dim, offset=offset, layout=layout, factor=factor)
+    """q and k, [tokens, heads * head_dim] or [batch, seq, heads * head_dim] (k may be None,
+    their head counts may differ; column views of a packed projection are read in place),
+    with dims [offset, offset + rot_dim) of each head turned by positions * inv_freq, cos
+    and sin times factor; differentiable in q and k.
+
+    positions: int64 of any shape, one a token in order, or one a position of sequences of
+    equal length (seq of them; of [tokens, ...] a divisor of tokens); inv_freq, factor:
+    ``rotary_frequencies``; layout: pairs (i, i + rot_dim / 2), "half", or (2i, 2i + 1),
+    "interleaved"."""
+    n_positions = positions.numel()
+    for t, n in ((q, "q"), (k, "k")):
+        if t is None:
+            continue
+        if t.dim() not in (2, 3):
+            raise ValueError(f"apply_rotary: {n} must be [tokens, heads * head_dim] or [batch, seq, heads * head_dim] "
+                             f"(heads and head_dim in one dim), got {tuple(t.shape)}")
+        if t.dim() == 3 and n_positions not in (t.shape[1], t.shape[0] * t.shape[1]):
+            raise ValueError(f"apply_rotary: {n_positions} positions are neither one a token nor one a position of "
+                             f"{n} {tuple(t.shape)}")
+    how = dict(head_dim=head_dim, rot_dim=rot_dim, offset=offset, layout=layout, factor=float(factor))
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
         return RotaryFunction.apply(q, k, positions, inv_freq, how)

@@ -202,6 +202,8 @@ def test_refusals():
         block_norms(x[:, :60].contiguous(), x[:, :60].contiguous(), w[:60])
     with pytest.raises(ValueError, match="rstd_post"):
         ops.block_norms_bwd(x, x, x, x, w, w, rstd_pre=torch.ones(4, device=DEV))
+    with pytest.raises(TypeError, match="gate"):
+        block_norms(x, x, w, scale=torch.ones((), device=DEV, requires_grad=True))
     with pytest.raises(ValueError, match="needs dy"):
         ops.block_norms_bwd(x, None, x, x, None, w, rstd_pre=torch.ones(4, device=DEV))
 

@@ -187,6 +187,25 @@ def test_refusals():
     ops.rotary_fwd(both[:, :128], None, pos, f, head_dim=64, out=(both[:, 128:], None))  # beside it
 
 
+def test_heads_in_a_dim_of_their_own_are_refused():
+    """[batch, seq, heads, head_dim] and [tokens, heads, head_dim] would give heads for tokens."""
+    from femtotron_amd import apply_rotary
+    f, how = _freq(32), dict(head_dim=32)
+    q = torch.zeros(2, 6, 4, 32, device=DEV)
+    with pytest.raises(ValueError, match="in one dim"):
+        apply_rotary(q, None, torch.arange(6, device=DEV), f, **how)
+    with pytest.raises(ValueError, match="neither"):
+        apply_rotary(q[0], None, torch.arange(6, device=DEV), f, **how)
+    with pytest.raises(ValueError, match="in one dim"):
+        apply_rotary(q[0, 0, 0], None, torch.arange(1, device=DEV), f, **how)
+    x = randn((2, 6, 128), 18).to(DEV)
+    pos = torch.randint(0, 900, (2, 6), generator=torch.Generator().manual_seed(3)).to(DEV)
+    a, _ = apply_rotary(x, None, pos, f, **how)
+    b, _ = apply_rotary(x.view(12, 128), None, pos.view(-1), f, **how)
+    c = torch.cat([apply_rotary(x[i:i + 1], None, pos[i], f, **how)[0] for i in range(2)])
+    assert torch.equal(a.view(12, 128), b) and torch.equal(a, c)
+
+
 def test_offsets_past_32_bits():
     """More than 2^32 elements: the last rows equal those turned alone."""
     ops = _ops()

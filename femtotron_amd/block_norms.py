@@ -22,31 +22,31 @@ class BlockNormsFunction(torch.autograd.Function):
     """Saved: a, h, the vectors and the gate, and two fp32 values a row."""
 
     @staticmethod
-    def forward(ctx, x, a, w_post, w_pre, gate, scale, eps):
-        rows = x.numel() // max(x.size(-1), 1)
+    def forward(ctx, args, x, a, w_post, w_pre, gate, scale, eps):
+        rows = args[2]
         rstd_post = None if w_post is None else x.new_empty(rows, dtype=torch.float32)
         rstd_pre = None if w_pre is None else x.new_empty(rows, dtype=torch.float32)
-        h, y = ops.block_norms_fwd(x, a, w_post, w_pre, eps, gate=gate, scale=scale, rstd_post=rstd_post,
-                                   rstd_pre=rstd_pre)
-        ctx.save_for_backward(a if w_post is not None or gate is not None else None, None if w_pre is None else h, w_post,
+        h, y = ops.block_norms_fwd_checked(args, x, a, w_post, w_pre, gate, scale, eps, rstd_post, rstd_pre)
+        ctx.save_for_backward(None if w_pre is None else h, a if w_post is not None or gate is not None else None, w_post,
                               w_pre, gate, rstd_post, rstd_pre)
-        ctx.scale = scale
+        ctx.args, ctx.scale = args, scale
         ctx.set_materialize_grads(False)
         return h, y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dy):
-        a, h, w_post, w_pre, gate, rstd_post, rstd_pre = ctx.saved_tensors
         if dh is None and dy is None:
-            return (None,) * 7
+            return (None,) * 8
+        h, a, w_post, w_pre, gate, rstd_post, rstd_pre = ctx.saved_tensors
         dh, dy = ops.aligned(dh), ops.aligned(dy)
         if dh is None:
             dh = torch.zeros_like(dy)
         if dy is None and w_pre is not None:
             dy = torch.zeros_like(dh)
-        return (*ops.block_norms_bwd(dh, dy, h, a, w_post, w_pre, gate=gate, scale=ctx.scale, rstd_post=rstd_post,
-                                     rstd_pre=rstd_pre), None, None)
+        # autograd hands gradients in of the outputs' shape, dtype and device
+        return (None, *ops.block_norms_bwd_checked(ctx.args, dh, dy, h, a, w_post, w_pre, gate, ctx.scale, rstd_post,
+                                                   rstd_pre), None, None)
 
 
 def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = None,
@@ -67,6 +67,6 @@ def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = 
         gate = gate.reshape(-1)
     tensors = tuple(map(ops.aligned, (x, a, w_post, w_pre, gate)))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return BlockNormsFunction.apply(*tensors, float(scale), float(eps))
+        return BlockNormsFunction.apply(ops.block_norms_check("block_norms", *tensors), *tensors, float(scale), float(eps))
     x, a, w_post, w_pre, gate = tensors
     return ops.block_norms_fwd(x, a, w_post, w_pre, float(eps), gate=gate, scale=float(scale))

@@ -86,11 +86,13 @@ def _launch(name: str, t: torch.Tensor, *args) -> None:
     """Calls an entry point on the current stream of t's device, with that device
     the current one (the default stream's handle is 0 on every device)."""
     index = t.get_device()
-    if torch._C._cuda_getDevice() == index:
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        return
+    status = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def aligned(t: torch.Tensor | None) -> torch.Tensor | None:
@@ -358,10 +360,9 @@ def rope_bwd_(dqk: torch.Tensor, n_heads: int, head_dim: int, seq_len: int, cos:
 
 
 # --------------------------------------------------- norms around a block
-def _block_norms_args(name: str, like: torch.Tensor, w_post, w_pre, gate) -> tuple[int, int, int, int]:
+def _block_norms_shapes(name: str, like: torch.Tensor, w_post, w_pre, gate) -> tuple[int, int, int, int]:
     """(dtype code, gate_per_token, rows, cols) of block norms over `like`'s rows, checked."""
     cols = like.size(-1) if like.dim() else 0
-    rows = like.numel() // max(cols, 1)
     if w_post is None and w_pre is None:
         raise ValueError(f"{name}: at least one of w_post and w_pre is needed")
     for w, n in ((w_post, "w_post"), (w_pre, "w_pre")):
@@ -373,7 +374,16 @@ def _block_norms_args(name: str, like: torch.Tensor, w_post, w_pre, gate) -> tup
         if (per_token and gate.shape != like.shape) or not gate.is_contiguous():
             raise ValueError(f"{name}: gate must be contiguous, of shape [{cols}] or {tuple(like.shape)}, got "
                              f"{tuple(gate.shape)}")
-    return _dtype_code(like), per_token, rows, cols
+    return _dtype_code(like), per_token, like.numel() // max(cols, 1), cols
+
+
+def block_norms_check(name: str, x, a, w_post, w_pre, gate) -> tuple[int, int, int, int]:
+    """_block_norms_shapes of the forward's tensors, all of which are checked."""
+    _alike(x, a, w_post, w_pre, gate)
+    args = _block_norms_shapes(name, x, w_post, w_pre, gate)
+    if not x.is_contiguous() or not a.is_contiguous() or a.shape != x.shape:
+        raise ValueError(f"{name}: x and a must be contiguous, of one shape")
+    return args
 
 
 def block_norms_fwd(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None, w_pre: torch.Tensor | None, eps: float,
@@ -383,11 +393,14 @@ def block_norms_fwd(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | Non
     fp32 between those roundings (fh_block_norms_fwd).  w_post None: a enters as it is;
     w_pre None: no y; gate [cols], of x's shape, or None.  Returns (h, y or None);
     rstd_post and rstd_pre (fp32, one a row) receive what block_norms_bwd reads."""
-    _alike(x, a, w_post, w_pre, gate)
-    dt, per_token, rows, cols = _block_norms_args("block_norms_fwd", x, w_post, w_pre, gate)
-    if not x.is_contiguous() or not a.is_contiguous() or a.shape != x.shape:
-        raise ValueError("block_norms_fwd: x and a must be contiguous, of one shape")
-    _row_stats("block_norms_fwd", x, rows, rstd_post, rstd_pre)
+    args = block_norms_check("block_norms_fwd", x, a, w_post, w_pre, gate)
+    _row_stats("block_norms_fwd", x, args[2], rstd_post, rstd_pre)
+    return block_norms_fwd_checked(args, x, a, w_post, w_pre, gate, scale, eps, rstd_post, rstd_pre)
+
+
+def block_norms_fwd_checked(args: tuple, x, a, w_post, w_pre, gate, scale, eps, rstd_post, rstd_pre):
+    """block_norms_fwd of tensors that are known to fit; args: block_norms_check's."""
+    dt, per_token, rows, cols = args
     h = torch.empty_like(x)
     y = None if w_pre is None else torch.empty_like(x)
     _launch("fh_block_norms_fwd", x, dt, _ptr(x), _ptr(a), _ptr(w_post), _ptr(w_pre), _ptr(gate), per_token, scale, _ptr(h),
@@ -402,7 +415,7 @@ def block_norms_bwd(dh: torch.Tensor, dy: torch.Tensor | None, h: torch.Tensor |
     did not have.  dy, h and rstd_pre go with w_pre, rstd_post with w_post, a with
     w_post or a gate."""
     _alike(dh, dy, h, a, w_post, w_pre, gate)
-    dt, per_token, rows, cols = _block_norms_args("block_norms_bwd", dh, w_post, w_pre, gate)
+    args = _block_norms_shapes("block_norms_bwd", dh, w_post, w_pre, gate)
     if w_pre is not None and (dy is None or h is None or rstd_pre is None):
         raise ValueError("block_norms_bwd: w_pre needs dy, h and rstd_pre")
     if w_post is not None and rstd_post is None:
@@ -412,7 +425,13 @@ def block_norms_bwd(dh: torch.Tensor, dy: torch.Tensor | None, h: torch.Tensor |
     for t, n in ((dh, "dh"), (dy, "dy"), (h, "h"), (a, "a")):
         if t is not None and (not t.is_contiguous() or t.shape != dh.shape):
             raise ValueError(f"block_norms_bwd: {n} must be contiguous, of dh's shape")
-    _row_stats("block_norms_bwd", dh, rows, rstd_post, rstd_pre)
+    _row_stats("block_norms_bwd", dh, args[2], rstd_post, rstd_pre)
+    return block_norms_bwd_checked(args, dh, dy, h, a, w_post, w_pre, gate, scale, rstd_post, rstd_pre)
+
+
+def block_norms_bwd_checked(args: tuple, dh, dy, h, a, w_post, w_pre, gate, scale, rstd_post, rstd_pre):
+    """block_norms_bwd of tensors that are known to fit; args: block_norms_check's."""
+    dt, per_token, rows, cols = args
     dx, da = torch.empty_like(dh), torch.empty_like(dh)
     dw_post, dw_pre, dgate = (None if t is None else torch.empty_like(t) for t in (w_post, w_pre, gate))
     nbytes = _lib.lib().fh_block_norms_bwd_workspace_size(rows, cols)

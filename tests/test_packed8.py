@@ -123,6 +123,7 @@ def test_off_the_gpu_the_input_is_kept_as_it_is():
 def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
     """Where the tensors' device is not the current one, the call is made with it current."""
     from contextlib import contextmanager
+    from types import SimpleNamespace
 
     from femtotron_amd import ops
     lib = _lib()
@@ -137,7 +138,7 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
     monkeypatch.setattr(torch.cuda, "device", device)
-    monkeypatch.setattr(lib, "call", lambda name, *a: seen.append((current[0], a)))
+    monkeypatch.setattr(lib, "lib", lambda: SimpleNamespace(fh_x=lambda *a: seen.append((current[0], a)) or 0))
 
     class T:
         def __init__(self, i):

@@ -70,17 +70,24 @@ constexpr int kWavesPerBlock = 4;  // 256 threads
 // (two input rows): 45.2 -> 43.1 us at T = 16384, H = 2048 and 50.5 -> 48.8 us
 // at T = 8192, H = 4096; the one-input form measured no gain from it.
 // PACK: x also goes out in 8 bits (a format of fh_pack8.hpp; kNoPack: it does not).
-template <typename T, typename XS, int NV, bool ADD, bool PIPE, int PACK, bool RND>
+// WPR waves share a row, each NV chunks a lane; with more than one a block's waves
+// go through its steps together (rows behind the last one are computed on zeros).
+template <typename T, typename XS, int NV, int WPR, bool ADD, bool PIPE, int PACK, bool RND>
 __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
     const typename XS::Item* __restrict__ x, const uint8_t* __restrict__ xe, const T* __restrict__ a,
     const T* __restrict__ w, T* __restrict__ h, T* __restrict__ y, float* __restrict__ rstd,
     uint8_t* __restrict__ codes, uint8_t* __restrict__ exps, int64_t rows, int cols, float eps) {
   using Raw = typename Elem<T>::Raw;
   using XRaw = typename XS::Raw;
-  const int lane = threadIdx.x & (kWave - 1);
-  int64_t row = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
-  if (row >= rows) return;  // uniform per wave
+  constexpr int RPB = kWavesPerBlock / WPR;  // rows of a block's step
+  [[maybe_unused]] __shared__ float red[2][kWavesPerBlock];  // [step parity][wave]
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int rsub = wave / WPR, slice = wave % WPR;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + rsub;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * RPB;
+  if (WPR == 1 && row >= rows) return;  // uniform per wave
+  auto col = [&](int i) { return ((slice * NV + i) * kWave + lane) * 8; };
+  auto in = [&](int c, int64_t rr) { return c < cols && (WPR == 1 || rr < rows); };
 
   XRaw xn[NV];
   Raw wr[NV];
@@ -89,8 +96,8 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
     const int64_t base = rr * cols;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * kWave + lane) * 8;
-      if (c < cols) {
+      const int c = col(i);
+      if (in(c, rr)) {
         xn[i] = XS::load(x, xe, rr, cols, c);
         if constexpr (ADD) an[i] = Elem<T>::ldraw(a + base + c);
       }
@@ -99,17 +106,18 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
   load_row(row);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * kWave + lane) * 8;
+    const int c = col(i);
     if (c < cols) wr[i] = Elem<T>::ldraw(w + c);
   }
+  [[maybe_unused]] int par = 0;
   // Normalises row rr from its loaded chunks (xr, and ar with ADD).
   auto norm_row = [&](int64_t rr, XRaw* xr, [[maybe_unused]] Raw* ar) {
     const int64_t base = rr * cols;
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * kWave + lane) * 8;
-      if (c < cols) {
+      const int c = col(i);
+      if (in(c, rr)) {
         float v[8];
         XS::unpack(xr[i], v);
         if constexpr (ADD) {  // h = to_dtype(x + a), kept packed (in a's place) for the normalisation
@@ -125,16 +133,24 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
       }
       if constexpr (PACK != kNoPack) {
         float v[8] = {};
-        if (c < cols) XS::unpack(xr[i], v);
-        pack8_store<PACK>(v, codes, exps, rr, cols, c);
+        if (in(c, rr)) XS::unpack(xr[i], v);
+        pack8_store<PACK>(v, codes, exps, rr, in(c, rr) ? cols : 0, c);
       }
     }
     ss = wave_sum(ss);
+    if constexpr (WPR > 1) {
+      if (lane == 0) red[par][wave] = ss;
+      __syncthreads();
+      ss = 0.f;
+#pragma unroll
+      for (int s = 0; s < WPR; ++s) ss += red[par][rsub * WPR + s];
+      par ^= 1;
+    }
     const float r = rsqrtf(ss / static_cast<float>(cols) + eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * kWave + lane) * 8;
-      if (c < cols) {
+      const int c = col(i);
+      if (in(c, rr)) {
         float v[8], wv[8], o[8];
         if constexpr (ADD) Elem<T>::unpack(ar[i], v);
         else XS::unpack(xr[i], v);
@@ -144,12 +160,12 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
         Elem<T>::store8(y + base + c, o);
       }
     }
-    if (rstd != nullptr && lane == 0) rstd[rr] = r;
+    if (rstd != nullptr && lane == 0 && slice == 0 && in(0, rr)) rstd[rr] = r;
   };
   if constexpr (!PIPE) {
     norm_row(row, xn, an);
   } else {
-    for (; row < rows; row += stride) {  // uniform per wave
+    for (; row - rsub * (WPR > 1) < rows; row += stride) {  // uniform per wave, and per block where waves share rows
       XRaw xr[NV];
       [[maybe_unused]] Raw ar[NV];
 #pragma unroll
@@ -410,13 +426,22 @@ template <typename T, typename XS, int PACK, int NV, bool RND = true>
 void launch_fwd(const void* x, const void* a, const void* w, void* h, void* y, float* rstd, const void* codes,
                 const uint8_t* exps, int64_t rows, int cols, float eps, hipStream_t s) {
   using Item = typename XS::Item;
-  const int64_t need = (rows + kWavesPerBlock - 1) / kWavesPerBlock;
+  constexpr int kRaw = sizeof(typename Elem<T>::Raw);
+  constexpr bool kBf16 = kRaw == 16;
+  // A call that does not promise fh_rmsnorm_fwd's bits (its order of a row's sum)
+  // gives a wave at most 4096 bf16 or 2048 fp32 columns.  One and more waves a row,
+  // us: 8192 x 8192 bf16, packed x 65.1 and 35.5, its add + norm 117 and 92, packing
+  // 71.7 and 66.8; 4096 x 8192 25.2 and 18.9, 48.9 and 41.3, 37.7 and 34.0; fp32 8192
+  // x 4096 34.1 and 28.5, 105 and 89, 56.8 and 51.6.
+  constexpr int WPR = !RND && NV * kRaw > 128 ? NV * kRaw / 128 : 1, NVW = NV / WPR;
+  constexpr int kRows = kWavesPerBlock / WPR;
+  const int64_t need = (rows + kRows - 1) / kRows;
   const Item* const xp = static_cast<const Item*>(XS::kPacked ? codes : x);
   auto* const co = const_cast<uint8_t*>(static_cast<const uint8_t*>(codes));
   auto* const eo = const_cast<uint8_t*>(exps);
   auto go = [&](auto add, auto pipe, int64_t blocks) {
     if constexpr (PACK == kNoPack || !add())
-      hipLaunchKernelGGL((k_rmsnorm_fwd<T, XS, NV, add(), pipe(), PACK, RND>), dim3(static_cast<unsigned>(blocks)),
+      hipLaunchKernelGGL((k_rmsnorm_fwd<T, XS, NVW, WPR, add(), pipe(), PACK, RND>), dim3(static_cast<unsigned>(blocks)),
                          dim3(256), 0, s, xp, exps, static_cast<const T*>(a), static_cast<const T*>(w),
                          static_cast<T*>(h), static_cast<T*>(y), rstd, co, eo, rows, cols, eps);
   };
@@ -425,13 +450,13 @@ void launch_fwd(const void* x, const void* a, const void* w, void* h, void* y, f
   if (a != nullptr) {
     // add+RMSNorm: pipelined over a capped grid where the two rows of x and a
     // in flight fit the registers (bf16 up to 4096 columns, fp32 up to 2048)
-    constexpr bool kPipe = NV * sizeof(typename Elem<T>::Raw) <= 128;
+    constexpr bool kPipe = NVW * kRaw <= 128;
     go(yes, std::bool_constant<kPipe>{}, kPipe && need > kFwdPipeBlocks ? kFwdPipeBlocks : need);
-  } else if (XS::kPacked && NV == 4 && sizeof(typename Elem<T>::Raw) == 16 && need > kFwdPipeBlocks8) {
+  } else if (XS::kPacked && NV == 4 && kBf16 && need > kFwdPipeBlocks8) {
     // packed x, 1025-2048 bf16 columns: 19.2 -> 17.1 us at T = 16384, H = 2048
     // (half the loads of a bf16 row in flight a wave; at 1024 columns no gain)
     go(no, yes, kFwdPipeBlocks8);
-  } else if (NV == 8 && sizeof(typename Elem<T>::Raw) == 16 && need > kFwdPipeBlocks1) {
+  } else if (((NVW == 8 && kBf16) || WPR > 1) && need > kFwdPipeBlocks1) {
     // one input, 2049-4096 bf16 columns: pipelined over a capped grid (kernel
     // time 15.3 -> 14.1 us at T = 4096, 26.1 -> 23.7 us at 8192, H = 4096)
     go(no, yes, kFwdPipeBlocks1);
@@ -501,8 +526,11 @@ void launch_bwd(const void* dy, const void* x, const uint8_t* xe, const void* w,
                 float eps, hipStream_t s) {
   auto go = [&](auto res) {
     // The rows' sums are added in the split's order: where a call promises
-    // fh_rmsnorm_bwd's bits it takes fh_rmsnorm_bwd's split.
-    using SP = std::conditional_t<RND, BwdSplit<NV, res()>, Bwd8Split<NV, res()>>;
+    // fh_rmsnorm_bwd's bits it takes fh_rmsnorm_bwd's split.  So do fp32 rows of up to
+    // 2048 columns (with the residual gradient 42.6 us against 44.5 at 8192 x 2048;
+    // 89.2 against 78.1 at 8192 x 4096).
+    constexpr bool kStock = RND || (NV <= 4 && sizeof(typename Elem<T>::Raw) > 16);
+    using SP = std::conditional_t<kStock, BwdSplit<NV, res()>, Bwd8Split<NV, res()>>;
     const int blocks = bwd_blocks(rows, SP::RPB, SP::kBlocks);
     if (rstd != nullptr) launch_bwd_k<T, XS, SP, res(), true, RND>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);
     else launch_bwd_k<T, XS, SP, res(), false, RND>(dy, x, xe, w, rstd, dres, dx, part, rows, cols, eps, blocks, s);

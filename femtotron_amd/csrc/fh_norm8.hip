@@ -61,17 +61,19 @@ int check_rows(fh_dtype dt, int64_t rows, int64_t cols) {
   return FH_OK;
 }
 
-// f(element type tag, format) for a checked dtype and format; with `rounding`,
-// f(tag, format, whether the normalised value is rounded: in fp32 it is either way).
+// f(element type tag, format, std::bool_constant<rounding>) for a checked dtype and format.
 template <typename F>
 void with_types(fh_dtype dt, fh_fmt8 fmt, bool rounding, F&& f) {
   auto go = [&](auto tag, auto rnd) {
     if (fmt == FH_INT8) f(tag, std::integral_constant<int, kFmtInt8>{}, rnd);
     else f(tag, std::integral_constant<int, kFmtE4M3>{}, rnd);
   };
-  if (dt != FH_BF16) go(float{}, std::true_type{});
-  else if (rounding) go(uint16_t{}, std::true_type{});
-  else go(uint16_t{}, std::false_type{});
+  auto rnd = [&](auto tag) {
+    if (rounding) go(tag, std::true_type{});
+    else go(tag, std::false_type{});
+  };
+  if (dt == FH_BF16) rnd(uint16_t{});
+  else rnd(float{});
 }
 
 // Grid of a pack or unpack: FH_ERR_INVALID where it would pass the largest.

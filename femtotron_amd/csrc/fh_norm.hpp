@@ -30,8 +30,10 @@ struct RowsT {
   static constexpr bool kPacked = false;
   using Item = T;
   using Raw = typename Elem<T>::Raw;
-  __device__ __forceinline__ static Raw load(const T* x, const uint8_t*, int64_t row, int cols, int c) {
-    return Elem<T>::ldraw(x + row * cols + c);
+  // Elements c..c+7 of the row that starts at base (and, kept in 8 bits, its
+  // exponents at ebase): both computed once a row, outside the column tests.
+  __device__ __forceinline__ static Raw load(const T* x, const uint8_t*, int64_t base, int64_t, int c) {
+    return Elem<T>::ldraw(x + base + c);
   }
   __device__ __forceinline__ static void unpack(const Raw& q, float v[8]) { Elem<T>::unpack(q, v); }
 };
@@ -42,8 +44,8 @@ struct Rows8 {
   static constexpr bool kPacked = true;
   using Item = uint8_t;
   using Raw = Raw8;
-  __device__ __forceinline__ static Raw load(const uint8_t* x, const uint8_t* xe, int64_t row, int cols, int c) {
-    return load8_codes(x, xe, row, cols, c);
+  __device__ __forceinline__ static Raw load(const uint8_t* x, const uint8_t* xe, int64_t base, int64_t ebase, int c) {
+    return load8_codes(x + base, xe + ebase, c);
   }
   __device__ __forceinline__ static void unpack(const Raw& q, float v[8]) { unpack8<FMT>(q, v); }
 };
@@ -70,13 +72,16 @@ constexpr int kWavesPerBlock = 4;  // 256 threads
 // (two input rows): 45.2 -> 43.1 us at T = 16384, H = 2048 and 50.5 -> 48.8 us
 // at T = 8192, H = 4096; the one-input form measured no gain from it.
 // PACK: x also goes out in 8 bits (a format of fh_pack8.hpp; kNoPack: it does not).
+// The arguments of packed calls alone stand last: the others fill one 64-byte line,
+// and in the second one rows and cols cost every wave a wait (add + norm of 8192 x
+// 4096 47.2 us, 48.2 with them there).
 // WPR waves share a row, each NV chunks a lane; with more than one a block's waves
 // go through its steps together (rows behind the last one are computed on zeros).
 template <typename T, typename XS, int NV, int WPR, bool ADD, bool PIPE, int PACK, bool RND>
 __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
-    const typename XS::Item* __restrict__ x, const uint8_t* __restrict__ xe, const T* __restrict__ a,
-    const T* __restrict__ w, T* __restrict__ h, T* __restrict__ y, float* __restrict__ rstd,
-    uint8_t* __restrict__ codes, uint8_t* __restrict__ exps, int64_t rows, int cols, float eps) {
+    const typename XS::Item* __restrict__ x, const T* __restrict__ a, const T* __restrict__ w, T* __restrict__ h,
+    T* __restrict__ y, float* __restrict__ rstd, int64_t rows, int cols, float eps, const uint8_t* __restrict__ xe,
+    uint8_t* __restrict__ codes, uint8_t* __restrict__ exps) {
   using Raw = typename Elem<T>::Raw;
   using XRaw = typename XS::Raw;
   constexpr int RPB = kWavesPerBlock / WPR;  // rows of a block's step
@@ -94,11 +99,12 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
   [[maybe_unused]] Raw an[NV];
   auto load_row = [&](int64_t rr) {
     const int64_t base = rr * cols;
+    [[maybe_unused]] const int64_t ebase = XS::kPacked ? rr * blocks8(cols) : 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = col(i);
       if (in(c, rr)) {
-        xn[i] = XS::load(x, xe, rr, cols, c);
+        xn[i] = XS::load(x, xe, base, ebase, c);
         if constexpr (ADD) an[i] = Elem<T>::ldraw(a + base + c);
       }
     }
@@ -113,6 +119,7 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
   // Normalises row rr from its loaded chunks (xr, and ar with ADD).
   auto norm_row = [&](int64_t rr, XRaw* xr, [[maybe_unused]] Raw* ar) {
     const int64_t base = rr * cols;
+    [[maybe_unused]] const int64_t ebase = PACK != kNoPack ? rr * blocks8(cols) : 0;
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -120,13 +127,17 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
       if (in(c, rr)) {
         float v[8];
         XS::unpack(xr[i], v);
-        if constexpr (ADD) {  // h = to_dtype(x + a), kept packed (in a's place) for the normalisation
+        if constexpr (ADD) {  // h = to_dtype(x + a), kept packed (in x's place, or a's) for the normalisation
           float b[8];
           Elem<T>::unpack(ar[i], b);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = Elem<T>::rnd(v[j] + b[j]);
-          ar[i] = Elem<T>::pack(v);
-          Elem<T>::straw(h + base + c, ar[i]);
+          auto& hr = [&]() -> Raw& {
+            if constexpr (XS::kPacked) return ar[i];
+            else return xr[i];
+          }();
+          hr = Elem<T>::pack(v);
+          Elem<T>::straw(h + base + c, hr);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
@@ -134,7 +145,7 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
       if constexpr (PACK != kNoPack) {
         float v[8] = {};
         if (in(c, rr)) XS::unpack(xr[i], v);
-        pack8_store<PACK>(v, codes, exps, rr, in(c, rr) ? cols : 0, c);
+        pack8_store<PACK>(v, codes + base, exps + ebase, in(c, rr), c);
       }
     }
     ss = wave_sum(ss);
@@ -152,7 +163,7 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
       const int c = col(i);
       if (in(c, rr)) {
         float v[8], wv[8], o[8];
-        if constexpr (ADD) Elem<T>::unpack(ar[i], v);
+        if constexpr (ADD && XS::kPacked) Elem<T>::unpack(ar[i], v);
         else XS::unpack(xr[i], v);
         Elem<T>::unpack(wr[i], wv);
 #pragma unroll
@@ -160,7 +171,7 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
         Elem<T>::store8(y + base + c, o);
       }
     }
-    if (rstd != nullptr && lane == 0 && slice == 0 && in(0, rr)) rstd[rr] = r;
+    if (rstd != nullptr && lane == 0 && slice == 0 && (WPR == 1 || rr < rows)) rstd[rr] = r;
   };
   if constexpr (!PIPE) {
     norm_row(row, xn, an);
@@ -200,10 +211,9 @@ __global__ __launch_bounds__(256) void k_rmsnorm_fwd(
 template <typename T, typename XS, int NVW, int WPR, int NWB, bool RES, bool HAVE_RSTD, bool PF, bool RND,
           bool STREAM>
 __global__ __launch_bounds__(64 * NWB) void k_rmsnorm_bwd(
-    const T* __restrict__ dy, const typename XS::Item* __restrict__ x, const uint8_t* __restrict__ xe,
-    const T* __restrict__ w, const float* __restrict__ rstd, const T* __restrict__ dres,
-    T* __restrict__ dx, float* __restrict__ part, int64_t rows, int cols,
-    float eps) {
+    const T* __restrict__ dy, const typename XS::Item* __restrict__ x, const T* __restrict__ w,
+    const float* __restrict__ rstd, const T* __restrict__ dres, T* __restrict__ dx, float* __restrict__ part,
+    int64_t rows, int cols, float eps, const uint8_t* __restrict__ xe) {
   using Raw = typename Elem<T>::Raw;
   using XRaw = typename XS::Raw;
   constexpr int RPB = NWB / WPR;  // rows per block step (NWB waves per block)
@@ -234,11 +244,12 @@ __global__ __launch_bounds__(64 * NWB) void k_rmsnorm_bwd(
   auto load_row = [&](int64_t row) {
     if (row >= rows) return;
     const int64_t base = row * cols;
+    [[maybe_unused]] const int64_t ebase = XS::kPacked ? row * blocks8(cols) : 0;
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
       const int c = col(i);
       if (c < cols) {
-        xn[i] = XS::load(x, xe, row, cols, c);
+        xn[i] = XS::load(x, xe, base, ebase, c);
         gn[i] = load_if<T, STREAM>(dy + base + c);
         if constexpr (RES) rn[i] = load_if<T, STREAM>(dres + base + c);
       }
@@ -442,8 +453,8 @@ void launch_fwd(const void* x, const void* a, const void* w, void* h, void* y, f
   auto go = [&](auto add, auto pipe, int64_t blocks) {
     if constexpr (PACK == kNoPack || !add())
       hipLaunchKernelGGL((k_rmsnorm_fwd<T, XS, NVW, WPR, add(), pipe(), PACK, RND>), dim3(static_cast<unsigned>(blocks)),
-                         dim3(256), 0, s, xp, exps, static_cast<const T*>(a), static_cast<const T*>(w),
-                         static_cast<T*>(h), static_cast<T*>(y), rstd, co, eo, rows, cols, eps);
+                         dim3(256), 0, s, xp, static_cast<const T*>(a), static_cast<const T*>(w), static_cast<T*>(h),
+                         static_cast<T*>(y), rstd, rows, cols, eps, exps, co, eo);
   };
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
@@ -516,8 +527,8 @@ void launch_bwd_k(const void* dy, const void* x, const uint8_t* xe, const void* 
                   int blocks, hipStream_t s) {
   hipLaunchKernelGGL((k_rmsnorm_bwd<T, XS, SP::NVW, SP::WPR, SP::NWB, RES, HR, SP::PF, RND, SP::STREAM>), dim3(blocks),
                      dim3(64 * SP::NWB), static_cast<size_t>(cols) * sizeof(float), s, static_cast<const T*>(dy),
-                     static_cast<const typename XS::Item*>(x), xe, static_cast<const T*>(w), rstd,
-                     static_cast<const T*>(dres), static_cast<T*>(dx), part, rows, cols, eps);
+                     static_cast<const typename XS::Item*>(x), static_cast<const T*>(w), rstd,
+                     static_cast<const T*>(dres), static_cast<T*>(dx), part, rows, cols, eps, xe);
 }
 
 template <typename T, typename XS, int NV, bool RND = true>

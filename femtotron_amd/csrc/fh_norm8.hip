@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, uint8_t*
   const bool in = row < rows && c < cols;
   float v[8] = {};
   if (in) Elem<T>::unpack(Elem<T>::ldraw_stream(x + row * cols + c), v);
-  pack8_store<FMT>(v, codes, exps, row, in ? cols : 0, c);
+  pack8_store<FMT>(v, codes + row * cols, exps + row * blocks8(cols), in, c);
 }
 
 template <typename T, int FMT>
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void k_unpack8(const uint8_t* __restrict__ cod
   row_chunk(idx, cpr, fd, row, c);
   if (row >= rows || c >= cols) return;
   float v[8];
-  unpack8<FMT>(load8_codes(codes, exps, row, cols, c), v);
+  unpack8<FMT>(load8_codes(codes + row * cols, exps + row * blocks8(cols), c), v);
   Elem<T>::store8(x + row * cols + c, v);
 }
 

@@ -37,12 +37,12 @@ struct Raw8 {
   uint32_t e;
 };
 
-// Codes c..c+7 of a row (c % 8 == 0, so within one block); cols % 8 == 0 keeps
-// them 8-byte aligned.
-__device__ __forceinline__ Raw8 load8_codes(const uint8_t* codes, const uint8_t* exps, int64_t row, int cols, int c) {
+// Codes c..c+7 of the row at codes and exps (c % 8 == 0, so within one block); a
+// row is a multiple of 8 codes, which keeps them 8-byte aligned.
+__device__ __forceinline__ Raw8 load8_codes(const uint8_t* codes, const uint8_t* exps, int c) {
   Raw8 r;
-  r.c = *reinterpret_cast<const uint2*>(codes + row * cols + c);
-  r.e = exps[row * blocks8(cols) + (c / kBlock8)];
+  r.c = *reinterpret_cast<const uint2*>(codes + c);
+  r.e = exps[c / kBlock8];
   return r;
 }
 
@@ -114,16 +114,15 @@ __device__ __forceinline__ uint2 codes8(const float v[8], uint32_t e) {
   return make_uint2(bad ? 0u : w[0], bad ? 0u : w[1]);
 }
 
-// Packs elements c..c+7 of a row; the four lanes of a quad hold one block
-// (lane l of a wave at c = 8 l modulo 512) and all call this, those with
-// c >= cols with zeros, of which nothing is stored.
+// Packs elements c..c+7 of the row at codes and exps; the four lanes of a quad hold
+// one block (lane l of a wave at c = 8 l modulo 512) and all call this, those behind
+// the row's end (!in) with zeros, of which nothing is stored.
 template <int FMT>
-__device__ __forceinline__ void pack8_store(const float v[8], uint8_t* codes, uint8_t* exps, int64_t row, int cols,
-                                            int c) {
+__device__ __forceinline__ void pack8_store(const float v[8], uint8_t* codes, uint8_t* exps, bool in, int c) {
   const uint32_t e = exp_byte<FMT>(v);
-  if (c >= cols) return;
-  *reinterpret_cast<uint2*>(codes + row * cols + c) = codes8<FMT>(v, e);
-  if ((c & (kBlock8 - 1)) == 0) exps[row * blocks8(cols) + c / kBlock8] = static_cast<uint8_t>(e);
+  if (!in) return;
+  *reinterpret_cast<uint2*>(codes + c) = codes8<FMT>(v, e);
+  if ((c & (kBlock8 - 1)) == 0) exps[c / kBlock8] = static_cast<uint8_t>(e);
 }
 
 }  // namespace fh

@@ -15,6 +15,10 @@
 // registers between the two reductions.  WPR waves share a row (at most 1024
 // columns each, NVW <= 2 chunks of 8 a lane), which keeps the backward's four
 // rows, three vectors and two sums under 128 registers: four waves a SIMD.
+// 16384 x 2048 bf16 with a channel gate: forward 45.9 us call after call (268 MB,
+// 5.8 TB/s) and 52 with a backward between (5.1), backward 75.5 us (403 MB, 5.3)
+// and its sums 4; a copy runs at 5.4.  Non-temporal stores of h and y or of dx and
+// da cost 4 to 5 us each.
 #include "femtohip_blocks.h"
 #include "fh_common.hpp"
 

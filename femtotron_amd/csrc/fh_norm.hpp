@@ -463,17 +463,22 @@ void launch_fwd(const void* x, const void* a, const void* w, void* h, void* y, f
     // in flight fit the registers (bf16 up to 4096 columns, fp32 up to 2048)
     constexpr bool kPipe = NVW * kRaw <= 128;
     go(yes, std::bool_constant<kPipe>{}, kPipe && need > kFwdPipeBlocks ? kFwdPipeBlocks : need);
-  } else if (XS::kPacked && NV == 4 && kBf16 && need > kFwdPipeBlocks8) {
-    // packed x, 1025-2048 bf16 columns: 19.2 -> 17.1 us at T = 16384, H = 2048
-    // (half the loads of a bf16 row in flight a wave; at 1024 columns no gain)
-    go(no, yes, kFwdPipeBlocks8);
-  } else if (((NVW == 8 && kBf16) || WPR > 1) && need > kFwdPipeBlocks1) {
-    // one input, 2049-4096 bf16 columns: pipelined over a capped grid (kernel
-    // time 15.3 -> 14.1 us at T = 4096, 26.1 -> 23.7 us at 8192, H = 4096)
-    go(no, yes, kFwdPipeBlocks1);
-  } else {
-    go(no, no, need);
+    return;
   }
+  // One input, pipelined over a capped grid: 2049-4096 bf16 columns (kernel time
+  // 15.3 -> 14.1 us at T = 4096, 26.1 -> 23.7 us at 8192, H = 4096) and rows that waves
+  // share; of a packed x also 1025-2048 bf16 columns (19.2 -> 17.1 us at T = 16384,
+  // H = 2048: half the loads of a bf16 row in flight a wave; at 1024 columns no gain).
+  constexpr int64_t kCap = XS::kPacked && NV == 4 && kBf16          ? kFwdPipeBlocks8
+                           : (NVW == 8 && kBf16) || WPR > 1         ? kFwdPipeBlocks1
+                                                                    : 0;
+  if constexpr (kCap > 0) {
+    if (need > kCap) {
+      go(no, yes, kCap);
+      return;
+    }
+  }
+  go(no, no, need);
 }
 
 // Backward row split: WPR waves per row, NVW chunks of 8 per lane, NWB waves

@@ -16,14 +16,22 @@ namespace {
 
 // One thread = 8 elements.  Rows are counted in blocks of 32 (four threads), so
 // that a quad of lanes holds one block also where a row ends inside it: thread
-// -> (row, chunk of 8) over ceil(cols / 32) * 4 chunks a row.
+// -> (row, chunk of 8) over ceil(cols / 32) * 4 chunks a row.  16 elements a thread
+// pack 16384 x 2048 in 17.9 us against 19.5, but unpack them in 18.9 against 16.5 and
+// gain nothing at 32768 x 4096; two or four pieces a thread are slower at most sizes.
 __device__ __forceinline__ void row_chunk(uint32_t idx, int cpr, const FastDiv& fd, int64_t& row, int& c) {
   const uint32_t q = fd.div(idx);
   row = q;
   c = static_cast<int>(idx - q * static_cast<uint32_t>(cpr)) * 8;
 }
 
-template <typename T, int FMT>
+// STREAM: x with non-temporal loads.  Below 128 MiB of x plain ones are faster (an
+// activation was mostly written just before and is still in the 256 MB cache: bf16
+// 4096 x 2048 6.3 us against 7.2, 16384 x 2048 19.5 against 20.7, fp32 8192 x 2048 15.3
+// against 16.5).  From there on x does not stay anyway, and streamed it leaves the
+// codes in the cache for their reader: pack and unpack of bf16 32768 x 2048 68.1 us
+// against 69.6, 32768 x 4096 135 against 144, fp32 16384 x 4096 108 against 136.
+template <typename T, int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, uint8_t* __restrict__ codes,
                                                uint8_t* __restrict__ exps, int64_t rows, int cols, int cpr,
                                                FastDiv fd) {
@@ -33,7 +41,7 @@ __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, uint8_t*
   row_chunk(idx, cpr, fd, row, c);
   const bool in = row < rows && c < cols;
   float v[8] = {};
-  if (in) Elem<T>::unpack(Elem<T>::ldraw_stream(x + row * cols + c), v);
+  if (in) Elem<T>::unpack(load_if<T, STREAM>(x + row * cols + c), v);
   pack8_store<FMT>(v, codes + row * cols, exps + row * blocks8(cols), in, c);
 }
 
@@ -65,19 +73,20 @@ int check_rows(fh_dtype dt, int64_t rows, int64_t cols) {
   return FH_OK;
 }
 
-// f(element type tag, format, std::bool_constant<rounding>) for a checked dtype and format.
+// f(element type tag, format, std::bool_constant<flag>) for a checked dtype and format;
+// the flag is a norm's rounding, or pack's streaming.
 template <typename F>
-void with_types(fh_dtype dt, fh_fmt8 fmt, bool rounding, F&& f) {
-  auto go = [&](auto tag, auto rnd) {
-    if (fmt == FH_INT8) f(tag, std::integral_constant<int, kFmtInt8>{}, rnd);
-    else f(tag, std::integral_constant<int, kFmtE4M3>{}, rnd);
+void with_types(fh_dtype dt, fh_fmt8 fmt, bool flag, F&& f) {
+  auto go = [&](auto tag, auto flg) {
+    if (fmt == FH_INT8) f(tag, std::integral_constant<int, kFmtInt8>{}, flg);
+    else f(tag, std::integral_constant<int, kFmtE4M3>{}, flg);
   };
-  auto rnd = [&](auto tag) {
-    if (rounding) go(tag, std::true_type{});
+  auto type = [&](auto tag) {
+    if (flag) go(tag, std::true_type{});
     else go(tag, std::false_type{});
   };
-  if (dt == FH_BF16) rnd(uint16_t{});
-  else rnd(float{});
+  if (dt == FH_BF16) type(uint16_t{});
+  else type(float{});
 }
 
 // Grid of a pack or unpack: FH_ERR_INVALID where it would pass the largest.
@@ -109,9 +118,10 @@ extern "C" int fh_pack8(fh_dtype dt, fh_fmt8 fmt, const void* x, void* codes, ui
   FH_REQUIRE(aligned16(x) && aligned8(codes), "pack8: x must be 16-byte and codes 8-byte aligned");
   const int cpr = static_cast<int>(blocks8(cols) * 4);
   const FastDiv fd(static_cast<uint32_t>(cpr));
-  with_types(dt, fmt, true, [&](auto tag, auto f, auto) {
+  const bool stream_x = rows * cols * (dt == FH_BF16 ? 2 : 4) >= (int64_t(128) << 20);
+  with_types(dt, fmt, stream_x, [&](auto tag, auto f, auto st) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((k_pack8<T, f()>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
+    hipLaunchKernelGGL((k_pack8<T, f(), st()>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
                        stream, static_cast<const T*>(x), static_cast<uint8_t*>(codes), exps, rows,
                        static_cast<int>(cols), cpr, fd);
   });

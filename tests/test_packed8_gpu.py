@@ -79,6 +79,22 @@ def test_storage_equals_the_oracles(rows, cols, fmt, dtype):
         assert got.dtype == out and np.array_equal(_f64(got), ob.unpack8(codes, exps), equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", FMTS)
+def test_a_tensor_above_the_cache_is_packed_as_its_rows_are(fmt, dtype):
+    ops = _ops()
+    cols = 1000
+    edge = (128 << 20) // (cols * dtype.itemsize)  # the last whole row below 128 MiB
+    x = torch.randn(edge + 5, cols, generator=torch.Generator(DEV).manual_seed(5), device=DEV).to(dtype)
+    x[:14, :72], x[-14:, -72:] = _awkward(dtype).to(DEV), _awkward(dtype).to(DEV)
+    below, above = ops.pack8(x[:edge], fmt), ops.pack8(x, fmt)
+    assert torch.equal(above.codes[:edge].view(torch.uint8), below.codes.view(torch.uint8))
+    assert torch.equal(above.exps[:edge], below.exps)
+    codes, exps = ob.pack8(_f64(x[-40:]), fmt)
+    assert np.array_equal(above.exps[-40:].cpu().numpy(), exps)
+    assert np.array_equal(above.codes[-40:].float().cpu().numpy(), codes)
+
+
 def test_storage_takes_any_leading_shape_and_refuses_what_it_cannot_read():
     ops = _ops()
     x = randn((2, 3, 64), 4).bfloat16().to(DEV)

@@ -106,7 +106,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_fwd(
       ra = rsqrtf(row_sum<WPR>(ss, red[par][0], wave, lane) * inv_cols + eps);
       if (rstd_a != nullptr && valid && slice == 0 && lane == 0) rstd_a[row] = ra;
     }
-    const float f = ra * scale;
+    // (a r) w_post and s g first, then their product, and (h r) w_pre below: where a
+    // row's squares overflow r is 0, and so is a r w_post, while a w_post may be infinite.
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
@@ -117,16 +118,12 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_fwd(
       if constexpr (POST) {
         E::unpack(wpo[i], t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) n[j] *= t[j];
+        for (int j = 0; j < 8; ++j) n[j] = n[j] * ra * t[j];
       }
-      if constexpr (GATE != kNoGate) {
-        E::unpack(GATE == kChannelGate ? gc[i] : gr[i], t);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) n[j] *= t[j];
-      }
+      if constexpr (GATE != kNoGate) E::unpack(GATE == kChannelGate ? gc[i] : gr[i], t);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = E::rnd(fmaf(n[j], f, v[j]));
+        v[j] = E::rnd(fmaf(n[j], GATE != kNoGate ? scale * t[j] : scale, v[j]));
         ss = fmaf(v[j], v[j], ss);
       }
       xr[i] = E::pack(v);
@@ -142,7 +139,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_fwd(
         E::unpack(xr[i], v);
         E::unpack(wpr[i], t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= rh * t[j];
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * rh * t[j];
         E::store8(y + base + col(i), v);
       }
     }

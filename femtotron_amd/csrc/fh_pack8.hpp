@@ -7,7 +7,8 @@
 //   int8:  E = e - 6, code = rint(x 2^-E) with ties to even, at most 127 in
 //          magnitude (only a magnitude above 127.5 * 2^E is cut);
 //   e4m3:  E = e - 8, one more where m 2^-E would pass 448, the largest e4m3
-//          value (so none is cut); code = x 2^-E rounded to e4m3.
+//          value; code = x 2^-E rounded to e4m3, at E = 120 at most 240 in magnitude
+//          (only from 248 * 2^120 on is one cut: 256 * 2^120 is infinite).
 // A power of two, and not m / 127: the scaling is then exact in fp32, the codes
 // do not depend on how a quotient rounds, and code * 2^E is a value that bf16
 // holds, so a kernel that reads codes gives the bits that it gives for the
@@ -28,6 +29,7 @@ constexpr int kFmtInt8 = 0, kFmtE4M3 = 1;  // FH_INT8, FH_E4M3
 constexpr int kBlock8 = 32;
 constexpr uint32_t kMinExpByte = 9;    // E = -118
 constexpr uint32_t kNanExpByte = 255;
+constexpr uint32_t kTopExpByteE4M3 = 247;  // E = 120, e4m3's largest: 256 * 2^E is infinite
 
 __host__ __device__ __forceinline__ int64_t blocks8(int64_t cols) { return (cols + kBlock8 - 1) / kBlock8; }
 
@@ -105,8 +107,12 @@ __device__ __forceinline__ uint2 codes8(const float v[8], uint32_t e) {
         u[j] = __float_as_uint(__builtin_amdgcn_fmed3f(v[4 * i + j] * inv, -127.f, 127.f) + 12582912.f);
       w[i] = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u) | __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
     } else {
-      int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inv, v[4 * i + 1] * inv, 0, false);
-      t = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inv, v[4 * i + 3] * inv, t, true);
+      const float most = e == kTopExpByteE4M3 ? 240.f : 448.f;
+      float u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = __builtin_amdgcn_fmed3f(v[4 * i + j] * inv, -most, most);
+      int t = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], 0, false);
+      t = __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], t, true);
       w[i] = static_cast<uint32_t>(t);
     }
   }

@@ -31,7 +31,8 @@ int fh_blocks_abi_version(void);
  *   FH_INT8  E = e - 6, code = rint(x 2^-E), ties to even, at most 127 in
  *            magnitude: off by at most 2^(E-1), where it is cut by less than 2^E;
  *   FH_E4M3  E = e - 8, or e - 7 where m 2^-E would pass 448; code = x 2^-E
- *            rounded to e4m3: off by at most 2^-4 |x| or 2^(E-10).
+ *            rounded to e4m3, at most 240 in magnitude at E = 120 (256 * 2^120 is
+ *            infinite): off by at most 2^-4 |x| or 2^(E-10).
  * E >= -118.  A block that holds an infinity or a NaN has the byte 255 and codes
  * 0, and reads as NaN.  bf16 and fp32 hold every code * 2^E exactly.
  * codes: [rows, cols] bytes (8-byte aligned); exps: [rows, ceil(cols / 32)]

@@ -35,6 +35,7 @@ def pack8(x: np.ndarray, fmt: str) -> tuple[np.ndarray, np.ndarray]:
         E = np.maximum(e - 8, MIN_EXP)
         E = E + (m * np.ldexp(1.0, -E) > 448)
         c = _e4m3(xb * np.ldexp(1.0, -E)[..., None])
+        c = np.where((E == 120)[..., None], np.clip(c, -240, 240), c)  # 256 * 2^120 is no finite fp32 or bf16
     return c.reshape(T, nb * BLOCK)[:, :H], np.where(bad, 255, E + 127).astype(np.uint8)
 
 

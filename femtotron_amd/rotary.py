@@ -19,17 +19,21 @@ from . import ops
 SCALINGS = ("default", "linear", "dynamic", "yarn", "llama3")
 
 
-def rotary_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None, *,
+def rotary_frequencies(rot_dim: int, theta: float | None = None, scaling: dict | None = None, *,
                        seq_len: int | None = None, device=None) -> tuple[torch.Tensor, float]:
     """(inv_freq, factor) of ``apply_rotary``: the angle a position of each of the rot_dim / 2
     pairs (float64), theta^(-2i / rot_dim) unless scaled, and the factor on cos and sin.
+
+    ``theta``: given here, or else ``scaling``'s "rope_theta" (two that differ are refused),
+    or 10000.  ``rot_dim`` is what is rotated of a head: "partial_rotary_factor" is not read.
 
     ``scaling``: the dict of a Hugging Face config (``rope_scaling``), its "rope_type"
     (or "type") one of
       "default"  unscaled;
       "linear"   positions divided by "factor";
       "dynamic"  theta raised for a sequence of ``seq_len`` past
-                 "original_max_position_embeddings" (NTK-aware), by "factor";
+                 "original_max_position_embeddings" (NTK-aware), by "factor"; a config
+                 has that length as its max_position_embeddings, to be put in;
       "yarn"     pairs that turn fewer than "beta_slow" times in the original context
                  divided by "factor", more than "beta_fast" times kept, a ramp between
                  (its ends at whole pairs unless "truncate" is False);
@@ -40,9 +44,14 @@ def rotary_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | Non
     """
     if rot_dim <= 0 or rot_dim % 2:
         raise ValueError(f"rot_dim must be positive and even, got {rot_dim}")
+    scaling = dict(scaling or {})
+    own = scaling.get("rope_theta")
+    if theta is None:
+        theta = 10000.0 if own is None else float(own)
+    elif own is not None and float(own) != float(theta):
+        raise ValueError(f"theta is {theta}, the scaling's rope_theta {own}")
     if not theta > 1:
         raise ValueError(f"theta must be over 1, got {theta}")
-    scaling = dict(scaling or {})
     kind = scaling.get("rope_type", scaling.get("type", "default"))
     if kind not in SCALINGS:
         raise ValueError(f"rope_type must be one of {SCALINGS}, got {kind!r}")

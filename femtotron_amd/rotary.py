@@ -45,6 +45,9 @@ def rotary_frequencies(rot_dim: int, theta: float | None = None, scaling: dict |
     if rot_dim <= 0 or rot_dim % 2:
         raise ValueError(f"rot_dim must be positive and even, got {rot_dim}")
     scaling = dict(scaling or {})
+    layers = [k for k, v in scaling.items() if isinstance(v, dict)]
+    if layers:
+        raise ValueError(f"scaling holds one dict for each of {layers}: pass the one of the layer")
     own = scaling.get("rope_theta")
     if theta is None:
         theta = 10000.0 if own is None else float(own)

@@ -54,7 +54,7 @@ def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = 
                 eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(h, y) = (x + scale * gate * RMSNorm(a; w_post), RMSNorm(h; w_pre)) over the last
     dim of x and a (one shape, bf16 or fp32, on a HIP device), differentiable in every
-    tensor.
+    tensor (once, and in reverse mode).
 
     ``w_post`` None: a enters without a norm; ``w_pre`` None: y is None (one of the
     two is given).  ``gate``: one value a channel ([hidden], or with leading ones), one an
@@ -66,7 +66,7 @@ def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = 
     if gate is not None and gate.shape != x.shape and gate.numel() == x.shape[-1] == gate.shape[-1]:
         gate = gate.reshape(-1)
     tensors = tuple(map(ops.aligned, (x, a, w_post, w_pre, gate)))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if ops.differentiated(*tensors):
         return BlockNormsFunction.apply(ops.block_norms_check("block_norms", *tensors), *tensors, float(scale), float(eps))
     x, a, w_post, w_pre, gate = tensors
     return ops.block_norms_fwd(x, a, w_post, w_pre, float(eps), gate=gate, scale=float(scale))

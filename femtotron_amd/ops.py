@@ -11,6 +11,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -101,6 +102,15 @@ def aligned(t: torch.Tensor | None) -> torch.Tensor | None:
         return None
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these tensors has to go through its autograd node: one wants a
+    gradient, or forward-mode derivatives are on (their dual tensors do not say that they
+    want one, and the node is what refuses them: it has no jvp)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _ptr(t: torch.Tensor | None):

@@ -145,7 +145,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     """q and k, [tokens, heads * head_dim] or [batch, seq, heads * head_dim] (k may be None,
     their head counts may differ; column views of a packed projection are read in place),
     with dims [offset, offset + rot_dim) of each head turned by positions * inv_freq, cos
-    and sin times factor; differentiable in q and k.
+    and sin times factor; differentiable in q and k (once, and in reverse mode).
 
     positions: int64 of any shape, one a token in order, or one a position of sequences of
     equal length (seq of them; of [tokens, ...] a divisor of tokens); inv_freq, factor:
@@ -163,6 +163,6 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
                              f"{n} {tuple(t.shape)}")
     how = dict(head_dim=head_dim, rot_dim=rot_dim, offset=offset, layout=layout, factor=float(factor))
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+    if ops.differentiated(q, k):
         return RotaryFunction.apply(q, k, positions, inv_freq, how)
     return _turn(ops.rotary_fwd, q, k, positions, inv_freq, how)

@@ -83,9 +83,17 @@ def _stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+_jit_trace, _mode = torch._C._get_tracing_state, torch._C._get_dispatch_mode
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
 def _launch(name: str, t: torch.Tensor, *args) -> None:
     """Calls an entry point on the current stream of t's device, with that device
-    the current one (the default stream's handle is 0 on every device)."""
+    the current one (the default stream's handle is 0 on every device).  Refused while
+    torch records the operations it sees, of which a kernel is none."""
+    if _jit_trace() is not None or _mode(_PROXY) is not None:
+        raise RuntimeError(f"{name}: torch.jit.trace and make_fx do not see this library's kernels; "
+                           "a trace would return uninitialised memory")
     index = t.get_device()
     if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):

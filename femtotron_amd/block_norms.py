@@ -61,7 +61,7 @@ def block_norms(x: torch.Tensor, a: torch.Tensor, w_post: torch.Tensor | None = 
     element (x's shape: expand a gate that is shared along some dims), or None.
     y is the norm of h in x's dtype, as returned.  ``scale`` is a number: a learned one
     belongs in the gate."""
-    if isinstance(scale, torch.Tensor) and scale.requires_grad:
+    if isinstance(scale, torch.Tensor) and (scale.requires_grad or ops.wants_derivative(scale)):
         raise TypeError("block_norms: scale is a number and gets no gradient; fold a learned one into the gate")
     if gate is not None and gate.shape != x.shape and gate.numel() == x.shape[-1] == gate.shape[-1]:
         gate = gate.reshape(-1)

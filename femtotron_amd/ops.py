@@ -121,6 +121,13 @@ def differentiated(*tensors: torch.Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def wants_derivative(v) -> bool:
+    """Whether v, a constant of an operator, is a tensor that asks for a derivative."""
+    return isinstance(v, torch.Tensor) and ((v.requires_grad and torch.is_grad_enabled())
+                                            or (forward_ad._current_level >= 0
+                                                and forward_ad.unpack_dual(v).tangent is not None))
+
+
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 

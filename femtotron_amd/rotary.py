@@ -149,8 +149,11 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
 
     positions: int64 of any shape, one a token in order, or one a position of sequences of
     equal length (seq of them; of [tokens, ...] a divisor of tokens); inv_freq, factor:
-    ``rotary_frequencies``; layout: pairs (i, i + rot_dim / 2), "half", or (2i, 2i + 1),
+    ``rotary_frequencies``, constants (refused where they want a gradient); layout: pairs (i, i + rot_dim / 2), "half", or (2i, 2i + 1),
     "interleaved"."""
+    for v, n in ((inv_freq, "inv_freq"), (factor, "factor")):
+        if ops.wants_derivative(v):
+            raise TypeError(f"apply_rotary: {n} is a constant and gets no gradient")
     n_positions = positions.numel()
     for t, n in ((q, "q"), (k, "k")):
         if t is None:

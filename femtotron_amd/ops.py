@@ -116,9 +116,11 @@ def differentiated(*tensors: torch.Tensor | None) -> bool:
     """Whether a call on these tensors has to go through its autograd node: one wants a
     gradient, or forward-mode derivatives are on (their dual tensors do not say that they
     want one, and the node is what refuses them: it has no jvp)."""
-    if forward_ad._current_level >= 0:
-        return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0
 
 
 def wants_derivative(v) -> bool:
@@ -387,7 +389,8 @@ def rope_bwd_(dqk: torch.Tensor, n_heads: int, head_dim: int, seq_len: int, cos:
 # --------------------------------------------------- norms around a block
 def _block_norms_shapes(name: str, like: torch.Tensor, w_post, w_pre, gate) -> tuple[int, int, int, int]:
     """(dtype code, gate_per_token, rows, cols) of block norms over `like`'s rows, checked."""
-    cols = like.size(-1) if like.dim() else 0
+    shape = like.shape
+    cols = shape[-1] if shape else 0
     if w_post is None and w_pre is None:
         raise ValueError(f"{name}: at least one of w_post and w_pre is needed")
     for w, n in ((w_post, "w_post"), (w_pre, "w_pre")):
@@ -396,8 +399,8 @@ def _block_norms_shapes(name: str, like: torch.Tensor, w_post, w_pre, gate) -> t
     per_token = 0
     if gate is not None:
         per_token = int(gate.shape != (cols,))
-        if (per_token and gate.shape != like.shape) or not gate.is_contiguous():
-            raise ValueError(f"{name}: gate must be contiguous, of shape [{cols}] or {tuple(like.shape)}, got "
+        if (per_token and gate.shape != shape) or not gate.is_contiguous():
+            raise ValueError(f"{name}: gate must be contiguous, of shape [{cols}] or {tuple(shape)}, got "
                              f"{tuple(gate.shape)}")
     return _dtype_code(like), per_token, like.numel() // max(cols, 1), cols
 

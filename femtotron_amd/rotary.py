@@ -130,7 +130,8 @@ def _rows(t: torch.Tensor | None) -> torch.Tensor | None:
         return None
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 and t.stride(0) >= t.size(1) else t.contiguous()
+    ld, unit = t.stride()
+    return t if unit == 1 and ld >= t.shape[1] else t.contiguous()
 
 
 def _turn(op, q, k, positions, inv_freq, how):
@@ -151,9 +152,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     equal length (seq of them; of [tokens, ...] a divisor of tokens); inv_freq, factor:
     ``rotary_frequencies``, constants (refused where they want a gradient); layout: pairs (i, i + rot_dim / 2), "half", or (2i, 2i + 1),
     "interleaved"."""
-    for v, n in ((inv_freq, "inv_freq"), (factor, "factor")):
-        if ops.wants_derivative(v):
-            raise TypeError(f"apply_rotary: {n} is a constant and gets no gradient")
+    if ops.wants_derivative(inv_freq) or ops.wants_derivative(factor):
+        raise TypeError("apply_rotary: inv_freq and factor are constants and get no gradient")
     n_positions = positions.numel()
     for t, n in ((q, "q"), (k, "k")):
         if t is None:

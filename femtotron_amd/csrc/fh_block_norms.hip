@@ -17,8 +17,11 @@
 // rows, three vectors and two sums under 128 registers: four waves a SIMD.
 // 16384 x 2048 bf16 with a channel gate: forward 45.9 us call after call (268 MB,
 // 5.8 TB/s) and 52 with a backward between (5.1), backward 75.5 us (403 MB, 5.3)
-// and its sums 4; a copy runs at 5.4.  Non-temporal stores of h and y or of dx and
-// da cost 4 to 5 us each.
+// and its sums 4; a copy runs at 5.4.  Non-temporal stores of h and y cost 4.1 us
+// (55.5 -> 59.6 with a backward between), of dx and da 2.7 (81.4 -> 84.1).  With a gate
+// per token, 8192 x 4096: forward 59 us (336 MB, 5.7 TB/s), backward 100 (537 MB, 5.4).
+// fp32: 16384 x 2048 with a channel gate 110 and 160 (537 and 805 MB, 4.9 and 5.0),
+// 8192 x 4096 with a gate per token 126 and 216 (671 and 1074 MB, 5.3 and 5.0).
 #include "femtohip_blocks.h"
 #include "fh_common.hpp"
 

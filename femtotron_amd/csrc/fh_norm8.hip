@@ -7,7 +7,10 @@
 // int8, us a launch: pack 70 and unpack 67 at 32768 x 4096 (407 MB, 5.8 and 6.1
 // TB/s); at 16384 x 2048 the norm that packs 28 (169 MB, 5.9), the norm from codes
 // 17 (102 MB, 6.0), its add + norm 38 (236 MB, 6.1), the backward with the residual
-// gradient 39 (236 MB, 6.1) and its reduction 4.  A copy runs at 5.4.
+// gradient 39 (236 MB, 6.1) and its reduction 4.  A copy runs at 5.4.  Those norms are
+// rounded once; with llama_rounding, which eight_bit_checkpoint asks for, the norm
+// from codes takes 21, in one run of all (the codes read by others before) the
+// backward 51 against 49, the others within 2 us.
 #include "femtohip_blocks.h"
 #include "fh_norm.hpp"
 
@@ -25,12 +28,19 @@ __device__ __forceinline__ void row_chunk(uint32_t idx, int cpr, const FastDiv& 
   c = static_cast<int>(idx - q * static_cast<uint32_t>(cpr)) * 8;
 }
 
-// STREAM: x with non-temporal loads.  Below 128 MiB of x plain ones are faster (an
-// activation was mostly written just before and is still in the 256 MB cache: bf16
-// 4096 x 2048 6.3 us against 7.2, 16384 x 2048 19.5 against 20.7, fp32 8192 x 2048 15.3
-// against 16.5).  From there on x does not stay anyway, and streamed it leaves the
-// codes in the cache for their reader: pack and unpack of bf16 32768 x 2048 68.1 us
-// against 69.6, 32768 x 4096 135 against 144, fp32 16384 x 4096 108 against 136.
+// STREAM: x with non-temporal loads.  An x that was read or written just before is
+// still in the 256 MB cache below 128 MiB, and plain loads are then faster; one that
+// is not there is faster streamed, at every size.  From 128 MiB on it hardly stays,
+// and streaming wins both ways.  The kernel, us, plain and streamed, packed call after
+// call (two x in turn) | with 1 GiB copied before:
+//   bf16 4096 x 2048     6.6   7.6 |  8.4   7.1
+//   bf16 16384 x 2048   18.2  20.8 | 21.9  19.9
+//   bf16 32768 x 2048   43.7  36.5 | 40.4  37.5
+//   bf16 32768 x 4096   80.0  71.9 | 74.0  69.3
+//   fp32 8192 x 2048    13.5  18.4 | 19.9  16.1
+//   fp32 16384 x 4096   78.2  61.5 | 70.9  61.6
+// What unpacks the codes takes the same either way: 66.0 and 66.1 us at 32768 x 4096
+// with 1 GiB copied between, as between a forward and its backward.
 template <typename T, int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void k_pack8(const T* __restrict__ x, uint8_t* __restrict__ codes,
                                                uint8_t* __restrict__ exps, int64_t rows, int cols, int cpr,

@@ -1,9 +1,10 @@
 // Activations in 8 bits: the storage, its packing and unpacking in registers.
 //
 // 32 consecutive elements of a row (the last block of a row may be shorter)
-// share an exponent E, kept as the byte E + 127; an element is code * 2^E (the
-// layouts MXINT8 and MXFP8-E4M3 of the OCP microscaling formats, 8.25 bits an
-// element).  With m the block's largest magnitude and e = floor(log2 m):
+// share an exponent E, kept as the byte E + 127; an element is code * 2^E, 8.25
+// bits an element.  (The e4m3 bytes are those of the OCP microscaling format
+// MXFP8-E4M3.  MXINT8 has the same codes, but counts them in 2^-6: its scale byte
+// is this one plus 6.)  With m the block's largest magnitude and e = floor(log2 m):
 //   int8:  E = e - 6, code = rint(x 2^-E) with ties to even, at most 127 in
 //          magnitude (only a magnitude above 127.5 * 2^E is cut);
 //   e4m3:  E = e - 8, one more where m 2^-E would pass 448, the largest e4m3
@@ -13,9 +14,10 @@
 // do not depend on how a quotient rounds, and code * 2^E is a value that bf16
 // holds, so a kernel that reads codes gives the bits that it gives for the
 // unpacked tensor.  What it costs is up to one bit of int8's seven (steps of
-// m/127 to m/64); e4m3 has its step in each element's own exponent and loses
-// nothing.  E is at least -118 (blocks of magnitudes below 2^-112 keep steps of
-// 2^-118 and 2^-127).  A block with an infinity or a NaN has the byte 255 and
+// m/127 to m/64); e4m3 has its step in each element's own exponent, and so loses
+// none of its bits to it, down to the format's smallest step 2^(E-9): an element
+// is off by at most 2^-4 of itself or 2^(E-10), which is under 2^-17 m.  E is at
+// least -118: no step is under 2^-118 in int8, 2^-127 in e4m3.  A block with an infinity or a NaN has the byte 255 and
 // codes 0 and reads as NaN throughout, so that a bad activation reaches the
 // gradients instead of being cut to a finite one.
 #pragma once

@@ -14,6 +14,8 @@
 // computed by each block into LDS for the heads it has of a token, so no table is
 // read.  bf16, us a launch: 16384 tokens of 36 heads of 64 28 (151 MB, 5.4 TB/s),
 // 32768 tokens of 64 heads of 128, half of each turned, 182-185 (1074 MB, 5.8-5.9).
+// fp32: 16384 tokens of 36 heads of 64 67 (302 MB, 4.5), of what was just written 51
+// (5.9); 8192 tokens of 40 heads of 128 69 and 57 (336 MB, 4.9 and 5.9).
 #include "femtohip_blocks.h"
 #include "fh_common.hpp"
 
@@ -112,10 +114,11 @@ constexpr int kMaxPairs = 254 * 8 + 1024;
 // An item is V pairs of one head of one token, or 2V of its passing elements: two
 // accesses of V elements each way.  A thread has one, of the call's items token by
 // token, and has its loads under way before the block computes the angles of the
-// tokens it touches.  (More items a thread, or blocks of whole tokens, measured
-// slower: 16384 tokens of 36 heads of 64, forward and backward, 55 us with one
-// item, 60, 63 and 69 with two, four and eight; 86 with the loads behind the
-// angles.)
+// tokens it touches.  Measured otherwise, forward and backward, 16384 tokens of 36
+// heads of 64 and 32768 of 64 heads of 128, half of each turned: this 56 and 366 us;
+// blocks of whole tokens 55 and 388; those with two, four and eight items a thread
+// 60, 63 and 69, and (with eight) 413; with four, the loads behind the angles, 86
+// and 537.
 template <typename T, int V, bool INTER, bool BWD>
 __global__ __launch_bounds__(256) void k_rotary(RotaryArgs p) {
   __shared__ __align__(16) float cs[kMaxPairs], sn[kMaxPairs];

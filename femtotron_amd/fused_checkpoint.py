@@ -289,8 +289,10 @@ _PACKED = {FusedDecoderLayerFunction: PackedDecoderLayerFunction, FusedMLPFuncti
 def eight_bit_checkpoint(fmt: str = "int8"):
     """A ``checkpoint_fn`` like ``fused_checkpoint`` that keeps the input of a fused
     call in 8 bits from the forward to the backward: blocks of 32 elements with
-    one power-of-two exponent and codes in "int8" (the finer steps) or "e4m3"
-    (small elements beside a large one keep theirs), 8.25 bits an element.
+    one power-of-two exponent and codes in "int8" (off by up to 2^-7 of the block's
+    largest element) or "e4m3" (by up to 2^-4 of each element, or 2^-17 of the largest
+    where that is more: small elements beside a large one keep more of theirs), 8.25
+    bits an element.
     Outputs are those of ``fused_checkpoint``; gradients are taken at the kept
     value.  Calls that are not fused keep their input as it is."""
     if fmt not in ops.FORMATS8:

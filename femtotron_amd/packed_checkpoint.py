@@ -8,8 +8,9 @@ kept as ``ops.Packed8``: 8.25 bits an element instead of 16 or 32.
 
 The forward computes from the input itself, so outputs and losses are those of
 ``fused_checkpoint`` bit for bit.  The backward is that of ``fused_checkpoint`` at
-the kept value x^ (|x^ - x| at most 2^-7 of the largest magnitude of x's block of 32
-in "int8", 2^-4 |x| in "e4m3"), again bit for bit.
+the kept value x^, again bit for bit.  With m the largest magnitude of x's block of
+32, |x^ - x| is at most the larger of 2^-7 m and 2^-119 in "int8", and of 2^-4 |x|, 2^-17 m
+and 2^-128 in "e4m3".
 
 * decoder layer: the first norm's pass packs x; in the backward the recompute's
   norm and residual add + norm and the norm's backward read the codes, and x^ is

@@ -24,6 +24,7 @@
 // 8192 x 4096 with a gate per token 126 and 216 (671 and 1074 MB, 5.3 and 5.0).
 #include "femtohip_blocks.h"
 #include "fh_common.hpp"
+#include "fh_parts.hpp"
 
 namespace fh {
 namespace {
@@ -47,17 +48,11 @@ __device__ __forceinline__ float row_sum(float v, float* red, int wave, int lane
   return s;
 }
 
-// 8 elements of a row, with STREAM as non-temporal loads: data read once.  16384 x
-// 2048, us: backward 86.6 -> 81.4, forward with a per-token gate (8192 x 4096) 62.1
-// -> 56.7; the forward's two rows without one 45.9 against 47.1, so not there.
-template <typename T, bool STREAM>
-__device__ __forceinline__ typename Elem<T>::Raw load_once(const T* p) {
-  if constexpr (STREAM) return Elem<T>::ldraw_stream(p);
-  else return Elem<T>::ldraw(p);
-}
-
 // A block takes kWaves / WPR rows a step; its barriers are reached by every wave
 // (the step loop is uniform, rows behind the last one are computed on zeros).
+// Non-temporal loads, 16384 x 2048, us: backward 86.6 -> 81.4, forward with a per-token
+// gate (8192 x 4096) 62.1 -> 56.7; the forward's two rows without one 45.9 against
+// 47.1, so not there.
 template <typename T, int NVW, int WPR, int GATE, bool POST, bool PRE>
 __global__ __launch_bounds__(64 * kWaves) void k_block_norms_fwd(
     const T* __restrict__ x, const T* __restrict__ a, const T* __restrict__ w_post, const T* __restrict__ w_pre,
@@ -91,9 +86,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_fwd(
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
       if (!in(i)) continue;
-      ar[i] = load_once<T, GATE == kTokenGate>(a + base + col(i));
-      xr[i] = load_once<T, GATE == kTokenGate>(x + base + col(i));
-      if constexpr (GATE == kTokenGate) gr[i] = load_once<T, GATE == kTokenGate>(gate + base + col(i));
+      ar[i] = load_if<T, GATE == kTokenGate>(a + base + col(i));
+      xr[i] = load_if<T, GATE == kTokenGate>(x + base + col(i));
+      if constexpr (GATE == kTokenGate) gr[i] = load_if<T, GATE == kTokenGate>(gate + base + col(i));
     }
     float ra = 1.f;
     if constexpr (POST) {
@@ -201,12 +196,12 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_bwd(
     for (int i = 0; i < NVW; ++i) {
       if (!in(i)) continue;
       if constexpr (PRE) {
-        dyr[i] = load_once<T, true>(dy + base + col(i));
-        hr[i] = load_once<T, true>(h + base + col(i));
+        dyr[i] = load_if<T, true>(dy + base + col(i));
+        hr[i] = load_if<T, true>(h + base + col(i));
       }
-      dhr[i] = load_once<T, true>(dh + base + col(i));
-      if constexpr (A) ar[i] = load_once<T, true>(a + base + col(i));
-      if constexpr (GATE == kTokenGate) gr[i] = load_once<T, true>(gate + base + col(i));
+      dhr[i] = load_if<T, true>(dh + base + col(i));
+      if constexpr (A) ar[i] = load_if<T, true>(a + base + col(i));
+      if constexpr (GATE == kTokenGate) gr[i] = load_if<T, true>(gate + base + col(i));
     }
     float D[NVW][8];
     float dot = 0.f, rh = 0.f;
@@ -310,53 +305,22 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_bwd(
   if constexpr (SUM) put(acc_sum);
 }
 
-// The sums over the partial rows and, from them, the vectors' gradients.  A block
-// owns 16 columns of one sum (blockIdx.y): 64 row groups x 4 column quads, the
-// groups added in order.
+// The sums over the partial rows (fh_parts.hpp; blockIdx.y: which of a row's) and, from
+// them, the vectors' gradients.
 template <typename T>
 __global__ __launch_bounds__(256) void k_block_norms_sums(const float* __restrict__ part, int nparts, int nsums,
                                                           int cols, bool pre, const T* __restrict__ w_post,
                                                           const T* __restrict__ gate, bool channel,
                                                           T* __restrict__ dw_pre, T* __restrict__ dw_post,
                                                           T* __restrict__ dgate) {
-  constexpr int G = 64, U = 8;
-  __shared__ float red[G][17];
-  const int q = threadIdx.x & 3, g = threadIdx.x >> 2;
-  const int c = blockIdx.x * 16 + q * 4;  // cols % 8 == 0: a quad is wholly in or out
-  const int64_t ld = static_cast<int64_t>(nsums) * cols;
-  const float* src = part + static_cast<int64_t>(blockIdx.y) * cols + c;
-  float4 s = {0.f, 0.f, 0.f, 0.f};
-  if (c < cols) {
-    int p = g;
-    for (; p + G * (U - 1) < nparts; p += G * U) {
-      float4 v[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) v[k] = *reinterpret_cast<const float4*>(src + (p + G * k) * ld);
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w;
-      }
-    }
-    for (; p < nparts; p += G) {
-      const float4 v = *reinterpret_cast<const float4*>(src + p * ld);
-      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-    }
-  }
-  red[g][q * 4 + 0] = s.x;
-  red[g][q * 4 + 1] = s.y;
-  red[g][q * 4 + 2] = s.z;
-  red[g][q * 4 + 3] = s.w;
-  __syncthreads();
-  const int cc = blockIdx.x * 16 + static_cast<int>(threadIdx.x);
-  if (threadIdx.x < 16 && cc < cols) {
-    float t = 0.f;
-    for (int k = 0; k < G; ++k) t += red[k][threadIdx.x];
-    if (pre && blockIdx.y == 0) {
-      Elem<T>::st1(dw_pre + cc, t);
-    } else {
-      if (dw_post != nullptr) Elem<T>::st1(dw_post + cc, channel ? t * Elem<T>::ld1(gate + cc) : t);
-      if (channel) Elem<T>::st1(dgate + cc, w_post != nullptr ? t * Elem<T>::ld1(w_post + cc) : t);
-    }
+  const float t = sum_parts(part + static_cast<int64_t>(blockIdx.y) * cols, static_cast<int64_t>(nsums) * cols, nparts, cols);
+  const int c = blockIdx.x * 16 + static_cast<int>(threadIdx.x);
+  if (threadIdx.x >= 16 || c >= cols) return;
+  if (pre && blockIdx.y == 0) {
+    Elem<T>::st1(dw_pre + c, t);
+  } else {
+    if (dw_post != nullptr) Elem<T>::st1(dw_post + c, channel ? t * Elem<T>::ld1(gate + c) : t);
+    if (channel) Elem<T>::st1(dgate + c, w_post != nullptr ? t * Elem<T>::ld1(w_post + c) : t);
   }
 }
 

@@ -148,6 +148,13 @@ struct Elem<float> {
   __device__ __forceinline__ static void st1(float* p, float f) { *p = f; }
 };
 
+// 8 elements, with STREAM as a non-temporal load: data read once.
+template <typename T, bool STREAM>
+__device__ __forceinline__ typename Elem<T>::Raw load_if(const T* p) {
+  if constexpr (STREAM) return Elem<T>::ldraw_stream(p);
+  else return Elem<T>::ldraw(p);
+}
+
 // ------------------------------------------------------------ RoPE pair
 // Rotate-half rotary embedding of one pair (x0 at dim i, x1 at dim
 // i + head_dim/2; cos c0, c1 and sin s0, s1 at those dims), rounded with

@@ -20,6 +20,7 @@
 
 #include "fh_common.hpp"
 #include "fh_pack8.hpp"
+#include "fh_parts.hpp"
 
 namespace fh {
 namespace {
@@ -54,13 +55,6 @@ template <typename T, bool RND>
 __device__ __forceinline__ float rnd_if(float f) {
   if constexpr (RND) return Elem<T>::rnd(f);
   else return f;
-}
-
-// 8 elements, with STREAM as a non-temporal load: data read once.
-template <typename T, bool STREAM>
-__device__ __forceinline__ typename Elem<T>::Raw load_if(const T* p) {
-  if constexpr (STREAM) return Elem<T>::ldraw_stream(p);
-  else return Elem<T>::ldraw(p);
 }
 
 constexpr int kWavesPerBlock = 4;  // 256 threads
@@ -365,50 +359,13 @@ __global__ __launch_bounds__(64 * NWB) void k_rmsnorm_bwd(
   for (int c = threadIdx.x; c < cols; c += blockDim.x) dst[c] = lds_acc[c];
 }
 
-// dw[c] = sum_p part[p, c], deterministic, in one launch.  A block owns 16
-// columns: its 256 threads are 64 row groups x 4 column quads; thread (g, q)
-// sums the float4 of rows p = g, g + 64, g + 128, ... in order (eight loads in
-// flight), and the 64 group sums of a column are added in group order.  One
-// launch instead of a partial pass plus a stage pass measured 1-2 us faster
-// per backward call (one launch gap fewer).
+// dw[c] = sum_p part[p, c] (fh_parts.hpp).
 template <typename T>
 __global__ __launch_bounds__(256) void k_reduce_parts(const float* __restrict__ part, int nparts,
                                                       int cols, T* __restrict__ out) {
-  constexpr int G = 64, U = 8;
-  __shared__ float red[G][17];
-  const int q = threadIdx.x & 3, g = threadIdx.x >> 2;
-  const int c = blockIdx.x * 16 + q * 4;  // cols % 8 == 0: a quad is wholly in or out
-  float4 s = {0.f, 0.f, 0.f, 0.f};
-  if (c < cols) {
-    auto at = [&](int p) {
-      return *reinterpret_cast<const float4*>(part + static_cast<int64_t>(p) * cols + c);
-    };
-    int p = g;
-    for (; p + G * (U - 1) < nparts; p += G * U) {
-      float4 v[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) v[k] = at(p + G * k);
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w;
-      }
-    }
-    for (; p < nparts; p += G) {
-      const float4 v = at(p);
-      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-    }
-  }
-  red[g][q * 4 + 0] = s.x;
-  red[g][q * 4 + 1] = s.y;
-  red[g][q * 4 + 2] = s.z;
-  red[g][q * 4 + 3] = s.w;
-  __syncthreads();
-  const int cc = blockIdx.x * 16 + static_cast<int>(threadIdx.x);
-  if (threadIdx.x < 16 && cc < cols) {
-    float t = 0.f;
-    for (int k = 0; k < G; ++k) t += red[k][threadIdx.x];
-    Elem<T>::st1(out + cc, t);
-  }
+  const float t = sum_parts(part, cols, nparts, cols);
+  const int c = blockIdx.x * 16 + static_cast<int>(threadIdx.x);
+  if (threadIdx.x < 16 && c < cols) Elem<T>::st1(out + c, t);
 }
 
 template <typename T>

@@ -41,7 +41,7 @@ import types
 import torch
 
 from . import _lib, ops
-from .fused_checkpoint import _aligned, _causal_attention_reason, _check_params, _linear_weight
+from .fused_checkpoint import _causal_attention_reason, _check_params, _linear_weight
 from .fused_layer import (LayerShape, _WgradStream, _cat_rows, attn_bwd, grad_target, qkv_attention,
                           split_rows)
 from .projections import linear, linear_dgrad
@@ -183,7 +183,7 @@ def _fused_forward(self, hidden_states, position_embeddings=None, attention_mask
     cos, sin = position_embeddings
     with _counts_lock:
         _counts["fused"] += 1
-    out = FusedAttentionFunction.apply(_aligned(hidden_states), _aligned(cos), _aligned(sin), shp, *ws)
+    out = FusedAttentionFunction.apply(ops.aligned(hidden_states), ops.aligned(cos), ops.aligned(sin), shp, *ws)
     return out, None
 
 

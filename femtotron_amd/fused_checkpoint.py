@@ -132,11 +132,6 @@ def _check_params(x: torch.Tensor, weights) -> str | None:
     return None
 
 
-def _aligned(x: torch.Tensor) -> torch.Tensor:
-    x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
-
-
 def _plan(module: Any, args: tuple, kwargs: dict):
     """Return (autograd Function, its apply() arguments) if the call can be fused,
     else a reason string."""
@@ -174,7 +169,7 @@ def _plan_mlp(mlp: Any, x: torch.Tensor, kwargs: dict):
         return "unexpected MLP weight shapes"
     if H % 8 or F_ % 8:
         return "hidden % 8 and ffn % 8 required"
-    return FusedMLPFunction, (_aligned(x), wg, wu, wd)
+    return FusedMLPFunction, (ops.aligned(x), wg, wu, wd)
 
 
 def _plan_norm(norm: Any, x: torch.Tensor, kwargs: dict):
@@ -191,7 +186,7 @@ def _plan_norm(norm: Any, x: torch.Tensor, kwargs: dict):
         return "RMSNorm weight size != last dim"
     if H % 8 or H > 8192:
         return "hidden % 8 and hidden <= 8192 required"
-    return FusedRMSNormFunction, (_aligned(x), w, float(norm.variance_epsilon))
+    return FusedRMSNormFunction, (ops.aligned(x), w, float(norm.variance_epsilon))
 
 
 def _plan_layer(module: Any, x: torch.Tensor, kwargs: dict):
@@ -254,7 +249,7 @@ def _plan_layer(module: Any, x: torch.Tensor, kwargs: dict):
     shp = LayerShape(hidden=H, n_heads=nh, n_kv_heads=nkv, head_dim=hd, ffn=F_,
                      eps1=float(ln1.variance_epsilon), eps2=float(ln2.variance_epsilon),
                      scale=float(attn.scaling))
-    return FusedDecoderLayerFunction, (_aligned(x), _aligned(cos), _aligned(sin), shp, *weights)
+    return FusedDecoderLayerFunction, (ops.aligned(x), ops.aligned(cos), ops.aligned(sin), shp, *weights)
 
 
 _KINDS: dict = {}

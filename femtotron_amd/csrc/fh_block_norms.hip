@@ -152,7 +152,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_block_norms_fwd(
 //   dw_post = sum P n_a
 //   dg = s D n_a w_post, summed over the rows for a channel gate
 // D stays in fp32 registers between the two norms.  Of a channel gate both
-// dw_post and dg come from S = sum D n_a: dw_post = s g S, dg = s w_post S.  part:
+// dw_post and dg come from S = sum s D n_a: dw_post = g S, dg = w_post S.  part:
 // per block one row of sum dy n_h (PRE) and one of S, or of sum P n_a for a token
 // gate (SUM), in fp32; k_block_norms_sums adds them in a fixed order.
 template <typename T, int NVW, int WPR, int GATE, bool POST, bool PRE>

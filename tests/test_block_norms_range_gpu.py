@@ -52,3 +52,23 @@ def test_a_large_weight_on_a_small_row(dtype):
     _, y = block_norms(x, torch.zeros_like(x), None, w)
     ref = 2.0 ** 85 / (2.0 ** -80 + EPS) ** 0.5
     assert float((y.double() / ref - 1).abs().max()) <= torch.finfo(dtype).eps / 2 + 80 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("gate", [None, "channel", "token"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_gradients_of_a_row_whose_squares_overflow(gate, dtype):
+    """r is 0, so nothing reaches a, its weight or its gate; dx is what it is for a row of zeros in a."""
+    from femtotron_amd import block_norms
+    rows, cols = 3, 2048
+    g = None if gate is None else torch.full((cols,) if gate == "channel" else (rows, cols), 3.0, dtype=dtype, device=DEV)
+    w, w_pre = torch.full((cols,), 4.0, dtype=dtype, device=DEV), (1 + randn((cols,), 2, 0.1)).to(dtype).to(DEV)
+    dh, dy = (randn((rows, cols), s).to(dtype).to(DEV) for s in (3, 4))
+    grads = []
+    for fill in (1.5e38, 0.0):
+        x = randn((rows, cols), 1).to(dtype).to(DEV)
+        t = [v.clone().requires_grad_(True) for v in (x, torch.full_like(x, fill), w, w_pre) + (() if g is None else (g,))]
+        h, y = block_norms(*t[:4], gate=None if g is None else t[4], scale=2.0)
+        grads.append(torch.autograd.grad((h, y), t, (dh, dy)))
+    (dx, da, dw, dw_pre, *dg), (dx0, _, _, dw_pre0, *_) = grads
+    assert torch.equal(dx, dx0) and torch.equal(dw_pre, dw_pre0)
+    assert all(torch.count_nonzero(v) == 0 for v in (da, dw, *dg))  # a NaN counts

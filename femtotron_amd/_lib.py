@@ -1,5 +1,6 @@
-"""ctypes binding of ``libfemtohip.so`` (the C ABI declared in include/femtohip.h
-and, for what stands around a checkpointed block, include/femtohip_blocks.h).
+"""ctypes binding of ``libfemtohip.so`` (the C ABI declared in include/femtohip.h;
+for what stands around a checkpointed block, in include/femtohip_blocks.h; for a step
+over packed documents, in include/femtohip_packed.h).
 
 The library is built in-tree by ``femtotron_amd.csrc.build`` (``__graft_entry__.build()``).
 There is no fallback: if the library is missing or does not load, ``lib()`` raises,
@@ -15,6 +16,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libfemtohip.so"
 ABI_VERSION = 7
 BLOCKS_ABI_VERSION = 1
+PACKED_ABI_VERSION = 1
 
 FH_BF16 = 0
 FH_F32 = 1
@@ -46,6 +48,11 @@ class FhGemmProblem(ctypes.Structure):
     fh_gemm_bf16_grouped)."""
     _fields_ = [("a", _V), ("lda", _I64), ("b", _V), ("ldb", _I64), ("c", _V), ("ldc", _I64),
                 ("residual", _V), ("ldr", _I64), ("m", _I64), ("n", _I64)]
+
+
+class FhGrad(ctypes.Structure):
+    """fh_grad of include/femtohip_packed.h."""
+    _fields_ = [("grad", _V), ("out", _V), ("numel", _I64), ("grad_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32)]
 
 
 class FhLayer(ctypes.Structure):
@@ -131,6 +138,25 @@ BLOCK_SIGNATURES: dict[str, tuple] = {
                               _V, _I64, _V, _F, _V]),
 }
 
+# The same of include/femtohip_packed.h.
+PACKED_SIGNATURES: dict[str, tuple] = {
+    "fh_packed_abi_version": (c_int, []),
+    "fh_attn_mask_size": (c_size_t, [_I64]),
+    "fh_attn_mask": (c_int, [_V, _V, _V, _I64, _I64, _I64, _I64, c_int, _V, _V]),
+    "fh_masked_attn_fwd": (c_int, [c_int, _V, _I64, _V, _I64, _V, _I64, _V, _I64, _V, _V, _V, _I64, _I64, _I64, _I64, _F,
+                                   _F, _V, _V]),
+    "fh_masked_attn_bwd_workspace_size": (c_size_t, [c_int, _I64, _I64, _I64, _I64]),
+    "fh_masked_attn_bwd": (c_int, [c_int, _V, _I64, _V, _I64, _V, _I64, _V, _I64, _V, _I64, _V, _V, _V, _I64, _V, _I64,
+                                   _V, _I64, _V, _V, _I64, _I64, _I64, _I64, _F, _F, _V, _V]),
+    "fh_cache_attn_workspace_size": (c_size_t, [c_int, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "fh_cache_attn": (c_int, [c_int, _V, _I64, _V, _I64, _I64, _I64, _V, _I64, _I64, _I64, _V, _I64, _V, _I64, _I64, _I64,
+                              _I64, _I64, _I64, _I64, _F, _F, _V, _V, _V]),
+    "fh_embedding_scaled_fwd": (c_int, [c_int, _V, _V, _V, _I64, _I64, _I64, _F, _V]),
+    "fh_embedding_scaled_bwd": (c_int, [c_int, _V, _V, _V, _I64, _I64, _I64, _I64, _F, _V, _V]),
+    "fh_clip_grads_workspace_size": (c_size_t, [_I64]),
+    "fh_clip_grads": (c_int, [_I64, _V, _F, _V, _V, _V]),
+}
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -162,7 +188,11 @@ def lib() -> ctypes.CDLL:
         got = 0 if blocks is None else blocks()
         if got != BLOCKS_ABI_VERSION:
             raise FemtoHipError(f"libfemtohip blocks ABI {got} != expected {BLOCKS_ABI_VERSION}: rebuild it")
-        for name, (restype, argtypes) in (SIGNATURES | BLOCK_SIGNATURES).items():
+        packed = getattr(handle, "fh_packed_abi_version", None)
+        got = 0 if packed is None else packed()
+        if got != PACKED_ABI_VERSION:
+            raise FemtoHipError(f"libfemtohip packed ABI {got} != expected {PACKED_ABI_VERSION}: rebuild it")
+        for name, (restype, argtypes) in (SIGNATURES | BLOCK_SIGNATURES | PACKED_SIGNATURES).items():
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes

@@ -25,6 +25,7 @@
 // order; no float is ever summed in a run-dependent order.
 #include <type_traits>
 
+#include "femtohip_packed.h"
 #include "fh_common.hpp"
 
 namespace fh {
@@ -39,11 +40,12 @@ constexpr int kBins = 256;                          // 8-bit digits
 size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
 
 // ------------------------------------------------------------- forward
-template <typename T>
+// SCALED: times `factor`, rounded once; without it the row's bits.
+template <typename T, bool SCALED>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_fwd(const T* __restrict__ w,
                                                            const int64_t* __restrict__ ids,
                                                            T* __restrict__ out, int64_t n_tokens,
-                                                           int64_t vocab, int64_t hidden) {
+                                                           int64_t vocab, int64_t hidden, float factor) {
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 6);
   if (t >= n_tokens) return;
   const int lane = threadIdx.x & (kWave - 1);
@@ -52,8 +54,17 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_fwd(const T* __restrict__
   T* dst = out + t * hidden;
   if (ok) {
     const T* src = w + id * hidden;
-    for (int64_t c = lane * 8; c < hidden; c += kWave * 8)
-      Elem<T>::straw(dst + c, Elem<T>::ldraw(src + c));
+    for (int64_t c = lane * 8; c < hidden; c += kWave * 8) {
+      if constexpr (SCALED) {
+        float v[8];
+        Elem<T>::load8(src + c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= factor;
+        Elem<T>::store8(dst + c, v);
+      } else {
+        Elem<T>::straw(dst + c, Elem<T>::ldraw(src + c));
+      }
+    }
   } else {
     const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int64_t c = lane * 8; c < hidden; c += kWave * 8) Elem<T>::store8(dst + c, z);
@@ -311,7 +322,7 @@ constexpr int kHotDepth = sizeof(T) == 2 ? 64 : 32;
 // base, so a token costs two readlanes, a scalar add and a load.
 template <typename T>
 __device__ __forceinline__ void hot_columns(const T* __restrict__ dy, const uint32_t* __restrict__ tok, int n,
-                                            T* __restrict__ dst, int64_t c, int64_t hidden, int lane) {
+                                            T* __restrict__ dst, int64_t c, int64_t hidden, int lane, float factor) {
   using Pair = typename std::conditional<sizeof(T) == 2, uint32_t, float2>::type;
   const bool ok = c < hidden;  // hidden % 8 == 0: a pair is wholly in or out
   const char* col = reinterpret_cast<const char*>(dy + (ok ? c : 0));
@@ -354,6 +365,8 @@ __device__ __forceinline__ void hot_columns(const T* __restrict__ dy, const uint
     }
   }
   if (!ok) return;
+  a0 *= factor;
+  a1 *= factor;
   if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(dst + c) = pk_bf16(a0, a1);
   else *reinterpret_cast<float2*>(dst + c) = make_float2(a0, a1);
 }
@@ -368,7 +381,7 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const T* __restrict_
                                                             const uint32_t* __restrict__ seg_end,
                                                             T* __restrict__ dw, int64_t vocab,
                                                             int64_t hidden, int hot_blocks, int hot_parts,
-                                                            int hot_ids) {
+                                                            int hot_ids, float factor) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int block = blockIdx.x;
@@ -384,7 +397,7 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const T* __restrict_
     for (uint64_t hot = __ballot(len >= kHotTokens); hot != 0; hot &= hot - 1) {
       const int l = __builtin_ctzll(hot);
       hot_columns<T>(dy, tok + __builtin_amdgcn_readlane(lo, l), __builtin_amdgcn_readlane(len, l),
-                     dw + (v0 + l) * hidden, c0 + 2 * lane, hidden, lane);
+                     dw + (v0 + l) * hidden, c0 + 2 * lane, hidden, lane, factor);
     }
     return;
   }
@@ -413,7 +426,11 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const T* __restrict_
     }
 #pragma unroll
     for (int k = 0; k < kRowChunks; ++k)
-      if (c0 + k * kWave * 8 < hidden) Elem<T>::store8(dst + c0 + k * kWave * 8, acc[k]);
+      if (c0 + k * kWave * 8 < hidden) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[k][e] *= factor;
+        Elem<T>::store8(dst + c0 + k * kWave * 8, acc[k]);
+      }
   }
 }
 
@@ -448,9 +465,10 @@ BwdLayout bwd_layout(int64_t n_tokens, int64_t vocab) {
 
 using namespace fh;
 
-extern "C" int fh_embedding_fwd(fh_dtype dt, const void* weight, const int64_t* ids, void* out,
-                                int64_t n_tokens, int64_t vocab, int64_t hidden,
-                                hipStream_t stream) {
+namespace {
+
+int embedding_fwd_impl(fh_dtype dt, const void* weight, const int64_t* ids, void* out, int64_t n_tokens, int64_t vocab,
+                       int64_t hidden, float factor, hipStream_t stream) {
   FH_REQUIRE(dt == FH_BF16 || dt == FH_F32, "embedding_fwd: dtype must be FH_BF16 or FH_F32");
   FH_REQUIRE(n_tokens >= 0 && vocab > 0 && hidden > 0, "embedding_fwd: bad sizes");
   FH_REQUIRE(hidden % 8 == 0, "embedding_fwd: hidden must be a multiple of 8");
@@ -459,15 +477,33 @@ extern "C" int fh_embedding_fwd(fh_dtype dt, const void* weight, const int64_t* 
   FH_REQUIRE(aligned16(weight) && aligned16(out), "embedding_fwd: weight/out must be 16-byte aligned");
   FH_REQUIRE((n_tokens + kRowsPerBlock - 1) / kRowsPerBlock <= 0x7fffffff, "embedding_fwd: too many tokens");
   const dim3 grid(static_cast<unsigned>((n_tokens + kRowsPerBlock - 1) / kRowsPerBlock));
-  if (dt == FH_BF16)
-    hipLaunchKernelGGL(k_embed_fwd<uint16_t>, grid, dim3(kEmbThreads), 0, stream,
-                       static_cast<const uint16_t*>(weight), ids, static_cast<uint16_t*>(out),
-                       n_tokens, vocab, hidden);
-  else
-    hipLaunchKernelGGL(k_embed_fwd<float>, grid, dim3(kEmbThreads), 0, stream,
-                       static_cast<const float*>(weight), ids, static_cast<float*>(out), n_tokens,
-                       vocab, hidden);
+  auto launch = [&](auto tag, auto scaled) {
+    using T = decltype(tag);
+    hipLaunchKernelGGL((k_embed_fwd<T, decltype(scaled)::value>), grid, dim3(kEmbThreads), 0, stream,
+                       static_cast<const T*>(weight), ids, static_cast<T*>(out), n_tokens, vocab, hidden, factor);
+  };
+  auto typed = [&](auto tag) {
+    if (factor == 1.f) launch(tag, std::false_type{});
+    else launch(tag, std::true_type{});
+  };
+  if (dt == FH_BF16) typed(uint16_t{});
+  else typed(float{});
   return check_launch("fh_embedding_fwd");
+}
+
+}  // namespace
+
+extern "C" int fh_embedding_fwd(fh_dtype dt, const void* weight, const int64_t* ids, void* out,
+                                int64_t n_tokens, int64_t vocab, int64_t hidden,
+                                hipStream_t stream) {
+  return embedding_fwd_impl(dt, weight, ids, out, n_tokens, vocab, hidden, 1.f, stream);
+}
+
+extern "C" int fh_embedding_scaled_fwd(fh_dtype dt, const void* weight, const int64_t* ids, void* out,
+                                       int64_t n_tokens, int64_t vocab, int64_t hidden, float factor,
+                                       hipStream_t stream) {
+  FH_REQUIRE(factor - factor == 0.f, "embedding_fwd: factor must be finite");
+  return embedding_fwd_impl(dt, weight, ids, out, n_tokens, vocab, hidden, factor, stream);
 }
 
 extern "C" size_t fh_embedding_bwd_workspace_size(int64_t n_tokens, int64_t vocab) {
@@ -475,9 +511,10 @@ extern "C" size_t fh_embedding_bwd_workspace_size(int64_t n_tokens, int64_t voca
   return bwd_layout(n_tokens, vocab).total;
 }
 
-extern "C" int fh_embedding_bwd(fh_dtype dt, const void* dy, const int64_t* ids, void* dweight,
-                                int64_t n_tokens, int64_t vocab, int64_t hidden,
-                                int64_t padding_idx, void* workspace, hipStream_t stream) {
+namespace {
+
+int embedding_bwd_impl(fh_dtype dt, const void* dy, const int64_t* ids, void* dweight, int64_t n_tokens, int64_t vocab,
+                       int64_t hidden, int64_t padding_idx, float factor, void* workspace, hipStream_t stream) {
   FH_REQUIRE(dt == FH_BF16 || dt == FH_F32, "embedding_bwd: dtype must be FH_BF16 or FH_F32");
   FH_REQUIRE(n_tokens >= 0 && vocab > 0 && hidden > 0, "embedding_bwd: bad sizes");
   FH_REQUIRE(hidden % 8 == 0, "embedding_bwd: hidden must be a multiple of 8");
@@ -533,9 +570,24 @@ extern "C" int fh_embedding_bwd(fh_dtype dt, const void* dy, const int64_t* ids,
     using T = decltype(tag);
     hipLaunchKernelGGL(k_embed_rows<T>, dim3(static_cast<unsigned>(blocks)), dim3(kEmbThreads), 0, stream,
                        static_cast<const T*>(dy), vals[cur], seg_start, seg_end, static_cast<T*>(dweight), vocab,
-                       hidden, static_cast<int>(hot_blocks), static_cast<int>(hot_parts), static_cast<int>(hot_ids));
+                       hidden, static_cast<int>(hot_blocks), static_cast<int>(hot_parts), static_cast<int>(hot_ids), factor);
   };
   if (dt == FH_BF16) rows(uint16_t{});
   else rows(float{});
   return check_launch("fh_embedding_bwd");
+}
+
+}  // namespace
+
+extern "C" int fh_embedding_bwd(fh_dtype dt, const void* dy, const int64_t* ids, void* dweight,
+                                int64_t n_tokens, int64_t vocab, int64_t hidden,
+                                int64_t padding_idx, void* workspace, hipStream_t stream) {
+  return embedding_bwd_impl(dt, dy, ids, dweight, n_tokens, vocab, hidden, padding_idx, 1.f, workspace, stream);
+}
+
+extern "C" int fh_embedding_scaled_bwd(fh_dtype dt, const void* dy, const int64_t* ids, void* dweight,
+                                       int64_t n_tokens, int64_t vocab, int64_t hidden, int64_t padding_idx,
+                                       float factor, void* workspace, hipStream_t stream) {
+  FH_REQUIRE(factor - factor == 0.f, "embedding_bwd: factor must be finite");
+  return embedding_bwd_impl(dt, dy, ids, dweight, n_tokens, vocab, hidden, padding_idx, factor, workspace, stream);
 }

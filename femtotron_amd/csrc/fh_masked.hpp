@@ -1,0 +1,228 @@
+// What the kernels of attention under a mask share: the table of what a token sees,
+// the scores' cap and bias, and products that keep infinities and NaN where they are
+// seen.
+#pragma once
+
+#include "femtohip_packed.h"
+#include "fh_attn.hpp"
+
+namespace fh {
+
+// fh_attn_mask's table.  A row sees keys [x, y) and is seen by queries [z, w); of 32
+// rows `keys` and `queries` hold (smallest first, largest end, largest first, smallest
+// end) over the rows that see (are seen by) something: a range that misses [x, y) has
+// nothing for them, one inside [z, w) is seen by all of them.
+struct MaskTable {
+  const int4* rows;
+  const int4* keys;
+  const int4* queries;
+};
+
+constexpr int kMaskRows = 32;
+
+inline int64_t mask_tiles(int64_t tokens) { return (tokens + kMaskRows - 1) / kMaskRows; }
+
+inline MaskTable mask_table(const void* table, int64_t tokens) {
+  const int4* rows = static_cast<const int4*>(table);
+  return {rows, rows + tokens, rows + tokens + mask_tiles(tokens)};
+}
+
+namespace {
+
+// Ranges' bounds over tiles [t, t + n), those before `tiles` (nothing: x > y).
+__device__ __forceinline__ int4 mask_bounds(const int4* b, int t, int n, int tiles) {
+  int4 r = make_int4(0x7fffffff, 0, 0, 0x7fffffff);
+  for (int i = t; i < min(t + n, tiles); ++i) {
+    const int4 v = b[i];
+    r = make_int4(min(r.x, v.x), max(r.y, v.y), max(r.z, v.z), min(r.w, v.w));
+  }
+  return r;
+}
+
+// --------------------------------------------------------------------- scores
+// Scores in log2 units, from the raw products x = q . k:
+//   z2 = x scale_log2                                      MODE 0
+//   z2 = cap_log2 tanh(x scale / cap)                      kCap
+//   z2 -= slope_log2 |i - j|                               kBias
+// tanh(u) = 1 - 2 r with r = 1 / (1 + e^2u), its derivative 4 r (1 - r): one v_exp and
+// one v_rcp, off by about 2^-23 of tanh's 1 (of `cap` in the scores).
+constexpr int kCap = 1, kBias = 2;
+
+struct ScoreArgs {
+  float scale;       // of the gradients of q and k
+  float scale_log2;  // scale * log2(e)
+  float in;          // scale / cap
+  float in2;         // 2 log2(e) scale / cap
+  float cap_log2;    // cap * log2(e)
+  const float* slopes;
+};
+
+template <int MODE>
+struct Score {
+  float a, b, slope;
+  __device__ __forceinline__ Score(const ScoreArgs& s, int h) {
+    a = (MODE & kCap) ? s.in2 : s.scale_log2;
+    b = s.cap_log2;
+    slope = (MODE & kBias) ? s.slopes[h] * kLog2e : 0.f;
+  }
+  // r of the comment above.
+  __device__ __forceinline__ float half_sigmoid(float x) const {
+    return __builtin_amdgcn_rcpf(1.f + fast_exp2(x * a));
+  }
+  __device__ __forceinline__ float from_r(float r) const { return fmaf(-2.f * b, r, b); }
+  __device__ __forceinline__ float biased(float z, float away) const {
+    return (MODE & kBias) ? fmaf(-slope, fabsf(away), z) : z;
+  }
+  // The score of x, `away` tokens apart.
+  __device__ __forceinline__ float operator()(float x, float away) const {
+    return biased((MODE & kCap) ? from_r(half_sigmoid(x)) : x * a, away);
+  }
+  // e^(z - lse) and the score's derivative by s, nlse2 = -lse * log2(e).
+  __device__ __forceinline__ float weight(float x, float away, float nlse2, float& slope_of) const {
+    if constexpr (MODE & kCap) {
+      const float r = half_sigmoid(x);
+      slope_of = 4.f * fmaf(-r, r, r);
+      return fast_exp2(biased(from_r(r), away) + nlse2);
+    } else {
+      slope_of = 1.f;
+      if constexpr (MODE & kBias) return fast_exp2(fmaf(x, a, fmaf(-slope, fabsf(away), nlse2)));
+      else return fast_exp2(fmaf(x, a, nlse2));
+    }
+  }
+};
+
+// ------------------------------------------------------------ o beyond bf16
+// The four fp32 values x as bf16 (pk_bf16) and the next eight bits of each, signed: what
+// its bits are over those of the bf16 value, in steps of 2^8 (a bf16 step is 2^16).
+__device__ __forceinline__ uint32_t low_bits(const float (&x)[4], uint2 rounded) {
+  const uint32_t r[4] = {rounded.x << 16, rounded.x & 0xffff0000u, rounded.y << 16, rounded.y & 0xffff0000u};
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = static_cast<int>(__float_as_uint(x[i]) - r[i]);  // within +-2^15
+    w |= (static_cast<uint32_t>(min((d + 128) >> 8, 127)) & 0xffu) << (8 * i);
+  }
+  return w;
+}
+
+// A bf16 value's bits (in the high half) with its low_bits byte i of w.
+__device__ __forceinline__ float with_low(uint32_t high, uint32_t w, int i) {
+  return __uint_as_float(high + static_cast<uint32_t>(static_cast<int>(static_cast<int8_t>(w >> (8 * i))) << 8));
+}
+
+// ------------------------------------------------------- what is not seen
+// A weight of 0 does not keep an infinity or a NaN out of a sum on the matrix cores
+// (0 * inf).  A tile that some column sees a part of may bring one from a row that the
+// column does not see; the sums then hold a NaN, for a sum that has met one never loses
+// it.  The kernels therefore look at their finished sums once, and where a column that
+// sees something holds no finite value, the workgroup computes all of it again with
+// wsum_careful in those tiles, at a sixteenth of the speed: what is left are the
+// infinities and NaN that the column does see.
+
+// Whether the sums hold an infinity or a NaN.
+template <int ND>
+__device__ __forceinline__ bool not_finite(const f32x16 (&acc)[ND]) {
+  float s = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s = fmaf(acc[dt][j], 0.f, s);
+  return s != s;
+}
+
+// acc += X^T f over rows row0 .. row0+15 of the tile X, of which this lane's column sees
+// those n with first + n < count (unsigned): one row at a time, the others zero, and the
+// columns that do not see it keep their sums.
+template <int HD>
+__device__ __forceinline__ void wsum_careful(f32x16 (&acc)[HD / 32], bf16x8 f, const char* tile, int b0, int b8,
+                                             int row0, unsigned first, unsigned count, int hl) {
+#pragma unroll 1
+  for (int n = 0; n < 16; ++n) {
+    // Row n is element e of the lanes of one half (the permuted order of lds_frag_tr).
+    const int e = (n & 3) + ((n >> 3) << 2);
+    const bool mine = hl == ((n >> 2) & 1);
+    const uint32_t m = (e & 1) ? 0xffff0000u : 0x0000ffffu;
+    const uint32_t m0 = mine && (e >> 1) == 0 ? m : 0, m1 = mine && (e >> 1) == 1 ? m : 0;
+    const uint32_t m2 = mine && (e >> 1) == 2 ? m : 0, m3 = mine && (e >> 1) == 3 ? m : 0;
+    const bool seen = first + n < count;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt) {
+      const uint4 u = __builtin_bit_cast(uint4, lds_frag_tr<HD>(tile, b0, b8, row0, dt));
+      const f32x16 t = mfma(as_bf16x8(make_uint4(u.x & m0, u.y & m1, u.z & m2, u.w & m3)), f, acc[dt]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[dt][j] = seen ? t[j] : acc[dt][j];
+    }
+  }
+}
+
+// acc += X^T f over rows row0 .. row0+15 of the tile X.
+template <int HD>
+__device__ __forceinline__ void wsum(f32x16 (&acc)[HD / 32], bf16x8 f, const char* tile, int b0, int b8, int row0) {
+#pragma unroll
+  for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = mfma(lds_frag_tr<HD>(tile, b0, b8, row0, dt), f, acc[dt]);
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------ host
+// The checks and constants of a call, for every dtype.
+struct MaskedArgs {
+  int64_t tokens, n_heads, n_kv_heads, head_dim;
+  ScoreArgs score;
+  int mode;
+};
+
+int masked_args(const char* name, fh_dtype dt, int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                float scale, float cap, const float* slopes, MaskedArgs& a);
+
+// A row stride of heads of head_dim.
+int masked_stride(const char* name, const char* what, int64_t ld, int64_t heads, int64_t head_dim);
+
+struct MaskedFwd {
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv;
+  void* o;
+  int64_t ldo;
+  float* lse;
+  int8_t* o_low;
+  MaskTable table;
+};
+
+struct MaskedBwd {
+  const void *q, *k, *v, *o, *dout;
+  int64_t ldq, ldk, ldv, ldo, lddo;
+  const float* lse;
+  const int8_t* o_low;
+  void *dq, *dk, *dv;
+  int64_t lddq, lddk, lddv;
+  MaskTable table;
+  float* workspace;
+};
+
+void masked_fwd_bf16(const MaskedFwd& c, const MaskedArgs& a, hipStream_t stream);
+void masked_bwd_bf16(const MaskedBwd& c, const MaskedArgs& a, hipStream_t stream);
+void masked_fwd_f32(const MaskedFwd& c, const MaskedArgs& a, hipStream_t stream);
+void masked_bwd_f32(const MaskedBwd& c, const MaskedArgs& a, hipStream_t stream);
+
+// Workspace of the backward, in floats: delta and -lse * log2(e) [n_heads, tokens], then
+// from `parts` on the sums of a kv head's query heads where they are split.
+struct MaskedWorkspace {
+  int64_t parts, total;
+  int split;
+};
+MaskedWorkspace masked_workspace(fh_dtype dt, int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim);
+
+template <typename F>
+void dispatch_masked(int64_t head_dim, int mode, F&& f) {
+  auto with_mode = [&](auto hd) {
+    if (mode == 0) f(hd, std::integral_constant<int, 0>{});
+    else if (mode == kCap) f(hd, std::integral_constant<int, kCap>{});
+    else if (mode == kBias) f(hd, std::integral_constant<int, kBias>{});
+    else f(hd, std::integral_constant<int, kCap | kBias>{});
+  };
+  if (head_dim == 32) with_mode(std::integral_constant<int, 32>{});
+  else if (head_dim == 64) with_mode(std::integral_constant<int, 64>{});
+  else with_mode(std::integral_constant<int, 128>{});
+}
+
+}  // namespace fh

@@ -1,0 +1,196 @@
+// Attention under a mask, bf16 forward.
+//
+// The layout and the products are those of the causal kernel (fh_attention.hip): four
+// waves of 32 queries of one head, 64 keys a step, S^T = K Q^T with one query a lane,
+// an online softmax in fp32, O^T += V^T P^T.  Here the steps run over what the
+// workgroup's 128 queries see, from the first of those keys on: keys that none of them
+// sees are not read, a wave skips steps that its own 32 do not see, and only steps of
+// which some query sees a part are masked.
+#include <type_traits>
+
+#include "fh_masked.hpp"
+
+namespace fh {
+namespace {
+
+// Finite, so that a query without a key yet has weights 0 and not exp2(-inf + inf).
+constexpr float kNoMax = -3.0e38f;
+
+// One step of a wave: raw scores of 64 keys from K, the update of (m, l, oacc), and
+// oacc += V^T P^T.  base = the query's row - k0 - 4 hl; its keys are those at c (of the
+// step, less 4 hl) with c - lo < count.
+template <int HD, int MODE, bool CAREFUL>
+__device__ __forceinline__ void masked_step(const char* K, const char* V, const bf16x8 (&qf)[HD / 16],
+                                            f32x16 (&oacc)[HD / 32], float& m, float& l, int a_off, int b0, int b8,
+                                            const Score<MODE>& score, float base, bool whole, int lo, unsigned count,
+                                            int hl) {
+  constexpr int BN = 64, NS = HD / 16, ND = HD / 32;
+  f32x16 x[BN / 32];
+  __builtin_amdgcn_iglp_opt(0);  // LDS reads interleaved with MFMAs
+#pragma unroll
+  for (int t = 0; t < BN / 32; ++t) {
+    x[t] = zero16();
+#pragma unroll
+    for (int s = 0; s < NS; ++s) x[t] = mfma(lds_frag<HD>(K, a_off, 32 * t, s), qf[s], x[t]);
+  }
+  if constexpr (MODE != 0) {
+#pragma unroll
+    for (int t = 0; t < BN / 32; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[t][j] = score(x[t][j], base - (32 * t + acc_row(j, 0)));
+  }
+  float mloc = -INFINITY;
+  if (!whole) {
+#pragma unroll
+    for (int t = 0; t < BN / 32; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        x[t][j] = static_cast<unsigned>(32 * t + acc_row(j, 0) - lo) < count ? x[t][j] : -INFINITY;
+        mloc = fmaxf(mloc, x[t][j]);
+      }
+  } else {
+#pragma unroll
+    for (int t = 0; t < BN / 32; ++t)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mloc = fmaxf(mloc, x[t][j]);
+  }
+  mloc = xor32_max(mloc);
+  if constexpr (MODE == 0) mloc *= score.a;
+  if (wave_any(mloc > m + kRescaleSlack)) {
+    const float mnew = fmaxf(m, mloc);
+    const float alpha = fast_exp2(m - mnew);
+    m = mnew;
+    l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) oacc[dt][j] *= alpha;
+  }
+  const float nm = -m;
+#pragma unroll
+  for (int t = 0; t < BN / 32; ++t)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[t][j] = fast_exp2(MODE == 0 ? fmaf(x[t][j], score.a, nm) : x[t][j] + nm);
+  // The row sums add the bf16 weights that P V multiplies, so that the normalisation
+  // matches the weights used.
+  float lsum = 0.f;
+#pragma unroll
+  for (int s = 0; s < BN / 16; ++s) {
+    const bf16x8 pf = pack_frag(x[s >> 1], 8 * (s & 1));
+    lsum = sum_bf16x8(pf, lsum);
+    if constexpr (CAREFUL) {
+      if (!whole) {  // lo counts from the step's first key less 4 hl
+        wsum_careful<HD>(oacc, pf, V, b0, b8, 16 * s, static_cast<unsigned>(16 * s - (lo + 4 * hl)), count, hl);
+        continue;
+      }
+    }
+    wsum<HD>(oacc, pf, V, b0, b8, 16 * s);
+  }
+  l += lsum;
+}
+
+// HPB = 2: 8 waves take the same rows of two query heads of one kv head, which read the
+// same K and V tiles.
+template <int HD, int HPB, int MODE>
+__global__ __launch_bounds__(256 * HPB) __attribute__((amdgpu_waves_per_eu(2))) void k_masked_fwd(
+    const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
+    const uint16_t* __restrict__ v, int64_t ldv, uint16_t* __restrict__ o, int64_t ldo, float* __restrict__ lse,
+    int8_t* __restrict__ o_low, int T, int group, ScoreArgs args, MaskTable mask) {
+  constexpr int BM = 128, BN = 64, NS = HD / 16, ND = HD / 32, TILE = BN * 2 * HD;
+  // Three K/V stages up to head_dim 64 (48 KB); at 128 they would leave room for one
+  // workgroup a CU.
+  constexpr int STAGES = HD <= 64 ? 3 : 2, TILE3 = STAGES == 3 ? TILE : 16;
+  __shared__ __align__(16) char sk0[TILE], sk1[TILE], sk2[TILE3], sv0[TILE], sv1[TILE], sv2[TILE3];
+  const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const XcdOrder ord = xcd_order();
+  const int h = ord.y * HPB + (wave >> 2), kvh = h / group;
+  const int q0 = (gridDim.x - 1 - ord.rank) * BM;  // the latest queries, which see most, first
+  const int qw = q0 + (wave & 3) * 32, qi = qw + l32;
+  const int tiles = (T + kMaskRows - 1) / kMaskRows;
+  const int4 all = mask_bounds(mask.keys, q0 / kMaskRows, BM / kMaskRows, tiles);
+  const int4 mine = mask_bounds(mask.keys, qw / kMaskRows, 1, tiles);
+  const int2 sees = qi < T ? *reinterpret_cast<const int2*>(mask.rows + qi) : make_int2(0, 0);
+  const int kbeg = all.x, n_steps = all.y > all.x ? (all.y - all.x + BN - 1) / BN : 0;
+  const Score<MODE> score(args, h);
+  int a_off = lane_off_a<HD>(lane);
+  int b0 = lane_off_b<HD>(lane, 0), b8 = lane_off_b<HD>(lane, 8);
+
+  bf16x8 qf[NS];
+  auto load_q = [&]() __attribute__((always_inline)) {
+    const uint16_t* qrow = q + static_cast<int64_t>(qi) * ldq + static_cast<int64_t>(h) * HD + 8 * hl;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = qi < T ? ld_frag(qrow + 16 * s) : as_bf16x8(make_uint4(0, 0, 0, 0));
+  };
+  f32x16 oacc[ND];
+  float m, l;
+  const bool some = sees.x < sees.y;
+  if (n_steps > 0) {  // uniform
+    const uint16_t* kp = k + static_cast<int64_t>(kbeg) * ldk + static_cast<int64_t>(kvh) * HD;
+    const uint16_t* vp = v + static_cast<int64_t>(kbeg) * ldv + static_cast<int64_t>(kvh) * HD;
+    auto run = [&](auto careful) __attribute__((always_inline)) {
+      m = kNoMax;
+      l = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) oacc[dt] = zero16();
+      auto body = [&](int kb, const char* K, const char* V) __attribute__((always_inline)) {
+        refresh_offsets(a_off, b0, b8);
+        const int k0 = kbeg + kb * BN;
+        if (mine.x >= k0 + BN || mine.y <= k0) return;  // nothing for this wave's queries
+        masked_step<HD, MODE, decltype(careful)::value>(K, V, qf, oacc, m, l, a_off, b0, b8, score,
+                                                        static_cast<float>(qi - k0 - 4 * hl),
+                                                        mine.z <= k0 && mine.w >= k0 + BN, sees.x - k0 - 4 * hl,
+                                                        static_cast<unsigned>(sees.y - sees.x), hl);
+      };
+      if constexpr (STAGES == 3)
+        kv_block_loop3<BN, HD, 4 * HPB>(kp, ldk, vp, ldv, n_steps, T - kbeg, sk0, sk1, sk2, sv0, sv1, sv2, wave, lane,
+                                        body, load_q);
+      else
+        kv_block_loop<BN, HD, true, 4 * HPB>(kp, ldk, vp, ldv, n_steps, T - kbeg, sk0, sk1, sv0, sv1, wave, lane, body,
+                                             load_q);
+    };
+    run(std::false_type{});
+    if (__builtin_expect(__syncthreads_or(some && not_finite<ND>(oacc)), 0)) run(std::true_type{});
+  }
+  if (qi < T) {
+    const float lt = n_steps > 0 ? xor32_sum(l) : 0.f;
+    if (!some) {
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt) oacc[dt] = zero16();
+    }
+    const float mul = some ? 1.f / lt : 0.f;
+    uint16_t* row = o + static_cast<int64_t>(qi) * ldo + static_cast<int64_t>(h) * HD + 4 * hl;
+    int8_t* low = o_low + static_cast<int64_t>(qi) * (gridDim.y * HPB * HD) + static_cast<int64_t>(h) * HD + 4 * hl;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float x[4] = {oacc[dt][4 * g] * mul, oacc[dt][4 * g + 1] * mul, oacc[dt][4 * g + 2] * mul,
+                            oacc[dt][4 * g + 3] * mul};
+        const uint2 w = make_uint2(pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]));
+        *reinterpret_cast<uint2*>(row + dt * 32 + 8 * g) = w;
+        if (o_low != nullptr) *reinterpret_cast<uint32_t*>(low + dt * 32 + 8 * g) = low_bits(x, w);
+      }
+    if (lse != nullptr && hl == 0) lse[static_cast<int64_t>(h) * T + qi] = some ? (m + log2f(lt)) * kLn2 : 0.f;
+  }
+}
+
+}  // namespace
+
+void masked_fwd_bf16(const MaskedFwd& c, const MaskedArgs& a, hipStream_t stream) {
+  const int group = static_cast<int>(a.n_heads / a.n_kv_heads);
+  const bool pair = group % 2 == 0 && (a.n_heads / 2) % 8 == 0;
+  const dim3 grid(static_cast<unsigned>((a.tokens + 127) / 128), static_cast<unsigned>(a.n_heads / (pair ? 2 : 1)));
+  dispatch_masked(a.head_dim, a.mode, [&](auto hd, auto mode) {
+    auto launch = [&](auto hpb) {
+      hipLaunchKernelGGL((k_masked_fwd<hd(), hpb(), mode()>), grid, dim3(256 * hpb()), 0, stream,
+                         static_cast<const uint16_t*>(c.q), c.ldq, static_cast<const uint16_t*>(c.k), c.ldk,
+                         static_cast<const uint16_t*>(c.v), c.ldv, static_cast<uint16_t*>(c.o), c.ldo, c.lse, c.o_low,
+                         static_cast<int>(a.tokens), group, a.score, c.table);
+    };
+    if (pair) launch(std::integral_constant<int, 2>{});
+    else launch(std::integral_constant<int, 1>{});
+  });
+}
+
+}  // namespace fh

@@ -675,6 +675,146 @@ def attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
     _lib.call("fh_attn_bwd_rope", *args, _ptr(cos2), _ptr(sin2), per_token, _stream(q))
 
 
+# ----------------------------------------------------- attention under a mask
+def _int64_vector(name: str, t: torch.Tensor, n: int | None, dev: int) -> None:
+    if t.get_device() != dev or dev < 0:
+        raise ValueError(f"{name} must be on the mask's HIP device")
+    if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous int64 vector, got {t.dtype} {tuple(t.shape)}")
+    if n is not None and t.numel() != n:
+        raise ValueError(f"{name} must have one entry a document, {n}, got {t.numel()}")
+
+
+def attn_mask(tokens: int, seq_len: int, starts: torch.Tensor | None, lengths: torch.Tensor | None,
+              prefix: torch.Tensor | None, window: int, causal: bool, device: torch.device) -> torch.Tensor:
+    """The table of what each of `tokens` rows sees (fh_attn_mask): documents at rows starts
+    (int64, ascending) of lengths (None: up to the next), or, starts None, one for each
+    seq_len rows; window 0: none."""
+    dev = device.index if device.index is not None else torch.cuda.current_device()
+    n = tokens // max(seq_len, 1) if starts is None else starts.numel()
+    if starts is not None:
+        _int64_vector("attention_mask: starts", starts, None, dev)
+    for t, name in ((lengths, "lengths"), (prefix, "prefix")):
+        if t is not None:
+            _int64_vector("attention_mask: " + name, t, n, dev)
+    nbytes = _lib.lib().fh_attn_mask_size(tokens)
+    table = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _launch("fh_attn_mask", table, _ptr(starts), _ptr(lengths), _ptr(prefix), n, tokens, seq_len, window, int(causal),
+            _ptr(table))
+    return table
+
+
+def _masked_operands(name: str, tokens: int, head_dim: int, table: torch.Tensor, slopes: torch.Tensor | None,
+                     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> tuple[int, int]:
+    """(n_heads, n_kv_heads) of token-major q, k, v, checked."""
+    _alike(q, k, v)
+    if table.get_device() != q.get_device():
+        _require_gpu(q, table)
+    for t, n in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 2 or t.size(0) != tokens or t.size(1) % head_dim:
+            raise ValueError(f"{name}: {n} must be [{tokens}, heads * {head_dim}], got {tuple(t.shape)}")
+    if k.size(1) != v.size(1):
+        raise ValueError(f"{name}: k and v have {k.size(1)} and {v.size(1)} columns")
+    if table.dtype != torch.uint8 or table.numel() != _lib.lib().fh_attn_mask_size(tokens):
+        raise ValueError(f"{name}: the mask is not one of {tokens} tokens")
+    n_heads = q.size(1) // head_dim
+    if slopes is not None:
+        if slopes.get_device() != q.get_device():
+            _require_gpu(q, slopes)
+        if slopes.dtype != torch.float32 or slopes.numel() != n_heads or not slopes.is_contiguous():
+            raise ValueError(f"{name}: slopes must be contiguous fp32 with one entry a query head, {n_heads}")
+    return n_heads, k.size(1) // head_dim
+
+
+def _ld(t: torch.Tensor, name: str) -> int:
+    """The row stride of a 2-D view (of one row, which has none, its width)."""
+    ld = _rowmajor(t, name)
+    return ld if t.size(0) > 1 else t.size(1)
+
+
+def masked_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, *, head_dim: int,
+                    scale: float, cap: float = 0.0, slopes: torch.Tensor | None = None,
+                    need_grad: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Attention of token-major q [T, heads * head_dim] over k and v [T, kv heads * head_dim]
+    under attn_mask's table (fh_masked_attn_fwd): (o, lse, o_low), the latter two what
+    masked_attn_bwd reads (None without need_grad; o_low of bf16 only).  cap 0: scores are
+    not capped."""
+    T = q.size(0)
+    nh, nkv = _masked_operands("masked_attn_fwd", T, head_dim, table, slopes, q, k, v)
+    dt = _dtype_code(q)
+    o = torch.empty(T, q.size(1), dtype=q.dtype, device=q.device)
+    lse = low = None
+    if need_grad:
+        lse = torch.empty(nh, T, dtype=torch.float32, device=q.device)
+        low = torch.empty(o.shape, dtype=torch.int8, device=q.device) if dt == _lib.FH_BF16 else None
+    _launch("fh_masked_attn_fwd", q, dt, _ptr(q), _ld(q, "q"), _ptr(k), _ld(k, "k"), _ptr(v), _ld(v, "v"),
+            _ptr(o), o.size(1), _ptr(lse), _ptr(low), _ptr(table), T, nh, nkv, head_dim, scale, cap, _ptr(slopes))
+    return o, lse, low
+
+
+def masked_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, dout: torch.Tensor,
+                    lse: torch.Tensor, o_low: torch.Tensor | None, table: torch.Tensor, *, head_dim: int, scale: float,
+                    cap: float = 0.0, slopes: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of masked_attn_fwd for dout, with its o, lse and o_low: (dq, dk, dv)."""
+    T = q.size(0)
+    nh, nkv = _masked_operands("masked_attn_bwd", T, head_dim, table, slopes, q, k, v)
+    _alike(q, o, dout)
+    if o.shape != q.shape or dout.shape != q.shape:
+        raise ValueError("masked_attn_bwd: o and dout must have q's shape")
+    if lse.get_device() != q.get_device() or lse.dtype != torch.float32 or lse.numel() != nh * T or not lse.is_contiguous():
+        raise ValueError("masked_attn_bwd: lse must be contiguous fp32 [heads, tokens]")
+    dt = _dtype_code(q)
+    if (o_low is None) == (dt == _lib.FH_BF16):
+        raise ValueError("masked_attn_bwd: o_low goes with bf16")
+    if o_low is not None and (o_low.get_device() != q.get_device() or o_low.dtype != torch.int8 or o_low.shape != q.shape
+                              or not o_low.is_contiguous()):
+        raise ValueError("masked_attn_bwd: o_low must be contiguous int8 of q's shape")
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    nbytes = _lib.lib().fh_masked_attn_bwd_workspace_size(dt, T, nh, nkv, head_dim)
+    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=q.device)
+    _launch("fh_masked_attn_bwd", q, dt, _ptr(q), _ld(q, "q"), _ptr(k), _ld(k, "k"), _ptr(v), _ld(v, "v"), _ptr(o),
+            _ld(o, "o"), _ptr(dout), _ld(dout, "dout"), _ptr(lse), _ptr(o_low), _ptr(dq), dq.size(1), _ptr(dk), dk.size(1), _ptr(dv),
+            dv.size(1), _ptr(table), _ptr(ws), T, nh, nkv, head_dim, scale, cap, _ptr(slopes))
+    return dq, dk, dv
+
+
+def cache_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, n_new: int, scale: float,
+               cap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0) -> torch.Tensor:
+    """Attention of token-major q [batch * n_new, heads * head_dim] over caches k and v [batch,
+    room, kv heads, head_dim] (views of any strides whose last dim is contiguous), the new
+    tokens being each sequence's last of lengths (int64 [batch]) places (fh_cache_attn)."""
+    _alike(q, k, v)
+    if k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"cache_attn: k and v must be [batch, room, kv heads, head_dim], got {tuple(k.shape)}, {tuple(v.shape)}")
+    batch, room, nkv, head_dim = k.shape
+    if q.dim() != 2 or q.size(0) != batch * n_new or q.size(1) % head_dim:
+        raise ValueError(f"cache_attn: q must be [{batch} * {n_new}, heads * {head_dim}], got {tuple(q.shape)}")
+    nh = q.size(1) // head_dim
+    if lengths.get_device() != q.get_device():
+        _require_gpu(q, lengths)
+    if lengths.dtype != torch.int64 or lengths.shape != (batch,) or not lengths.is_contiguous():
+        raise ValueError(f"cache_attn: lengths must be contiguous int64 [{batch}], got {lengths.dtype} {tuple(lengths.shape)}")
+    if slopes is not None:
+        if slopes.get_device() != q.get_device():
+            _require_gpu(q, slopes)
+        if slopes.dtype != torch.float32 or slopes.numel() != nh or not slopes.is_contiguous():
+            raise ValueError(f"cache_attn: slopes must be contiguous fp32 with one entry a query head, {nh}")
+    strides = []
+    for t, n in ((k, "k"), (v, "v")):
+        sb, sr, sh, unit = t.stride()
+        if unit != 1:
+            raise ValueError(f"cache_attn: {n}'s last dim must be contiguous, got strides {t.stride()}")
+        # the stride of a dim of one is anything
+        strides += [sb if batch > 1 else 0, sr if room > 1 else head_dim, sh if nkv > 1 else 0]
+    dt = _dtype_code(q)
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    nbytes = _lib.lib().fh_cache_attn_workspace_size(dt, batch, n_new, room, nh, nkv, head_dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch("fh_cache_attn", q, dt, _ptr(q), _ld(q, "q"), _ptr(k), *strides[:3], _ptr(v), *strides[3:], _ptr(o), o.size(1),
+            _ptr(lengths), batch, n_new, room, nh, nkv, head_dim, window, scale, cap, _ptr(slopes), _ptr(ws))
+    return o
+
+
 # ------------------------------------------------------------- loss head
 def ce_fwd_bwd_(logits: torch.Tensor, labels: torch.Tensor, inv_count: torch.Tensor,
                 ignore_index: int = -100) -> torch.Tensor:
@@ -708,20 +848,23 @@ def _embedding_args(weight: torch.Tensor, ids: torch.Tensor) -> tuple[int, int]:
     return vocab, hidden
 
 
-def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
-    """weight[ids] with zero rows for ids outside [0, vocab): [*ids.shape, hidden]."""
-    _require_gpu(ids, weight)
+def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, factor: float = 1.0) -> torch.Tensor:
+    """factor * weight[ids] (rounded once) with zero rows for ids outside [0, vocab):
+    [*ids.shape, hidden]."""
+    _alike(weight)
+    if ids.get_device() != weight.get_device():
+        _require_gpu(ids, weight)
     vocab, hidden = _embedding_args(weight, ids)
     out = torch.empty(*ids.shape, hidden, dtype=weight.dtype, device=weight.device)
-    _lib.call("fh_embedding_fwd", _dtype_code(weight), _ptr(weight), _ptr(ids), _ptr(out),
-              ids.numel(), vocab, hidden, _stream(weight))
+    _launch("fh_embedding_scaled_fwd", weight, _dtype_code(weight), _ptr(weight), _ptr(ids), _ptr(out), ids.numel(), vocab,
+            hidden, factor)
     return out
 
 
-def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, vocab: int,
-                  padding_idx: int | None = None) -> torch.Tensor:
-    """Weight gradient of the lookup: [vocab, hidden], row v = sum of the dy rows
-    of the tokens with id v (fp32, token order), zero for unused ids; tokens with
+def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, vocab: int, padding_idx: int | None = None,
+                  factor: float = 1.0) -> torch.Tensor:
+    """Weight gradient of the lookup: [vocab, hidden], row v = factor times the sum of the dy
+    rows of the tokens with id v (fp32, token order), zero for unused ids; tokens with
     an id outside [0, vocab) or equal to padding_idx contribute nothing."""
     _require_gpu(dy, ids)
     hidden = dy.size(-1)
@@ -735,9 +878,41 @@ def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, vocab: int,
     n = ids.numel()
     ws = torch.empty(_lib.lib().fh_embedding_bwd_workspace_size(n, vocab), dtype=torch.uint8,
                      device=dy.device)
-    _lib.call("fh_embedding_bwd", _dtype_code(dy), _ptr(dy), _ptr(ids), _ptr(dw), n, vocab, hidden,
-              -1 if padding_idx is None else int(padding_idx), _ptr(ws), _stream(dy))
+    _launch("fh_embedding_scaled_bwd", dy, _dtype_code(dy), _ptr(dy), _ptr(ids), _ptr(dw), n, vocab, hidden,
+            -1 if padding_idx is None else int(padding_idx), factor, _ptr(ws))
     return dw
+
+
+# ------------------------------------------------------------- gradient norm
+def clip_grads(grads: list, outs: list | None, max_norm: float) -> torch.Tensor:
+    """The 2-norm of all grads (a one-element fp32 tensor) and, with outs, each of them times
+    min(1, max_norm / (norm + 1e-6)) (fh_clip_grads).  Tensors are dense, an out of its
+    gradient's strides, and on one device; an out may be its gradient."""
+    table = (_lib.FhGrad * len(grads))()
+    first = grads[0]
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError("femtohip ops take HIP device tensors only")
+    for i, g in enumerate(grads):
+        o = None if outs is None else outs[i]
+        t = table[i]
+        for x in (g, o):
+            if x is None:
+                continue
+            if x.get_device() != dev:
+                _require_gpu(first, x)
+            if x.layout != torch.strided or not (x.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(x)):
+                raise ValueError("clip_gradients: gradients must be dense")
+        if o is not None:
+            if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))):
+                raise ValueError(f"clip_gradients: an output must have its gradient's shape and strides, got "
+                                 f"{tuple(o.shape)} {o.stride()} for {tuple(g.shape)} {g.stride()}")
+            t.out, t.out_dtype = o.data_ptr(), _dtype_code(o)
+        t.grad, t.numel, t.grad_dtype = g.data_ptr(), g.numel(), _dtype_code(g)
+    norm = torch.empty((), dtype=torch.float32, device=first.device)
+    ws = torch.empty(_lib.lib().fh_clip_grads_workspace_size(len(grads)), dtype=torch.uint8, device=first.device)
+    _launch("fh_clip_grads", first, len(grads), ctypes.addressof(table), max_norm, _ptr(norm), _ptr(ws))
+    return norm
 
 
 # ------------------------------------------------------------- decoder layer

@@ -24,7 +24,7 @@ from typing import Iterable
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from ._lib import FhAdamHyper
 
 CHUNK = 2048  # elements per workgroup of fh_adamw_step
@@ -215,3 +215,43 @@ class FusedAdamW(torch.optim.Optimizer):
                 self.state[p]["step"] = int(st.get("step", state_dict.get("fused_step", 0)))
         self.step_count = int(state_dict.get("fused_step", 0))
         self._cache = None
+
+
+def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *,
+                   out: Iterable[torch.Tensor] | None = None) -> torch.Tensor:
+    """Multiplies all ``grads`` (bf16 and fp32, on one HIP device) by min(1, max_norm / (norm +
+    1e-6)), norm being their joint 2-norm, in place, or into ``out`` (one tensor a gradient,
+    either type: the fp32 gradients of an optimizer's own copies need no cast of their own).
+    Returns the norm, a device scalar that is not waited for.
+
+    The reference's ``ClipGradNorm`` (femtotron/training/grad_transform.py:13-63) for programs
+    whose optimizer is not ``FusedAdamW`` (which clips by itself).  The sum of squares is fp64
+    in a fixed order.  A norm that is NaN makes every gradient NaN, as torch's has it.  A
+    tensor may not stand in the list twice, nor overlap another."""
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"clip_gradients: {len(outs)} outputs for {len(grads)} gradients")
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_gradients: max_norm must not be negative, got {max_norm}")
+    if not grads:
+        return torch.zeros(())
+    with torch.no_grad():
+        norm = ops.clip_grads(grads, outs, max_norm)
+        torch.autograd.graph.increment_version(outs)  # the kernels' writes, as torch's own would be seen
+    return norm
+
+
+def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """``clip_gradients`` of the parameters' ``.grad`` (those that have one), in place, as
+    torch.nn.utils.clip_grad_norm_ is called."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return clip_gradients([p.grad for p in parameters if p.grad is not None], max_norm)
+
+
+def gradient_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
+    """The joint 2-norm of ``grads``, a device scalar, in one pass over them."""
+    grads = list(grads)
+    return ops.clip_grads(grads, None, 0.0) if grads else torch.zeros(())

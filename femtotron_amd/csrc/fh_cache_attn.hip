@@ -153,7 +153,7 @@ __device__ __forceinline__ void cache_tile(const char* K, const char* V, const b
     l = sum_bf16x8(pf, l);
     if constexpr (CAREFUL) {
       if (!whole) {
-        wsum_careful<HD>(oacc, pf, V, b0, b8, 16 * s, static_cast<unsigned>(16 * s - (lo + 4 * hl)), count, hl);
+        wsum_careful<HD>(oacc, pf, V, b0, b8, 16 * s, lo + 4 * hl, lo + 4 * hl + static_cast<int>(count), hl);
         continue;
       }
     }

@@ -87,6 +87,44 @@ __global__ __launch_bounds__(kMaskThreads) void k_attn_mask(MaskDocs docs, int T
   }
 }
 
+// Blocks of ROWS rows by falling length of what they look at, one workgroup for each of the
+// table's orders: a counting sort in LDS.  (Blocks of one length come in any order, which no
+// result depends on.)
+__global__ __launch_bounds__(1024) void k_mask_order(MaskTable m, int T, int* __restrict__ order_q,
+                                                     int* __restrict__ order_k128, int* __restrict__ order_k64) {
+  __shared__ int at[1024];
+  const int which = blockIdx.x, rows = which == 2 ? 64 : 128;
+  const int4* bounds = which == 0 ? m.keys : m.queries;
+  int* order = which == 0 ? order_q : which == 1 ? order_k128 : order_k64;
+  const int n = (T + rows - 1) / rows, tiles = (T + kMaskRows - 1) / kMaskRows, per = rows / kMaskRows;
+  const int unit = max(32, (T + 1022) / 1023);
+  auto bucket = [&](int i) {
+    int lo = 0x7fffffff, hi = 0;
+    for (int t = i * per; t < min((i + 1) * per, tiles); ++t) {
+      lo = min(lo, bounds[t].x);
+      hi = max(hi, bounds[t].y);
+    }
+    return hi > lo ? 1023 - min(1023, (hi - lo + unit - 1) / unit) : 1023;
+  };
+  const int tid = threadIdx.x;
+  at[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) atomicAdd(&at[bucket(i)], 1);
+  __syncthreads();
+  const int mine = at[tid];
+  for (int off = 1; off < 1024; off <<= 1) {
+    const int add = tid >= off ? at[tid - off] : 0;
+    __syncthreads();
+    at[tid] += add;
+    __syncthreads();
+  }
+  const int first = at[tid] - mine;
+  __syncthreads();
+  at[tid] = first;
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) order[atomicAdd(&at[bucket(i)], 1)] = i;
+}
+
 int check_tokens(const char* name, int64_t tokens) {
   if (tokens < 0 || tokens > (int64_t(1) << 30)) return fail(FH_ERR_INVALID, std::string(name) + ": tokens must be 0 to 2^30");
   return FH_OK;
@@ -135,7 +173,7 @@ extern "C" int fh_packed_abi_version(void) { return FH_PACKED_ABI_VERSION; }
 
 extern "C" size_t fh_attn_mask_size(int64_t tokens) {
   if (tokens <= 0 || tokens > (int64_t(1) << 30)) return 0;
-  return static_cast<size_t>(tokens + 2 * mask_tiles(tokens)) * sizeof(int4);
+  return mask_bytes(tokens);
 }
 
 extern "C" int fh_attn_mask(const int64_t* starts, const int64_t* lengths, const int64_t* prefix, int64_t n_documents,
@@ -157,6 +195,9 @@ extern "C" int fh_attn_mask(const int64_t* starts, const int64_t* lengths, const
                      MaskDocs{starts, lengths, prefix, n_documents, static_cast<int>(starts != nullptr ? 1 : seq_len)},
                      static_cast<int>(tokens), static_cast<int>(window < most ? window : most), causal ? 1 : 0,
                      const_cast<int4*>(m.rows), const_cast<int4*>(m.keys), const_cast<int4*>(m.queries));
+  if (m.order_q != nullptr)
+    hipLaunchKernelGGL(k_mask_order, dim3(3), dim3(1024), 0, stream, m, static_cast<int>(tokens),
+                       const_cast<int*>(m.order_q), const_cast<int*>(m.order_k128), const_cast<int*>(m.order_k64));
   return check_launch("fh_attn_mask");
 }
 

@@ -8,7 +8,8 @@
 
 namespace fh {
 
-// fh_attn_mask's table.  A row sees keys [x, y) and is seen by queries [z, w); of 32
+// fh_attn_mask's table: a row's ranges, their bounds over 32 rows, and for more than
+// kOrderedRows rows the blocks of 128 queries, 128 keys and 64 keys by falling work.  A row sees keys [x, y) and is seen by queries [z, w); of 32
 // rows `keys` and `queries` hold (smallest first, largest end, largest first, smallest
 // end) over the rows that see (are seen by) something: a range that misses [x, y) has
 // nothing for them, one inside [z, w) is seen by all of them.
@@ -16,27 +17,58 @@ struct MaskTable {
   const int4* rows;
   const int4* keys;
   const int4* queries;
+  const int* order_q;  // null: as they come
+  const int* order_k128;
+  const int* order_k64;
 };
 
 constexpr int kMaskRows = 32;
+// Up to here a head's blocks run at once whatever their order.
+constexpr int64_t kOrderedRows = 1024;
 
 inline int64_t mask_tiles(int64_t tokens) { return (tokens + kMaskRows - 1) / kMaskRows; }
+inline int64_t mask_blocks(int64_t tokens, int64_t rows) { return (tokens + rows - 1) / rows; }
+
+inline size_t mask_bytes(int64_t tokens) {
+  const int64_t order = tokens > kOrderedRows ? 2 * mask_blocks(tokens, 128) + mask_blocks(tokens, 64) : 0;
+  return static_cast<size_t>(tokens + 2 * mask_tiles(tokens)) * sizeof(int4) + static_cast<size_t>(order) * sizeof(int);
+}
 
 inline MaskTable mask_table(const void* table, int64_t tokens) {
   const int4* rows = static_cast<const int4*>(table);
-  return {rows, rows + tokens, rows + tokens + mask_tiles(tokens)};
+  const int4* keys = rows + tokens;
+  const int4* queries = keys + mask_tiles(tokens);
+  if (tokens <= kOrderedRows) return {rows, keys, queries, nullptr, nullptr, nullptr};
+  const int* order = reinterpret_cast<const int*>(queries + mask_tiles(tokens));
+  const int64_t n = mask_blocks(tokens, 128);
+  return {rows, keys, queries, order, order + n, order + 2 * n};
 }
 
 namespace {
 
-// Ranges' bounds over tiles [t, t + n), those before `tiles` (nothing: x > y).
-__device__ __forceinline__ int4 mask_bounds(const int4* b, int t, int n, int tiles) {
+// Ranges' bounds over tiles [t, t + N), those before `tiles` (nothing: x > y); t is uniform,
+// and so is the result, in scalar registers: what it decides are branches, not selects.
+template <int N>
+__device__ __forceinline__ int4 mask_bounds(const int4* b, int t, int tiles) {
   int4 r = make_int4(0x7fffffff, 0, 0, 0x7fffffff);
-  for (int i = t; i < min(t + n, tiles); ++i) {
-    const int4 v = b[i];
-    r = make_int4(min(r.x, v.x), max(r.y, v.y), max(r.z, v.z), min(r.w, v.w));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int4 v = b[min(t + i, tiles - 1)];  // a tile twice changes nothing
+    if (t < tiles) r = make_int4(min(r.x, v.x), max(r.y, v.y), max(r.z, v.z), min(r.w, v.w));
   }
-  return r;
+  return make_int4(__builtin_amdgcn_readfirstlane(r.x), __builtin_amdgcn_readfirstlane(r.y),
+                   __builtin_amdgcn_readfirstlane(r.z), __builtin_amdgcn_readfirstlane(r.w));
+}
+
+// Which block and head (y) a workgroup takes.  Ranks run by falling work, the heaviest first
+// on every XCD (workgroup L runs on XCD L % 8): with a multiple of eight heads each XCD has
+// heads of its own, whose tensors stay in its L2; else ranks and heads are dealt out in turn.
+// 16384 tokens in rows of 2048, 32/4 heads of 64, backward: XCDs by position in the row (block
+// x on XCD x % 8) 956 us, dealt out by falling work 567.
+__device__ __forceinline__ XcdOrder masked_order() {
+  if (gridDim.y % 8 == 0) return xcd_order();
+  const int L = blockIdx.x + gridDim.x * blockIdx.y, ny = gridDim.y;
+  return {L / ny, L % ny};
 }
 
 // --------------------------------------------------------------------- scores
@@ -131,11 +163,11 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&acc)[ND]) {
 }
 
 // acc += X^T f over rows row0 .. row0+15 of the tile X, of which this lane's column sees
-// those n with first + n < count (unsigned): one row at a time, the others zero, and the
-// columns that do not see it keep their sums.
+// rows lo <= row < hi: one row at a time, the others zero, and the columns that do not see
+// it keep their sums.
 template <int HD>
 __device__ __forceinline__ void wsum_careful(f32x16 (&acc)[HD / 32], bf16x8 f, const char* tile, int b0, int b8,
-                                             int row0, unsigned first, unsigned count, int hl) {
+                                             int row0, int lo, int hi, int hl) {
 #pragma unroll 1
   for (int n = 0; n < 16; ++n) {
     // Row n is element e of the lanes of one half (the permuted order of lds_frag_tr).
@@ -144,14 +176,32 @@ __device__ __forceinline__ void wsum_careful(f32x16 (&acc)[HD / 32], bf16x8 f, c
     const uint32_t m = (e & 1) ? 0xffff0000u : 0x0000ffffu;
     const uint32_t m0 = mine && (e >> 1) == 0 ? m : 0, m1 = mine && (e >> 1) == 1 ? m : 0;
     const uint32_t m2 = mine && (e >> 1) == 2 ? m : 0, m3 = mine && (e >> 1) == 3 ? m : 0;
-    const bool seen = first + n < count;
+    const bool seen = row0 + n >= lo && row0 + n < hi;
 #pragma unroll
     for (int dt = 0; dt < HD / 32; ++dt) {
       const uint4 u = __builtin_bit_cast(uint4, lds_frag_tr<HD>(tile, b0, b8, row0, dt));
       const f32x16 t = mfma(as_bf16x8(make_uint4(u.x & m0, u.y & m1, u.z & m2, u.w & m3)), f, acc[dt]);
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[dt][j] = seen ? t[j] : acc[dt][j];
+      __builtin_amdgcn_sched_barrier(0);  // one block's 16 registers at a time
     }
+  }
+}
+
+// x = `none` outside lo <= c < hi, c = the accumulator entry's row (less 4 hl) plus `first`.
+// Steps seen in part are few, so each side is a branch of its own, kept one by the empty
+// asm (as selects that every step pays for: 32 comparisons and selects of a forward step's
+// 270 vector instructions).
+__device__ __forceinline__ void mask_range(f32x16& x, bool ends, bool starts, int lo, int hi, int first, float none) {
+  if (ends) {
+    asm volatile("");
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = first + acc_row(j, 0) < hi ? x[j] : none;
+  }
+  if (starts) {
+    asm volatile("");
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = first + acc_row(j, 0) >= lo ? x[j] : none;
   }
 }
 

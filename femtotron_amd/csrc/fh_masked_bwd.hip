@@ -19,7 +19,7 @@ template <int HD, int MODE, bool CAREFUL>
 __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, const bf16x8 (&qf)[HD / 16],
                                                const bf16x8 (&gf)[HD / 16], f32x16 (&dqacc)[HD / 32], float nlse2,
                                                float dl, int a_off, int b0, int b8, const Score<MODE>& score,
-                                               float base, bool whole, int lo, unsigned count, int hl) {
+                                               float base, bool ends, bool starts, int lo, int hi, int hl) {
   constexpr int BN = 64, NS = HD / 16;
 #pragma unroll
   for (int t = 0; t < BN / 32; ++t) {
@@ -36,17 +36,14 @@ __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, con
       const float dz = p * (y[j] - dl);
       x[j] = (MODE & kCap) ? dz * ds : dz;
     }
-    if (!whole) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = static_cast<unsigned>(32 * t + acc_row(j, 0) - lo) < count ? x[j] : 0.f;
-    }
+    mask_range(x, ends, starts, lo, hi, 32 * t, 0.f);
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
       const bf16x8 df = pack_frag(x, 8 * s2);
       const int row0 = 32 * t + 16 * s2;
       if constexpr (CAREFUL) {
-        if (!whole) {
-          wsum_careful<HD>(dqacc, df, K, b0, b8, row0, static_cast<unsigned>(row0 - (lo + 4 * hl)), count, hl);
+        if (ends || starts) {
+          wsum_careful<HD>(dqacc, df, K, b0, b8, row0, lo + 4 * hl, hi + 4 * hl, hl);
           continue;
         }
       }
@@ -67,13 +64,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
   __shared__ __align__(16) char sk0[TILE], sk1[TILE], sv0[TILE], sv1[TILE];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const XcdOrder ord = xcd_order();
+  const XcdOrder ord = masked_order();
   const int h = ord.y, kvh = h / group;
-  const int q0 = (gridDim.x - 1 - ord.rank) * BM;
+  const int q0 = (mask.order_q != nullptr ? mask.order_q[ord.rank] : static_cast<int>(gridDim.x) - 1 - ord.rank) * BM;
   const int qw = q0 + wave * 32, qi = qw + l32;
   const int tiles = (T + kMaskRows - 1) / kMaskRows;
-  const int4 all = mask_bounds(mask.keys, q0 / kMaskRows, BM / kMaskRows, tiles);
-  const int4 mine = mask_bounds(mask.keys, qw / kMaskRows, 1, tiles);
+  const int4 all = mask_bounds<BM / kMaskRows>(mask.keys, q0 / kMaskRows, tiles);
+  const int4 mine = mask_bounds<1>(mask.keys, qw / kMaskRows, tiles);
   const int2 sees = qi < T ? *reinterpret_cast<const int2*>(mask.rows + qi) : make_int2(0, 0);
   const int kbeg = all.x, n_steps = all.y > all.x ? (all.y - all.x + BN - 1) / BN : 0;
   const Score<MODE> score(args, h);
@@ -136,7 +133,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
             if (mine.x >= k0 + BN || mine.y <= k0) return;
             masked_dq_step<HD, MODE, decltype(careful)::value>(
                 K, V, qf, gf, dqacc, nlse2, dl, a_off, b0, b8, score, static_cast<float>(qi - k0 - 4 * hl),
-                mine.z <= k0 && mine.w >= k0 + BN, sees.x - k0 - 4 * hl, static_cast<unsigned>(sees.y - sees.x), hl);
+                mine.w < k0 + BN, mine.z > k0, sees.x - k0 - 4 * hl, sees.y - k0 - 4 * hl, hl);
           },
           [] {});
     };
@@ -192,13 +189,14 @@ struct MaskedItems {
 
 // A wave's share of an item up to head_dim 64: the 32 queries at row hrow of the tiles Q
 // and dO against the wave's 32 keys.  base = the item's first query + 4 hl - the lane's
-// key; the lane's key is seen by the queries c (of the 32, less 4 hl) with c - lo < count.
+// key; the lane's key is seen by the queries lo <= c < hi of the 32 (less 4 hl); ends and
+// starts as in masked_step, of keys.
 template <int HD, int MODE, bool CAREFUL>
 __device__ __forceinline__ void masked_dkdv_item(const char* Q, const char* G, const float* sl, const float* sd,
                                                  const bf16x8 (&kf)[HD / 16], const bf16x8 (&vf)[HD / 16],
                                                  f32x16 (&dkacc)[HD / 32], f32x16 (&dvacc)[HD / 32], int a_off, int b0,
-                                                 int b8, int hrow, const Score<MODE>& score, float base, bool whole,
-                                                 int lo, unsigned count, int hl) {
+                                                 int b8, int hrow, const Score<MODE>& score, float base, bool ends,
+                                                 bool starts, int lo, int hi, int hl) {
   constexpr int NS = HD / 16;
   f32x16 x = zero16(), y = zero16();  // S, dP (rows = queries, column = key)
   __builtin_amdgcn_iglp_opt(0);
@@ -223,23 +221,16 @@ __device__ __forceinline__ void masked_dkdv_item(const char* Q, const char* G, c
       y[j] = (MODE & kCap) ? dz * ds : dz;
     }
   }
-  if (!whole) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const bool seen = static_cast<unsigned>(acc_row(j, 0) - lo) < count;
-      x[j] = seen ? x[j] : 0.f;
-      y[j] = seen ? y[j] : 0.f;
-    }
-  }
+  mask_range(x, ends, starts, lo, hi, 0, 0.f);
+  mask_range(y, ends, starts, lo, hi, 0, 0.f);
 #pragma unroll
   for (int s2 = 0; s2 < 2; ++s2) {
     const bf16x8 pf = pack_frag(x, 8 * s2);
     const bf16x8 df = pack_frag(y, 8 * s2);
     if constexpr (CAREFUL) {
-      if (!whole) {
-        const unsigned first = static_cast<unsigned>(16 * s2 - (lo + 4 * hl));
-        wsum_careful<HD>(dvacc, pf, G, b0, b8, 16 * s2, first, count, hl);
-        wsum_careful<HD>(dkacc, df, Q, b0, b8, 16 * s2, first, count, hl);
+      if (ends || starts) {
+        wsum_careful<HD>(dvacc, pf, G, b0, b8, 16 * s2, lo + 4 * hl, hi + 4 * hl, hl);
+        wsum_careful<HD>(dkacc, df, Q, b0, b8, 16 * s2, lo + 4 * hl, hi + 4 * hl, hl);
         continue;
       }
     }
@@ -275,14 +266,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
   const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = wave / NWH, wq = wave % NWH;
-  const XcdOrder ord = xcd_order();
+  const XcdOrder ord = masked_order();
   const int kvh = ord.y / hs.n, split = ord.y - kvh * hs.n;
   const int gs = group / hs.n;  // query heads of this workgroup
   const int h0 = kvh * group + split * gs;
-  const int k0 = ord.rank * kFusedKeys, kw = k0 + wq * 32, ki = kw + l32;
+  const int k0 = (mask.order_k128 != nullptr ? mask.order_k128[ord.rank] : ord.rank) * kFusedKeys, kw = k0 + wq * 32, ki = kw + l32;
   const int tiles = (T + kMaskRows - 1) / kMaskRows;
-  const int4 all = mask_bounds(mask.queries, k0 / kMaskRows, kFusedKeys / kMaskRows, tiles);
-  const int4 mine = mask_bounds(mask.queries, kw / kMaskRows, 1, tiles);
+  const int4 all = mask_bounds<kFusedKeys / kMaskRows>(mask.queries, k0 / kMaskRows, tiles);
+  const int4 mine = mask_bounds<1>(mask.queries, kw / kMaskRows, tiles);
   const int2 seen_by = ki < T ? *(reinterpret_cast<const int2*>(mask.rows + ki) + 1) : make_int2(0, 0);
   const int qbeg = all.x, n_tiles = all.y > all.x ? (all.y - all.x + BQ - 1) / BQ : 0;
   const int hrow = 32 * half;  // this wave's first query row within an item
@@ -333,8 +324,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
         if (it < n_it && mine.x < qh + 32 && mine.y > qh) {
           const Score<MODE> score(args, h0 + hh);
           masked_dkdv_item<HD, MODE, CAREFUL>(Q, G, L, D, kf, vf, dkacc, dvacc, a_off, b0, b8, hrow, score,
-                                              static_cast<float>(qh + 4 * hl - ki), mine.z <= qh && mine.w >= qh + 32,
-                                              seen_by.x - qh - 4 * hl, static_cast<unsigned>(seen_by.y - seen_by.x), hl);
+                                              static_cast<float>(qh + 4 * hl - ki), mine.w < qh + 32, mine.z > qh,
+                                              seen_by.x - qh - 4 * hl, seen_by.y - qh - 4 * hl, hl);
         }
         if (++hh == gs) {
           hh = 0;
@@ -393,7 +384,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
 constexpr int kSplitKeys = 64;
 
 template <int HD, int MODE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_masked_dkdv(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k_masked_dkdv(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
     const uint16_t* __restrict__ v, int64_t ldv, const uint16_t* __restrict__ dO, int64_t lddo,
     const float* __restrict__ nl2, const float* __restrict__ delta, uint16_t* __restrict__ dk, int64_t lddk,
@@ -409,13 +400,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool role_a = wave < NKS;
   const int sub = role_a ? wave : wave - NKS;
-  const XcdOrder ord = xcd_order();
+  const XcdOrder ord = masked_order();
   const int kvh = ord.y / hs.n, split = ord.y - kvh * hs.n;
   const int gs = group / hs.n, h0 = kvh * group + split * gs;
-  const int k0 = ord.rank * kSplitKeys, kw = k0 + sub * 32, ki = kw + l32;
+  const int k0 = (mask.order_k64 != nullptr ? mask.order_k64[ord.rank] : ord.rank) * kSplitKeys, kw = k0 + sub * 32, ki = kw + l32;
   const int tiles = (T + kMaskRows - 1) / kMaskRows;
-  const int4 all = mask_bounds(mask.queries, k0 / kMaskRows, kSplitKeys / kMaskRows, tiles);
-  const int4 mine = mask_bounds(mask.queries, kw / kMaskRows, 1, tiles);
+  const int4 all = mask_bounds<kSplitKeys / kMaskRows>(mask.queries, k0 / kMaskRows, tiles);
+  const int4 mine = mask_bounds<1>(mask.queries, kw / kMaskRows, tiles);
   const int2 seen_by = ki < T ? *(reinterpret_cast<const int2*>(mask.rows + ki) + 1) : make_int2(0, 0);
   const int qbeg = all.x, n_tiles = all.y > all.x ? (all.y - all.x + BQ - 1) / BQ : 0;
   int a_off = lane_off_a<HD>(lane);
@@ -452,9 +443,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         if (it + 1 < n_it) items.load(qg, ldq, gg, lddo, lg, dg, T, last, gs, XN, XN + TILE, LN, DN, wave, lane);
         const int qs = qbeg + qt * BQ;
         const bool active = it < n_it && mine.x < qs + BQ && mine.y > qs;  // the same for both roles
-        const bool whole = mine.z <= qs && mine.w >= qs + BQ;
-        const int lo = seen_by.x - qs - 4 * hl;
-        const unsigned count = static_cast<unsigned>(seen_by.y - seen_by.x);
+        const bool ends = mine.w < qs + BQ, starts = mine.z > qs;
+        const int lo = seen_by.x - qs - 4 * hl, hi = seen_by.y - qs - 4 * hl;
         f32x16 x;  // S then P (role A) / dP then dS (role B), rows = queries, column = key
         if (active) {
           const char* X = X0 + xoff;
@@ -476,10 +466,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
                 if constexpr (MODE & kCap) ds[4 * g + e] = d;
               }
             }
-            if (!whole) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) x[j] = static_cast<unsigned>(acc_row(j, 0) - lo) < count ? x[j] : 0.f;
-            }
+            mask_range(x, ends, starts, lo, hi, 0, 0.f);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               *reinterpret_cast<float4*>(&sp[sub][(g * 64 + lane) * 4]) =
@@ -510,18 +497,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
                 x[4 * g + e] = (MODE & kCap) ? dz * Sv[e] : dz;
               }
             }
-            if (!whole) {  // P is 0 there, but what it is multiplied by need not be finite
-#pragma unroll
-              for (int j = 0; j < 16; ++j) x[j] = static_cast<unsigned>(acc_row(j, 0) - lo) < count ? x[j] : 0.f;
-            }
+            // P is 0 there, but what it is multiplied by need not be finite
+            mask_range(x, ends, starts, lo, hi, 0, 0.f);
           }
           const char* Y = X0 + (TILE - xoff);
 #pragma unroll
           for (int s2 = 0; s2 < 2; ++s2) {
             const bf16x8 f = pack_frag(x, 8 * s2);
             if constexpr (CAREFUL) {
-              if (!whole) {
-                wsum_careful<HD>(acc, f, Y, b0, b8, 16 * s2, static_cast<unsigned>(16 * s2 - (lo + 4 * hl)), count, hl);
+              if (ends || starts) {
+                wsum_careful<HD>(acc, f, Y, b0, b8, 16 * s2, lo + 4 * hl, hi + 4 * hl, hl);
                 continue;
               }
             }

@@ -17,13 +17,14 @@ namespace {
 constexpr float kNoMax = -3.0e38f;
 
 // One step of a wave: raw scores of 64 keys from K, the update of (m, l, oacc), and
-// oacc += V^T P^T.  base = the query's row - k0 - 4 hl; its keys are those at c (of the
-// step, less 4 hl) with c - lo < count.
+// oacc += V^T P^T.  base = the query's row - k0 - 4 hl; it sees keys lo <= c < hi of the
+// step (less 4 hl).  ends, starts: some query sees no key from within the step on, before
+// a key within it.
 template <int HD, int MODE, bool CAREFUL>
 __device__ __forceinline__ void masked_step(const char* K, const char* V, const bf16x8 (&qf)[HD / 16],
                                             f32x16 (&oacc)[HD / 32], float& m, float& l, int a_off, int b0, int b8,
-                                            const Score<MODE>& score, float base, bool whole, int lo, unsigned count,
-                                            int hl) {
+                                            const Score<MODE>& score, float base, bool ends, bool starts, int lo,
+                                            int hi, int hl) {
   constexpr int BN = 64, NS = HD / 16, ND = HD / 32;
   f32x16 x[BN / 32];
   __builtin_amdgcn_iglp_opt(0);  // LDS reads interleaved with MFMAs
@@ -39,21 +40,13 @@ __device__ __forceinline__ void masked_step(const char* K, const char* V, const 
 #pragma unroll
       for (int j = 0; j < 16; ++j) x[t][j] = score(x[t][j], base - (32 * t + acc_row(j, 0)));
   }
+  mask_range(x[0], ends, starts, lo, hi, 0, -INFINITY);
+  mask_range(x[1], ends, starts, lo, hi, 32, -INFINITY);
   float mloc = -INFINITY;
-  if (!whole) {
 #pragma unroll
-    for (int t = 0; t < BN / 32; ++t)
+  for (int t = 0; t < BN / 32; ++t)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        x[t][j] = static_cast<unsigned>(32 * t + acc_row(j, 0) - lo) < count ? x[t][j] : -INFINITY;
-        mloc = fmaxf(mloc, x[t][j]);
-      }
-  } else {
-#pragma unroll
-    for (int t = 0; t < BN / 32; ++t)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) mloc = fmaxf(mloc, x[t][j]);
-  }
+    for (int j = 0; j < 16; ++j) mloc = fmaxf(mloc, x[t][j]);
   mloc = xor32_max(mloc);
   if constexpr (MODE == 0) mloc *= score.a;
   if (wave_any(mloc > m + kRescaleSlack)) {
@@ -79,8 +72,8 @@ __device__ __forceinline__ void masked_step(const char* K, const char* V, const 
     const bf16x8 pf = pack_frag(x[s >> 1], 8 * (s & 1));
     lsum = sum_bf16x8(pf, lsum);
     if constexpr (CAREFUL) {
-      if (!whole) {  // lo counts from the step's first key less 4 hl
-        wsum_careful<HD>(oacc, pf, V, b0, b8, 16 * s, static_cast<unsigned>(16 * s - (lo + 4 * hl)), count, hl);
+      if (ends || starts) {
+        wsum_careful<HD>(oacc, pf, V, b0, b8, 16 * s, lo + 4 * hl, hi + 4 * hl, hl);
         continue;
       }
     }
@@ -89,10 +82,13 @@ __device__ __forceinline__ void masked_step(const char* K, const char* V, const 
   l += lsum;
 }
 
+// Four waves a SIMD up to head_dim 64: what the registers (128) then lack is spilled in the
+// careful pass alone.  16384 tokens, 32/4 heads of 64, documents of about 600: 124 us with
+// three waves a SIMD (one workgroup a CU), 104 with four.
 // HPB = 2: 8 waves take the same rows of two query heads of one kv head, which read the
 // same K and V tiles.
 template <int HD, int HPB, int MODE>
-__global__ __launch_bounds__(256 * HPB) __attribute__((amdgpu_waves_per_eu(2))) void k_masked_fwd(
+__global__ __launch_bounds__(256 * HPB) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : HPB == 2 ? 4 : 3))) void k_masked_fwd(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
     const uint16_t* __restrict__ v, int64_t ldv, uint16_t* __restrict__ o, int64_t ldo, float* __restrict__ lse,
     int8_t* __restrict__ o_low, int T, int group, ScoreArgs args, MaskTable mask) {
@@ -103,13 +99,14 @@ __global__ __launch_bounds__(256 * HPB) __attribute__((amdgpu_waves_per_eu(2))) 
   __shared__ __align__(16) char sk0[TILE], sk1[TILE], sk2[TILE3], sv0[TILE], sv1[TILE], sv2[TILE3];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const XcdOrder ord = xcd_order();
+  const XcdOrder ord = masked_order();
   const int h = ord.y * HPB + (wave >> 2), kvh = h / group;
-  const int q0 = (gridDim.x - 1 - ord.rank) * BM;  // the latest queries, which see most, first
+  // The blocks that see most first, or else the latest.
+  const int q0 = (mask.order_q != nullptr ? mask.order_q[ord.rank] : static_cast<int>(gridDim.x) - 1 - ord.rank) * BM;
   const int qw = q0 + (wave & 3) * 32, qi = qw + l32;
   const int tiles = (T + kMaskRows - 1) / kMaskRows;
-  const int4 all = mask_bounds(mask.keys, q0 / kMaskRows, BM / kMaskRows, tiles);
-  const int4 mine = mask_bounds(mask.keys, qw / kMaskRows, 1, tiles);
+  const int4 all = mask_bounds<BM / kMaskRows>(mask.keys, q0 / kMaskRows, tiles);
+  const int4 mine = mask_bounds<1>(mask.keys, qw / kMaskRows, tiles);
   const int2 sees = qi < T ? *reinterpret_cast<const int2*>(mask.rows + qi) : make_int2(0, 0);
   const int kbeg = all.x, n_steps = all.y > all.x ? (all.y - all.x + BN - 1) / BN : 0;
   const Score<MODE> score(args, h);
@@ -139,8 +136,8 @@ __global__ __launch_bounds__(256 * HPB) __attribute__((amdgpu_waves_per_eu(2))) 
         if (mine.x >= k0 + BN || mine.y <= k0) return;  // nothing for this wave's queries
         masked_step<HD, MODE, decltype(careful)::value>(K, V, qf, oacc, m, l, a_off, b0, b8, score,
                                                         static_cast<float>(qi - k0 - 4 * hl),
-                                                        mine.z <= k0 && mine.w >= k0 + BN, sees.x - k0 - 4 * hl,
-                                                        static_cast<unsigned>(sees.y - sees.x), hl);
+                                                        mine.w < k0 + BN, mine.z > k0, sees.x - k0 - 4 * hl,
+                                                        sees.y - k0 - 4 * hl, hl);
       };
       if constexpr (STAGES == 3)
         kv_block_loop3<BN, HD, 4 * HPB>(kp, ldk, vp, ldv, n_steps, T - kbeg, sk0, sk1, sk2, sv0, sv1, sv2, wave, lane,
@@ -159,17 +156,30 @@ __global__ __launch_bounds__(256 * HPB) __attribute__((amdgpu_waves_per_eu(2))) 
       for (int dt = 0; dt < ND; ++dt) oacc[dt] = zero16();
     }
     const float mul = some ? 1.f / lt : 0.f;
-    uint16_t* row = o + static_cast<int64_t>(qi) * ldo + static_cast<int64_t>(h) * HD + 4 * hl;
-    int8_t* low = o_low + static_cast<int64_t>(qi) * (gridDim.y * HPB * HD) + static_cast<int64_t>(h) * HD + 4 * hl;
+    uint16_t* row = o + static_cast<int64_t>(qi) * ldo + static_cast<int64_t>(h) * HD + 8 * hl;
+    int8_t* low = o_low + static_cast<int64_t>(qi) * (gridDim.y * HPB * HD) + static_cast<int64_t>(h) * HD + 8 * hl;
+    // Lane half hl holds dims 8 g + 4 hl .. +3; the halves exchange so that each stores the 8
+    // dims of the groups g with g % 2 == hl.
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float x[4] = {oacc[dt][4 * g] * mul, oacc[dt][4 * g + 1] * mul, oacc[dt][4 * g + 2] * mul,
-                            oacc[dt][4 * g + 3] * mul};
-        const uint2 w = make_uint2(pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]));
-        *reinterpret_cast<uint2*>(row + dt * 32 + 8 * g) = w;
-        if (o_low != nullptr) *reinterpret_cast<uint32_t*>(low + dt * 32 + 8 * g) = low_bits(x, w);
+      for (int g = 0; g < 4; g += 2) {
+        uint2 w[2];
+        uint32_t b[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = 4 * (g + i);
+          const float x[4] = {oacc[dt][j] * mul, oacc[dt][j + 1] * mul, oacc[dt][j + 2] * mul, oacc[dt][j + 3] * mul};
+          w[i] = make_uint2(pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]));
+          b[i] = low_bits(x, w[i]);
+        }
+        const auto x = __builtin_amdgcn_permlane32_swap(w[0].x, w[1].x, false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(w[0].y, w[1].y, false, false);
+        *reinterpret_cast<uint4*>(row + dt * 32 + 8 * g) = make_uint4(x[0], y[0], x[1], y[1]);
+        if (o_low != nullptr) {
+          const auto z = __builtin_amdgcn_permlane32_swap(b[0], b[1], false, false);
+          *reinterpret_cast<uint2*>(low + dt * 32 + 8 * g) = make_uint2(z[0], z[1]);
+        }
       }
     if (lse != nullptr && hl == 0) lse[static_cast<int64_t>(h) * T + qi] = some ? (m + log2f(lt)) * kLn2 : 0.f;
   }

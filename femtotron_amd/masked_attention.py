@@ -11,6 +11,8 @@ over the j that token i sees, which ``attention_mask`` says.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -52,14 +54,14 @@ def attention_mask(batch: int, seq_len: int, starts: torch.Tensor | None = None,
         raise ValueError(f"attention_mask: window must be at least 1, got {window}")
     if prefix is not None and (window is not None or not causal):
         raise ValueError("attention_mask: a prefix goes with causal and without a window")
-    for t in (starts, lengths, prefix):
-        if t is not None:
-            if device is not None and torch.device(device) != t.device and torch.device(device).index is not None:
-                raise ValueError(f"attention_mask: a tensor on {t.device}, the mask on {device}")
-            device = t.device
+    given = next((t for t in (starts, lengths, prefix) if t is not None), None)
     if device is None:
-        device = torch.device("cuda")
-    device = torch.device(device)
+        device = torch.device("cuda") if given is None else given.device
+    else:
+        device = torch.device(device)
+        if given is not None and device.index is not None and device != given.device:
+            raise ValueError(f"attention_mask: a tensor on {given.device}, the mask on {device}")
+        device = device if given is None else given.device
     if device.type != "cuda":
         raise ValueError("femtohip ops take HIP device tensors only")
     starts, lengths, prefix = (None if t is None else t.contiguous() for t in (starts, lengths, prefix))
@@ -67,45 +69,50 @@ def attention_mask(batch: int, seq_len: int, starts: torch.Tensor | None = None,
     return AttentionMask(table, batch, seq_len)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t as token rows that the kernels read in place, laid out first where it is none."""
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    ld, unit = t.stride()
-    if (unit == 1 or t.shape[1] == 1) and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (ld >= t.shape[1] and ld % 8 == 0)):
-        return t
-    return ops.aligned(t)
+def _laid_out(t: torch.Tensor, seq_len: int) -> tuple[torch.Tensor, int]:
+    """t as token rows that the kernels read (itself, or a copy), and their row stride."""
+    ld = ops.token_rows(t, seq_len)
+    if ld:
+        return t, ld
+    return ops.aligned(t), t.size(-1)
 
 
 class MaskedAttentionFunction(torch.autograd.Function):
     """Saved: q, k, v, o (bf16: and 8 more bits of it) and an fp32 value a token and head."""
 
     @staticmethod
-    def forward(ctx, q, k, v, table, slopes, how):
-        rows = _rows(q), _rows(k), _rows(v)
-        o, lse, low = ops.masked_attn_fwd(*rows, table, slopes=slopes, **how)
-        ctx.save_for_backward(*rows, o, lse, low, table, slopes)
-        ctx.how, ctx.shapes = how, (q.shape, k.shape, v.shape)
-        return o.view(q.shape)
+    def forward(ctx, q, k, v, table, slopes, args, seq_len):
+        o, lse, low = ops.masked_attn_fwd_checked(args, q, k, v, table, slopes, True)
+        ctx.save_for_backward(q, k, v, o, lse, low, table, slopes)
+        ctx.args, ctx.seq_len = args, seq_len
+        return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, low, table, slopes = ctx.saved_tensors
-        grads = ops.masked_attn_bwd(q, k, v, o, _rows(do), lse, low, table, slopes=slopes, **ctx.how)
-        return (*(g.view(s) for g, s in zip(grads, ctx.shapes)), None, None, None)
+        # autograd hands the gradient in of the output's shape, dtype and device
+        do, lddo = _laid_out(do, ctx.seq_len)
+        return (*ops.masked_attn_bwd_checked(ctx.args, q, k, v, o, do, lddo, lse, low, table, slopes), None, None, None, None)
 
 
-def _score(name: str, head_dim: int, scale: float | None, cap: float | None, slopes: torch.Tensor | None) -> dict:
+def _score(name: str, head_dim: int, scale: float | None, cap: float | None,
+           slopes: torch.Tensor | None) -> tuple[float, float]:
+    """(scale, cap) as the kernels take them, 0 for no cap."""
     for v, n in ((scale, "scale"), (cap, "cap"), (slopes, "slopes")):
-        if ops.wants_derivative(v):
+        if v is not None and ops.wants_derivative(v):
             raise TypeError(f"{name}: {n} is a constant and gets no gradient")
+    if head_dim not in (32, 64, 128):
+        raise ValueError(f"{name}: head_dim must be 32, 64 or 128, got {head_dim}")
     scale = head_dim ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < float("inf"):
+    if not 0 < scale < math.inf:
         raise ValueError(f"{name}: scale must be positive, got {scale}")
-    if cap is not None and not 0 < cap < float("inf"):
+    if cap is None:
+        return scale, 0.0
+    cap = float(cap)
+    if not 0 < cap < math.inf:
         raise ValueError(f"{name}: cap must be positive, or None, got {cap}")
-    return dict(head_dim=head_dim, scale=scale, cap=float(cap or 0.0))
+    return scale, cap
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: AttentionMask, *, head_dim: int,
@@ -120,16 +127,20 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     become cap * tanh(score / cap); ``slopes`` (fp32, one a query head): less slopes[h] times
     the distance, after the cap.  bf16 or fp32 on a HIP device.  Nothing that a token does not
     see reaches it, infinities and NaN included."""
-    how = _score("masked_attention", head_dim, scale, cap, slopes)
-    tokens = mask.batch * mask.seq_len
+    scale, cap = _score("masked_attention", head_dim, scale, cap, slopes)
+    seq_len = mask.seq_len
+    tokens = mask.batch * seq_len
     for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() not in (2, 3) or t.numel() != tokens * t.shape[-1] or (t.dim() == 3 and t.shape[1] != mask.seq_len):
-            raise ValueError(f"masked_attention: {n} must be [{mask.batch}, {mask.seq_len}, heads * head_dim] or "
-                             f"[{tokens}, heads * head_dim] under this mask, got {tuple(t.shape)}")
+        shape = t.shape
+        if not (len(shape) == 3 and shape[0] == mask.batch and shape[1] == seq_len or len(shape) == 2 and shape[0] == tokens):
+            raise ValueError(f"masked_attention: {n} must be [{mask.batch}, {seq_len}, heads * head_dim] or "
+                             f"[{tokens}, heads * head_dim] under this mask, got {tuple(shape)}")
+    dt, nh, nkv = ops.masked_attn_check("masked_attention", q, k, v, mask.table, slopes, tokens, head_dim)
+    (q, ldq), (k, ldk), (v, ldv) = _laid_out(q, seq_len), _laid_out(k, seq_len), _laid_out(v, seq_len)
+    args = (dt, ldq, ldk, ldv, tokens, nh, nkv, head_dim, scale, cap)
     if ops.differentiated(q, k, v):
-        return MaskedAttentionFunction.apply(q, k, v, mask.table, slopes, how)
-    o, _, _ = ops.masked_attn_fwd(_rows(q), _rows(k), _rows(v), mask.table, slopes=slopes, need_grad=False, **how)
-    return o.view(q.shape)
+        return MaskedAttentionFunction.apply(q, k, v, mask.table, slopes, args, seq_len)
+    return ops.masked_attn_fwd_checked(args, q, k, v, mask.table, slopes, False)[0]
 
 
 def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, *, head_dim: int,
@@ -148,19 +159,11 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     for t, n in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
         if ops.wants_derivative(t):
             raise TypeError(f"cache_attention has no derivatives, and {n} wants one (use it under torch.no_grad())")
-    how = _score("cache_attention", head_dim, scale, cap, slopes)
+    scale, cap = _score("cache_attention", head_dim, scale, cap, slopes)
     if window is not None and window < 1:
         raise ValueError(f"cache_attention: window must be at least 1, got {window}")
     if q.dim() != 3:
         raise ValueError(f"cache_attention: q must be [batch, new, heads * head_dim], got {tuple(q.shape)}")
-    caches = []
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dim() == 3 and head_dim > 0 and t.shape[-1] % head_dim == 0:
-            t = t.unflatten(-1, (t.shape[-1] // head_dim, head_dim))
-        if t.dim() != 4 or t.shape[0] != q.shape[0] or t.shape[3] != head_dim:
-            raise ValueError(f"cache_attention: {n} must be [{q.shape[0]}, room, kv heads * {head_dim}] or "
-                             f"[{q.shape[0]}, room, kv heads, {head_dim}], got {tuple(t.shape)}")
-        caches.append(t)
-    del how["head_dim"]
-    o = ops.cache_attn(_rows(q), *caches, lengths.contiguous(), n_new=q.shape[1], slopes=slopes, window=window or 0, **how)
-    return o.view(q.shape)
+    q, ldq = _laid_out(q, q.shape[1])
+    return ops.cache_attn(q, ldq, k_cache, v_cache, lengths.contiguous(), head_dim=head_dim, scale=scale, cap=cap,
+                          slopes=slopes, window=window or 0)

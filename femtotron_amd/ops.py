@@ -678,7 +678,7 @@ def attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
 # ----------------------------------------------------- attention under a mask
 def _int64_vector(name: str, t: torch.Tensor, n: int | None, dev: int) -> None:
     if t.get_device() != dev or dev < 0:
-        raise ValueError(f"{name} must be on the mask's HIP device")
+        raise ValueError(f"{name} must be on the mask's HIP device (femtohip ops take HIP device tensors only)")
     if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous int64 vector, got {t.dtype} {tuple(t.shape)}")
     if n is not None and t.numel() != n:
@@ -704,32 +704,86 @@ def attn_mask(tokens: int, seq_len: int, starts: torch.Tensor | None, lengths: t
     return table
 
 
-def _masked_operands(name: str, tokens: int, head_dim: int, table: torch.Tensor, slopes: torch.Tensor | None,
-                     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> tuple[int, int]:
-    """(n_heads, n_kv_heads) of token-major q, k, v, checked."""
+def token_rows(t: torch.Tensor, seq_len: int) -> int:
+    """The row stride of [tokens, width] or [batch, seq_len, width] as token rows that the
+    attention kernels read in place (its width for one row, which has none); 0 where they
+    cannot."""
+    if t.dim() == 2:
+        ld, unit = t.stride()
+        rows = t.size(0)
+    else:
+        outer, ld, unit = t.stride()
+        rows = t.size(0)
+        if rows > 1 and seq_len > 1 and outer != seq_len * ld:
+            return 0
+        if seq_len == 1:
+            ld = outer
+        rows *= seq_len
+    width = t.size(-1)
+    if rows <= 1:
+        ld = width
+    return ld if unit == 1 and ld >= width and ld % 8 == 0 and t.data_ptr() % 16 == 0 else 0
+
+
+def masked_attn_check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
+                      slopes: torch.Tensor | None, tokens: int, head_dim: int) -> tuple[int, int, int]:
+    """(dtype code, n_heads, n_kv_heads) of token-major q, k and v of `tokens` rows, checked."""
     _alike(q, k, v)
-    if table.get_device() != q.get_device():
+    dev = q.get_device()
+    if table.get_device() != dev:
         _require_gpu(q, table)
-    for t, n in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 2 or t.size(0) != tokens or t.size(1) % head_dim:
-            raise ValueError(f"{name}: {n} must be [{tokens}, heads * {head_dim}], got {tuple(t.shape)}")
-    if k.size(1) != v.size(1):
-        raise ValueError(f"{name}: k and v have {k.size(1)} and {v.size(1)} columns")
+    wq, wk = q.size(-1), k.size(-1)
+    if head_dim <= 0 or wq % head_dim or wk % head_dim or k.shape != v.shape or q.shape[:-1] != k.shape[:-1] \
+            or q.numel() != tokens * wq:
+        raise ValueError(f"{name}: q must be [{tokens}, heads * {head_dim}], k and v [{tokens}, kv heads * {head_dim}], "
+                         f"got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
     if table.dtype != torch.uint8 or table.numel() != _lib.lib().fh_attn_mask_size(tokens):
         raise ValueError(f"{name}: the mask is not one of {tokens} tokens")
-    n_heads = q.size(1) // head_dim
+    n_heads = wq // head_dim
     if slopes is not None:
-        if slopes.get_device() != q.get_device():
+        if slopes.get_device() != dev:
             _require_gpu(q, slopes)
         if slopes.dtype != torch.float32 or slopes.numel() != n_heads or not slopes.is_contiguous():
             raise ValueError(f"{name}: slopes must be contiguous fp32 with one entry a query head, {n_heads}")
-    return n_heads, k.size(1) // head_dim
+    return _dtype_code(q), n_heads, wk // head_dim
 
 
-def _ld(t: torch.Tensor, name: str) -> int:
-    """The row stride of a 2-D view (of one row, which has none, its width)."""
-    ld = _rowmajor(t, name)
-    return ld if t.size(0) > 1 else t.size(1)
+def masked_attn_fwd_checked(args: tuple, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
+                            slopes: torch.Tensor | None, need_grad: bool):
+    """masked_attn_fwd of tensors that are known to fit; args: (dtype code, ldq, ldk, ldv, tokens,
+    n_heads, n_kv_heads, head_dim, scale, cap).  o has q's shape."""
+    dt, ldq, ldk, ldv, T, nh, nkv, hd, scale, cap = args
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = low = None
+    if need_grad:
+        lse = torch.empty((nh, T), dtype=torch.float32, device=q.device)
+        if dt == _lib.FH_BF16:
+            low = torch.empty(q.shape, dtype=torch.int8, device=q.device)
+    _launch("fh_masked_attn_fwd", q, dt, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), nh * hd,
+            _ptr(lse), _ptr(low), table.data_ptr(), T, nh, nkv, hd, scale, cap, _ptr(slopes))
+    return o, lse, low
+
+
+def masked_attn_bwd_checked(args: tuple, q, k, v, o, dout, lddo: int, lse, o_low, table, slopes):
+    """masked_attn_bwd of tensors that are known to fit (o contiguous, dout of row stride lddo);
+    args: masked_attn_fwd_checked's.  dq, dk, dv have q's, k's and v's shapes."""
+    dt, ldq, ldk, ldv, T, nh, nkv, hd, scale, cap = args
+    device, dtype = q.device, q.dtype
+    dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=device) for t in (q, k, v))
+    ws = torch.empty(max(_lib.lib().fh_masked_attn_bwd_workspace_size(dt, T, nh, nkv, hd), 4), dtype=torch.uint8, device=device)
+    _launch("fh_masked_attn_bwd", q, dt, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), nh * hd,
+            dout.data_ptr(), lddo, lse.data_ptr(), _ptr(o_low), dq.data_ptr(), nh * hd, dk.data_ptr(), nkv * hd, dv.data_ptr(),
+            nkv * hd, table.data_ptr(), ws.data_ptr(), T, nh, nkv, hd, scale, cap, _ptr(slopes))
+    return dq, dk, dv
+
+
+def _ld_of(name: str, **tensors: torch.Tensor) -> list[int]:
+    lds = [token_rows(t, 0) if t.dim() == 2 else 0 for t in tensors.values()]
+    for n, ld in zip(tensors, lds):
+        if not ld:
+            raise ValueError(f"{name}: {n} must be 2-D token rows, 16-byte aligned, its last dim contiguous and its row "
+                             "stride a multiple of 8")
+    return lds
 
 
 def masked_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, *, head_dim: int,
@@ -740,16 +794,9 @@ def masked_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: to
     masked_attn_bwd reads (None without need_grad; o_low of bf16 only).  cap 0: scores are
     not capped."""
     T = q.size(0)
-    nh, nkv = _masked_operands("masked_attn_fwd", T, head_dim, table, slopes, q, k, v)
-    dt = _dtype_code(q)
-    o = torch.empty(T, q.size(1), dtype=q.dtype, device=q.device)
-    lse = low = None
-    if need_grad:
-        lse = torch.empty(nh, T, dtype=torch.float32, device=q.device)
-        low = torch.empty(o.shape, dtype=torch.int8, device=q.device) if dt == _lib.FH_BF16 else None
-    _launch("fh_masked_attn_fwd", q, dt, _ptr(q), _ld(q, "q"), _ptr(k), _ld(k, "k"), _ptr(v), _ld(v, "v"),
-            _ptr(o), o.size(1), _ptr(lse), _ptr(low), _ptr(table), T, nh, nkv, head_dim, scale, cap, _ptr(slopes))
-    return o, lse, low
+    dt, nh, nkv = masked_attn_check("masked_attn_fwd", q, k, v, table, slopes, T, head_dim)
+    lds = _ld_of("masked_attn_fwd", q=q, k=k, v=v)
+    return masked_attn_fwd_checked((dt, *lds, T, nh, nkv, head_dim, scale, cap), q, k, v, table, slopes, need_grad)
 
 
 def masked_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, dout: torch.Tensor,
@@ -757,61 +804,71 @@ def masked_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.
                     cap: float = 0.0, slopes: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients of masked_attn_fwd for dout, with its o, lse and o_low: (dq, dk, dv)."""
     T = q.size(0)
-    nh, nkv = _masked_operands("masked_attn_bwd", T, head_dim, table, slopes, q, k, v)
+    dt, nh, nkv = masked_attn_check("masked_attn_bwd", q, k, v, table, slopes, T, head_dim)
+    ldq, ldk, ldv, lddo = _ld_of("masked_attn_bwd", q=q, k=k, v=v, dout=dout)
     _alike(q, o, dout)
-    if o.shape != q.shape or dout.shape != q.shape:
-        raise ValueError("masked_attn_bwd: o and dout must have q's shape")
+    if o.shape != q.shape or dout.shape != q.shape or not o.is_contiguous():
+        raise ValueError("masked_attn_bwd: o and dout must have q's shape, and o be contiguous")
     if lse.get_device() != q.get_device() or lse.dtype != torch.float32 or lse.numel() != nh * T or not lse.is_contiguous():
         raise ValueError("masked_attn_bwd: lse must be contiguous fp32 [heads, tokens]")
-    dt = _dtype_code(q)
     if (o_low is None) == (dt == _lib.FH_BF16):
         raise ValueError("masked_attn_bwd: o_low goes with bf16")
     if o_low is not None and (o_low.get_device() != q.get_device() or o_low.dtype != torch.int8 or o_low.shape != q.shape
                               or not o_low.is_contiguous()):
         raise ValueError("masked_attn_bwd: o_low must be contiguous int8 of q's shape")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    nbytes = _lib.lib().fh_masked_attn_bwd_workspace_size(dt, T, nh, nkv, head_dim)
-    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=q.device)
-    _launch("fh_masked_attn_bwd", q, dt, _ptr(q), _ld(q, "q"), _ptr(k), _ld(k, "k"), _ptr(v), _ld(v, "v"), _ptr(o),
-            _ld(o, "o"), _ptr(dout), _ld(dout, "dout"), _ptr(lse), _ptr(o_low), _ptr(dq), dq.size(1), _ptr(dk), dk.size(1), _ptr(dv),
-            dv.size(1), _ptr(table), _ptr(ws), T, nh, nkv, head_dim, scale, cap, _ptr(slopes))
-    return dq, dk, dv
+    return masked_attn_bwd_checked((dt, ldq, ldk, ldv, T, nh, nkv, head_dim, scale, cap), q, k, v, o, dout, lddo, lse, o_low,
+                                   table, slopes)
 
 
-def cache_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, n_new: int, scale: float,
-               cap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0) -> torch.Tensor:
-    """Attention of token-major q [batch * n_new, heads * head_dim] over caches k and v [batch,
-    room, kv heads, head_dim] (views of any strides whose last dim is contiguous), the new
-    tokens being each sequence's last of lengths (int64 [batch]) places (fh_cache_attn)."""
+def _cache_strides(name: str, t: torch.Tensor, batch: int, head_dim: int) -> tuple[int, int, int, int, int]:
+    """(room, kv heads, batch stride, row stride, head stride) of a cache [batch, room, kv heads *
+    head_dim] or [batch, room, kv heads, head_dim]; the stride of a dim of one is anything."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3 and shape[0] == batch and shape[2] % head_dim == 0:
+        _, room, width = shape
+        sb, sr, unit = stride
+        heads, sh = width // head_dim, head_dim
+    elif len(shape) == 4 and shape[0] == batch and shape[3] == head_dim:
+        _, room, heads, _ = shape
+        sb, sr, sh, unit = stride
+    else:
+        raise ValueError(f"cache_attn: {name} must be [{batch}, room, kv heads * {head_dim}] or [{batch}, room, kv heads, "
+                         f"{head_dim}], got {tuple(shape)}")
+    if unit != 1:
+        raise ValueError(f"cache_attn: {name}'s last dim must be contiguous, got strides {stride}")
+    return room, heads, sb if batch > 1 else 0, sr if room > 1 else head_dim, sh if heads > 1 else 0
+
+
+def cache_attn(q: torch.Tensor, ldq: int, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, *, head_dim: int,
+               scale: float, cap: float = 0.0, slopes: torch.Tensor | None = None, window: int = 0) -> torch.Tensor:
+    """Attention of q [batch, n_new, heads * head_dim] (token rows of stride ldq) over caches k and v
+    (_cache_strides), the new tokens being each sequence's last of lengths (int64 [batch])
+    places (fh_cache_attn)."""
     _alike(q, k, v)
-    if k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"cache_attn: k and v must be [batch, room, kv heads, head_dim], got {tuple(k.shape)}, {tuple(v.shape)}")
-    batch, room, nkv, head_dim = k.shape
-    if q.dim() != 2 or q.size(0) != batch * n_new or q.size(1) % head_dim:
-        raise ValueError(f"cache_attn: q must be [{batch} * {n_new}, heads * {head_dim}], got {tuple(q.shape)}")
-    nh = q.size(1) // head_dim
-    if lengths.get_device() != q.get_device():
+    dev = q.get_device()
+    batch, n_new, width = q.shape
+    room, nkv, kb, kr, kh = _cache_strides("k", k, batch, head_dim)
+    room2, nkv2, vb, vr, vh = _cache_strides("v", v, batch, head_dim)
+    if room2 != room or nkv2 != nkv:
+        raise ValueError(f"cache_attn: k and v are {tuple(k.shape)} and {tuple(v.shape)}")
+    if width % head_dim:
+        raise ValueError(f"cache_attn: q must be [{batch}, new, heads * {head_dim}], got {tuple(q.shape)}")
+    nh = width // head_dim
+    if lengths.get_device() != dev:
         _require_gpu(q, lengths)
     if lengths.dtype != torch.int64 or lengths.shape != (batch,) or not lengths.is_contiguous():
         raise ValueError(f"cache_attn: lengths must be contiguous int64 [{batch}], got {lengths.dtype} {tuple(lengths.shape)}")
     if slopes is not None:
-        if slopes.get_device() != q.get_device():
+        if slopes.get_device() != dev:
             _require_gpu(q, slopes)
         if slopes.dtype != torch.float32 or slopes.numel() != nh or not slopes.is_contiguous():
             raise ValueError(f"cache_attn: slopes must be contiguous fp32 with one entry a query head, {nh}")
-    strides = []
-    for t, n in ((k, "k"), (v, "v")):
-        sb, sr, sh, unit = t.stride()
-        if unit != 1:
-            raise ValueError(f"cache_attn: {n}'s last dim must be contiguous, got strides {t.stride()}")
-        # the stride of a dim of one is anything
-        strides += [sb if batch > 1 else 0, sr if room > 1 else head_dim, sh if nkv > 1 else 0]
     dt = _dtype_code(q)
     o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     nbytes = _lib.lib().fh_cache_attn_workspace_size(dt, batch, n_new, room, nh, nkv, head_dim)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _launch("fh_cache_attn", q, dt, _ptr(q), _ld(q, "q"), _ptr(k), *strides[:3], _ptr(v), *strides[3:], _ptr(o), o.size(1),
-            _ptr(lengths), batch, n_new, room, nh, nkv, head_dim, window, scale, cap, _ptr(slopes), _ptr(ws))
+    _launch("fh_cache_attn", q, dt, q.data_ptr(), ldq, k.data_ptr(), kb, kr, kh, v.data_ptr(), vb, vr, vh, o.data_ptr(), width,
+            lengths.data_ptr(), batch, n_new, room, nh, nkv, head_dim, window, scale, cap, _ptr(slopes), _ptr(ws))
     return o
 
 
@@ -888,30 +945,34 @@ def clip_grads(grads: list, outs: list | None, max_norm: float) -> torch.Tensor:
     """The 2-norm of all grads (a one-element fp32 tensor) and, with outs, each of them times
     min(1, max_norm / (norm + 1e-6)) (fh_clip_grads).  Tensors are dense, an out of its
     gradient's strides, and on one device; an out may be its gradient."""
-    table = (_lib.FhGrad * len(grads))()
     first = grads[0]
     dev = first.get_device()
-    if dev < 0:
-        raise ValueError("femtohip ops take HIP device tensors only")
-    for i, g in enumerate(grads):
-        o = None if outs is None else outs[i]
-        t = table[i]
-        for x in (g, o):
-            if x is None:
-                continue
-            if x.get_device() != dev:
-                _require_gpu(first, x)
-            if x.layout != torch.strided or not (x.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(x)):
+    in_place = outs is grads
+    all_contiguous = True
+    for ts in (grads,) if outs is None or in_place else (grads, outs):
+        if dev < 0 or any([t.get_device() != dev for t in ts]):
+            _require_gpu(first, *ts)
+        if not all([t.is_contiguous() for t in ts]):
+            all_contiguous = False
+            if not all([t.layout == torch.strided and torch.ops.aten.is_non_overlapping_and_dense(t) for t in ts]):
                 raise ValueError("clip_gradients: gradients must be dense")
-        if o is not None:
-            if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))):
-                raise ValueError(f"clip_gradients: an output must have its gradient's shape and strides, got "
-                                 f"{tuple(o.shape)} {o.stride()} for {tuple(g.shape)} {g.stride()}")
-            t.out, t.out_dtype = o.data_ptr(), _dtype_code(o)
-        t.grad, t.numel, t.grad_dtype = g.data_ptr(), g.numel(), _dtype_code(g)
+    if outs is not None and not in_place:
+        if [t.shape for t in grads] != [t.shape for t in outs] \
+                or not (all_contiguous or [t.stride() for t in grads] == [t.stride() for t in outs]):
+            raise ValueError("clip_gradients: an output must have its gradient's shape and strides")
+    n = len(grads)
+    table = (_lib.FhGrad * n)()
+    # an fh_grad as four 64-bit words: grad, out, numel, the dtypes
+    words = (ctypes.c_uint64 * (4 * n)).from_buffer(table)
+    words[0::4] = [t.data_ptr() for t in grads]
+    if outs is not None:
+        words[1::4] = words[0::4] if in_place else [t.data_ptr() for t in outs]
+    words[2::4] = [t.numel() for t in grads]
+    kinds = [_dtype_code(t) for t in grads]
+    words[3::4] = [a | b << 32 for a, b in zip(kinds, kinds if outs is None or in_place else map(_dtype_code, outs))]
     norm = torch.empty((), dtype=torch.float32, device=first.device)
-    ws = torch.empty(_lib.lib().fh_clip_grads_workspace_size(len(grads)), dtype=torch.uint8, device=first.device)
-    _launch("fh_clip_grads", first, len(grads), ctypes.addressof(table), max_norm, _ptr(norm), _ptr(ws))
+    ws = torch.empty(_lib.lib().fh_clip_grads_workspace_size(n), dtype=torch.uint8, device=first.device)
+    _launch("fh_clip_grads", first, n, ctypes.addressof(table), max_norm, norm.data_ptr(), ws.data_ptr())
     return norm
 
 

@@ -116,10 +116,10 @@ def test_entry_points_validate_on_the_host():
     refused(cache(kb=-6400), b"multiples of 8")
     refused(cache(window=-1), b"window")
     refused(cache(q=None), b"null")
-    refused(cache(room=1000, ws=None), b"workspace")
+    refused(cache(room=5000, ws=None), b"workspace")
     assert cache(batch=0) == 0 and cache(n_new=0) == 0
-    assert L.fh_cache_attn_workspace_size(0, 2, 1, 100, 2, 1, 64) == 0  # one chunk: nothing to join
-    assert L.fh_cache_attn_workspace_size(0, 2, 1, 1000, 2, 1, 64) > 0
+    assert L.fh_cache_attn_workspace_size(0, 2, 1, 100, 2, 1, 64) == 0  # a workgroup a sequence: nothing to join
+    assert L.fh_cache_attn_workspace_size(0, 2, 1, 5000, 2, 1, 64) > 0
 
     refused(L.fh_embedding_scaled_fwd(0, 16, 16, 16, 1, 10, 64, float("inf"), None), b"factor")
     refused(L.fh_embedding_scaled_bwd(0, 16, 16, 16, 1, 10, 64, -1, float("nan"), 16, None), b"factor")

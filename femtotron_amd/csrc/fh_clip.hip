@@ -6,7 +6,7 @@
 // there is no table to upload, and a captured call keeps its own copy.  A workgroup takes a
 // contiguous run of chunks of kChunkElems elements, across tensors; its sum of squares (in
 // fp64: exact products of fp32 values, no overflow below 1e154) is one partial, and every
-// workgroup of the second pass folds the at most kPartials + launches partials by itself, in
+// workgroup of the second pass folds the at most kPartials partials by itself, in
 // one order, which is cheaper than a launch in between.  The second pass takes the runs from
 // the last to the first: what the first pass read last is still in the cache.
 #include <algorithm>
@@ -22,8 +22,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kVecs = 4;                                  // of 8 elements, a thread and chunk
 constexpr int64_t kChunkElems = kThreads * 8 * kVecs;     // 8192
-constexpr int kTensors = 96;                              // a launch: 3.2 KB of arguments
-constexpr int64_t kPartials = 2048;                       // workgroups of a pass: 8 a CU
+constexpr int kTensors = 128;                             // a launch: 3.7 KB of arguments
+// Workgroups of a launch: four a CU, which all run at once.  (With eight, of which the
+// registers let six run, the last two rounds cost as much as three: 164 us a launch of 96
+// TinyLlama tensors, 1.0 GB; with a share of them by the launch's elements, a launch of
+// nine tensors left half of the chip idle.)
+constexpr int64_t kBlocks = 1024;
+constexpr int64_t kPartials = 16384;                      // in all; fewer workgroups a launch above 16 of them
 
 // Tensor i's chunks are first[i] .. first[i + 1] of the launch.
 struct Table {
@@ -34,7 +39,7 @@ struct Table {
   uint8_t kind[kTensors];  // 1: gradient bf16, 2: out bf16, 4: 16-byte aligned
   int n;
 };
-static_assert(sizeof(Table) <= 3584, "kernel arguments hold 4 KB");
+static_assert(sizeof(Table) <= 3840, "kernel arguments hold 4 KB");
 
 __device__ __forceinline__ int tensor_of(const Table& t, uint32_t chunk) {
   int lo = 0, hi = t.n;  // the last tensor whose first chunk is at or before `chunk`
@@ -115,19 +120,52 @@ __global__ __launch_bounds__(kThreads) void k_grad_squares(Table t, double* __re
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
+// N consecutive elements in one access, each of them read and written for the last time here
+// (non-temporal).
+template <typename T, int N>
+struct Pack {
+  typedef uint32_t W __attribute__((ext_vector_type(sizeof(T) * N / 4)));
+  __device__ __forceinline__ static W load(const T* p) { return __builtin_nontemporal_load(reinterpret_cast<const W*>(p)); }
+  __device__ __forceinline__ static void store(T* p, const float (&v)[N]) {
+    W w;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) w[e] = pk_bf16(v[2 * e], v[2 * e + 1]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e] = __float_as_uint(v[e]);
+    }
+    __builtin_nontemporal_store(w, reinterpret_cast<W*>(p));
+  }
+  __device__ __forceinline__ static void unpack(const W& w, float (&v)[N]) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        v[2 * e] = __uint_as_float(w[e] << 16);
+        v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = __uint_as_float(w[e]);
+    }
+  }
+};
+
 template <typename T, typename U>
 __device__ __forceinline__ void chunk_scale(const T* g, U* out, int64_t left, bool vec, float f) {
   if (vec && left >= kChunkElems) {
-    typename Elem<T>::Raw raw[kVecs];
+    // A wave's accesses are runs of whole lines on both sides: 16 bytes a lane on the wider.
+    constexpr int N = sizeof(T) == 4 || sizeof(U) == 4 ? 4 : 8, I = kChunkElems / (kThreads * N);
+    typename Pack<T, N>::W raw[I];
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) raw[i] = Elem<T>::ldraw(g + (i * kThreads + threadIdx.x) * 8);
+    for (int i = 0; i < I; ++i) raw[i] = Pack<T, N>::load(g + (i * kThreads + threadIdx.x) * N);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      float v[8];
-      Elem<T>::unpack(raw[i], v);
+    for (int i = 0; i < I; ++i) {
+      float v[N];
+      Pack<T, N>::unpack(raw[i], v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= f;
-      Elem<U>::store8(out + (i * kThreads + threadIdx.x) * 8, v);
+      for (int e = 0; e < N; ++e) v[e] *= f;
+      Pack<U, N>::store(out + (i * kThreads + threadIdx.x) * N, v);
     }
   } else {
     for (int i = 0; i < kVecs; ++i) {
@@ -240,8 +278,12 @@ int clip_grads(int64_t count, const fh_grad* grads, float max_norm, float* norm,
   FH_REQUIRE(!write || !overlaps(count, grads), "clip_grads: an output overlaps another operand");
   FH_REQUIRE(chunks < (int64_t(1) << 31), "clip_grads: too many elements");
 
-  // The launches: runs of tensors, each with its share of the workgroups.
+  // The launches: runs of kTensors tensors.
   int n_partials = 0;
+  int64_t tensors = 0;
+  for (int64_t i = 0; i < count; ++i) tensors += grads[i].numel > 0;
+  const int64_t launches = std::max<int64_t>(1, (tensors + kTensors - 1) / kTensors);
+  const int64_t most = std::max<int64_t>(1, std::min(kBlocks, kPartials / launches));
   auto each = [&](auto&& launch) {
     int64_t i = 0;
     while (i < count) {
@@ -262,8 +304,7 @@ int clip_grads(int64_t count, const fh_grad* grads, float max_norm, float* norm,
       }
       if (t.n == 0) continue;
       t.first[t.n] = at;
-      const int64_t share = (kPartials * at + chunks - 1) / chunks;
-      launch(t, static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(share, 1), at)));
+      launch(t, static_cast<unsigned>(std::min<int64_t>(most, at)));
     }
   };
   each([&](const Table& t, unsigned blocks) {
@@ -289,7 +330,7 @@ using namespace fh;
 
 extern "C" size_t fh_clip_grads_workspace_size(int64_t count) {
   if (count < 0) return 0;
-  return static_cast<size_t>(kPartials + (count + kTensors - 1) / kTensors + 2) * sizeof(double);
+  return static_cast<size_t>(std::max<int64_t>(kPartials, (count + kTensors - 1) / kTensors + 2)) * sizeof(double);
 }
 
 extern "C" int fh_clip_grads(int64_t count, const fh_grad* grads, float max_norm, float* norm, void* workspace,

@@ -52,7 +52,8 @@ __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, con
   }
 }
 
-// Also writes delta and -lse * log2(e), which the dK/dV kernels read.
+// Also writes delta and -lse * log2(e) (plus cap_log2: see Score), which the dK/dV kernels
+// read.
 template <int HD, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 3 : 2))) void k_masked_dq(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
     dl = xor32_sum(part);
     if (qi < T) {
       const int64_t at = static_cast<int64_t>(h) * T + qi;
-      nlse2 = -lse[at] * kLog2e;
+      nlse2 = fmaf(-kLog2e, lse[at], score.b);
       if (hl == 0) {
         delta[at] = dl;
         nl2[at] = nlse2;
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) dqacc[dt] = zero16();
     }
-    store_rows_T<HD>(dq + static_cast<int64_t>(qi) * lddq + static_cast<int64_t>(h) * HD, dqacc, args.scale, hl);
+    store_rows_T<HD>(dq + static_cast<int64_t>(qi) * lddq + static_cast<int64_t>(h) * HD, dqacc, grad_scale<MODE>(args), hl);
   }
 }
 
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
       store_rows_T_f32<HD>(hs.row(split, half, T, ki, nkv, kvh, HD), sum, hl);
     } else {
       uint16_t* row = half == 0 ? dk + static_cast<int64_t>(ki) * lddk : dv + static_cast<int64_t>(ki) * lddv;
-      store_rows_T<HD>(row + static_cast<int64_t>(kvh) * HD, sum, half == 0 ? args.scale : 1.f, hl);
+      store_rows_T<HD>(row + static_cast<int64_t>(kvh) * HD, sum, half == 0 ? grad_scale<MODE>(args) : 1.f, hl);
     }
   }
 }
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
       store_rows_T_f32<HD>(hs.row(split, role_a ? 1 : 0, T, ki, nkv, kvh, HD), acc, hl);
     } else {
       uint16_t* row = role_a ? dv + static_cast<int64_t>(ki) * lddv : dk + static_cast<int64_t>(ki) * lddk;
-      store_rows_T<HD>(row + static_cast<int64_t>(kvh) * HD, acc, role_a ? 1.f : args.scale, hl);
+      store_rows_T<HD>(row + static_cast<int64_t>(kvh) * HD, acc, role_a ? 1.f : grad_scale<MODE>(args), hl);
     }
   }
 }
@@ -592,7 +593,7 @@ void masked_bwd_bf16(const MaskedBwd& c, const MaskedArgs& a, hipStream_t stream
     if (hs.n > 1) {
       const int64_t threads = a.tokens * nkv * (HD / 8);
       hipLaunchKernelGGL((k_attn_dkdv_sum<HD>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream,
-                         hs, dk, c.lddk, dv, c.lddv, T, a.tokens, nkv, a.score.scale,
+                         hs, dk, c.lddk, dv, c.lddv, T, a.tokens, nkv, (MODE & kCap ? 4.f : 1.f) * a.score.scale,
                          RopeRows<uint16_t>{nullptr, nullptr, 0});
     }
   });

@@ -34,19 +34,24 @@ __device__ __forceinline__ void masked_step(const char* K, const char* V, const 
 #pragma unroll
     for (int s = 0; s < NS; ++s) x[t] = mfma(lds_frag<HD>(K, a_off, 32 * t, s), qf[s], x[t]);
   }
+  // What x holds now: raw products, under a cap alone r (which falls as the score rises), and
+  // with a bias the scores.
   if constexpr (MODE != 0) {
 #pragma unroll
     for (int t = 0; t < BN / 32; ++t)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x[t][j] = score(x[t][j], base - (32 * t + acc_row(j, 0)));
+      for (int j = 0; j < 16; ++j)
+        x[t][j] = MODE == kCap ? score.half_sigmoid(x[t][j]) : score(x[t][j], base - (32 * t + acc_row(j, 0)));
   }
-  mask_range(x[0], ends, starts, lo, hi, 0, -INFINITY);
-  mask_range(x[1], ends, starts, lo, hi, 32, -INFINITY);
-  float mloc = -INFINITY;
+  constexpr float kNone = MODE == kCap ? INFINITY : -INFINITY;
+  mask_range(x[0], ends, starts, lo, hi, 0, kNone);
+  mask_range(x[1], ends, starts, lo, hi, 32, kNone);
+  float mloc = kNone;
 #pragma unroll
   for (int t = 0; t < BN / 32; ++t)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) mloc = fmaxf(mloc, x[t][j]);
+    for (int j = 0; j < 16; ++j) mloc = MODE == kCap ? fminf(mloc, x[t][j]) : fmaxf(mloc, x[t][j]);
+  if constexpr (MODE == kCap) mloc = fmaf(score.c, mloc, score.b);
   mloc = xor32_max(mloc);
   if constexpr (MODE == 0) mloc *= score.a;
   if (wave_any(mloc > m + kRescaleSlack)) {
@@ -59,11 +64,15 @@ __device__ __forceinline__ void masked_step(const char* K, const char* V, const 
 #pragma unroll
       for (int j = 0; j < 16; ++j) oacc[dt][j] *= alpha;
   }
-  const float nm = -m;
+  const float nm = MODE == kCap ? score.b - m : -m;
 #pragma unroll
   for (int t = 0; t < BN / 32; ++t)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[t][j] = fast_exp2(MODE == 0 ? fmaf(x[t][j], score.a, nm) : x[t][j] + nm);
+    for (int j = 0; j < 16; ++j) {
+      if constexpr (MODE == 0) x[t][j] = fast_exp2(fmaf(x[t][j], score.a, nm));
+      else if constexpr (MODE == kCap) x[t][j] = fast_exp2(fmaf(score.c, x[t][j], nm));
+      else x[t][j] = fast_exp2(x[t][j] + nm);
+    }
   // The row sums add the bf16 weights that P V multiplies, so that the normalisation
   // matches the weights used.
   float lsum = 0.f;

@@ -218,6 +218,18 @@ __device__ __forceinline__ void mask_range(f32x16& x, bool ends, bool starts, in
   }
 }
 
+// What pack_frag's rounding leaves of entries j0 .. j0+7, rounded again.
+__device__ __forceinline__ bf16x8 rest_frag(const f32x16& acc, int j0) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = acc[j0 + 2 * i], b = acc[j0 + 2 * i + 1];
+    const uint32_t r = pk_bf16(a, b);
+    w[i] = pk_bf16(a - __uint_as_float(r << 16), b - __uint_as_float(r & 0xffff0000u));
+  }
+  return as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+}
+
 // acc += X^T f over rows row0 .. row0+15 of the tile X.
 template <int HD>
 __device__ __forceinline__ void wsum(f32x16 (&acc)[HD / 32], bf16x8 f, const char* tile, int b0, int b8, int row0) {

@@ -14,11 +14,17 @@ namespace fh {
 namespace {
 
 // ------------------------------------------------------------------------- dQ
-// One step of 64 keys of a wave (see masked_step).
+// One step of 64 keys of a wave (see masked_step).  dS enters its product in two bf16 parts,
+// the value and what rounding it left, on the same fragments of K; `sum` adds up dZ, which is
+// 0 over a row whose delta is exact.  delta comes from o, whose weights the forward rounded:
+// in rows that look at few tokens that error is as large as the roundings of dS and of dQ
+// together, 1.5 to 1.9 times what rounding dQ alone leaves; with the second part 1.05 to
+// 1.15 (8192 tokens, 32/8 heads of 128, capped: 2451 -> 2655 us for the backward; 16384
+// tokens, 32/4 heads of 64, documents of about 600, 305 -> 311).
 template <int HD, int MODE, bool CAREFUL>
 __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, const bf16x8 (&qf)[HD / 16],
-                                               const bf16x8 (&gf)[HD / 16], f32x16 (&dqacc)[HD / 32], float nlse2,
-                                               float dl, int a_off, int b0, int b8, const Score<MODE>& score,
+                                               const bf16x8 (&gf)[HD / 16], f32x16 (&dqacc)[HD / 32], float& sum,
+                                               float nlse2, float dl, int a_off, int b0, int b8, const Score<MODE>& score,
                                                float base, bool ends, bool starts, int lo, int hi, int hl) {
   constexpr int BN = 64, NS = HD / 16;
 #pragma unroll
@@ -33,10 +39,15 @@ __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, con
     for (int j = 0; j < 16; ++j) {
       float ds;
       const float p = score.weight(x[j], base - (32 * t + acc_row(j, 0)), nlse2, ds);
-      const float dz = p * (y[j] - dl);
-      x[j] = (MODE & kCap) ? dz * ds : dz;
+      x[j] = p * (y[j] - dl);
+      y[j] = ds;
     }
     mask_range(x, ends, starts, lo, hi, 32 * t, 0.f);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      sum += x[j];
+      if constexpr (MODE & kCap) x[j] *= y[j];
+    }
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
       const bf16x8 df = pack_frag(x, 8 * s2);
@@ -47,13 +58,19 @@ __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, con
           continue;
         }
       }
-      wsum<HD>(dqacc, df, K, b0, b8, row0);
+      const bf16x8 dr = rest_frag(x, 8 * s2);
+#pragma unroll
+      for (int dt = 0; dt < HD / 32; ++dt) {
+        const bf16x8 k = lds_frag_tr<HD>(K, b0, b8, row0, dt);
+        dqacc[dt] = mfma(k, df, dqacc[dt]);
+        dqacc[dt] = mfma(k, dr, dqacc[dt]);
+      }
     }
   }
 }
 
-// Also writes delta and -lse * log2(e) (plus cap_log2: see Score), which the dK/dV kernels
-// read.
+// Also writes -lse * log2(e) (plus cap_log2: see Score) and delta, put right by the sum of dZ,
+// which the dK/dV kernels read.
 template <int HD, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 3 : 2))) void k_masked_dq(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
@@ -112,13 +129,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
     if (qi < T) {
       const int64_t at = static_cast<int64_t>(h) * T + qi;
       nlse2 = fmaf(-kLog2e, lse[at], score.b);
-      if (hl == 0) {
-        delta[at] = dl;
-        nl2[at] = nlse2;
-      }
+      if (hl == 0) nl2[at] = nlse2;
     }
   }
   f32x16 dqacc[ND];
+  float sum = 0.f;  // of dZ over the lane's keys
   const bool some = sees.x < sees.y;
   if (n_steps > 0) {  // uniform
     const uint16_t* kp = k + static_cast<int64_t>(kbeg) * ldk + static_cast<int64_t>(kvh) * HD;
@@ -126,6 +141,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
     auto run = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) dqacc[dt] = zero16();
+      sum = 0.f;
       kv_block_loop<BN, HD, false, 4>(
           kp, ldk, vp, ldv, n_steps, T - kbeg, sk0, sk1, sv0, sv1, wave, lane,
           [&](int kb, const char* K, const char* V) __attribute__((always_inline)) {
@@ -133,7 +149,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
             const int k0 = kbeg + kb * BN;
             if (mine.x >= k0 + BN || mine.y <= k0) return;
             masked_dq_step<HD, MODE, decltype(careful)::value>(
-                K, V, qf, gf, dqacc, nlse2, dl, a_off, b0, b8, score, static_cast<float>(qi - k0 - 4 * hl),
+                K, V, qf, gf, dqacc, sum, nlse2, dl, a_off, b0, b8, score, static_cast<float>(qi - k0 - 4 * hl),
                 mine.w < k0 + BN, mine.z > k0, sees.x - k0 - 4 * hl, sees.y - k0 - 4 * hl, hl);
           },
           [] {});
@@ -142,6 +158,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 
     if (__builtin_expect(__syncthreads_or(some && not_finite<ND>(dqacc)), 0)) run(std::true_type{});
   }
   if (qi < T) {
+    const float off = xor32_sum(sum);
+    if (hl == 0) delta[static_cast<int64_t>(h) * T + qi] = dl + (some ? off : 0.f);
     if (!some) {
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) dqacc[dt] = zero16();

@@ -83,17 +83,17 @@ class MaskedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, slopes, args, seq_len):
         o, lse, low = ops.masked_attn_fwd_checked(args, q, k, v, table, slopes, True)
-        ctx.save_for_backward(q, k, v, o, lse, low, table, slopes)
-        ctx.args, ctx.seq_len = args, seq_len
+        ctx.save_for_backward(q, k, v, o, lse, low)
+        ctx.table, ctx.slopes, ctx.args, ctx.seq_len = table, slopes, args, seq_len  # the step's, not the layer's
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, low, table, slopes = ctx.saved_tensors
+        q, k, v, o, lse, low = ctx.saved_tensors
         # autograd hands the gradient in of the output's shape, dtype and device
         do, lddo = _laid_out(do, ctx.seq_len)
-        return (*ops.masked_attn_bwd_checked(ctx.args, q, k, v, o, do, lddo, lse, low, table, slopes), None, None, None, None)
+        return (*ops.masked_attn_bwd_checked(ctx.args, q, k, v, o, do, lddo, lse, low, ctx.table, ctx.slopes), None, None, None, None)
 
 
 def _score(name: str, head_dim: int, scale: float | None, cap: float | None,

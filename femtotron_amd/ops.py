@@ -732,8 +732,9 @@ def masked_attn_check(name: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     dev = q.get_device()
     if table.get_device() != dev:
         _require_gpu(q, table)
-    wq, wk = q.size(-1), k.size(-1)
-    if head_dim <= 0 or wq % head_dim or wk % head_dim or k.shape != v.shape or q.shape[:-1] != k.shape[:-1] \
+    q_shape, k_shape = q.shape, k.shape
+    wq, wk = q_shape[-1], k_shape[-1]
+    if head_dim <= 0 or wq % head_dim or wk % head_dim or k_shape != v.shape or q_shape[:-1] != k_shape[:-1] \
             or q.numel() != tokens * wq:
         raise ValueError(f"{name}: q must be [{tokens}, heads * {head_dim}], k and v [{tokens}, kv heads * {head_dim}], "
                          f"got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
@@ -753,12 +754,12 @@ def masked_attn_fwd_checked(args: tuple, q: torch.Tensor, k: torch.Tensor, v: to
     """masked_attn_fwd of tensors that are known to fit; args: (dtype code, ldq, ldk, ldv, tokens,
     n_heads, n_kv_heads, head_dim, scale, cap).  o has q's shape."""
     dt, ldq, ldk, ldv, T, nh, nkv, hd, scale, cap = args
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = q.new_empty(q.shape)
     lse = low = None
     if need_grad:
-        lse = torch.empty((nh, T), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((nh, T), dtype=torch.float32)
         if dt == _lib.FH_BF16:
-            low = torch.empty(q.shape, dtype=torch.int8, device=q.device)
+            low = q.new_empty(q.shape, dtype=torch.int8)
     _launch("fh_masked_attn_fwd", q, dt, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), nh * hd,
             _ptr(lse), _ptr(low), table.data_ptr(), T, nh, nkv, hd, scale, cap, _ptr(slopes))
     return o, lse, low
@@ -768,9 +769,8 @@ def masked_attn_bwd_checked(args: tuple, q, k, v, o, dout, lddo: int, lse, o_low
     """masked_attn_bwd of tensors that are known to fit (o contiguous, dout of row stride lddo);
     args: masked_attn_fwd_checked's.  dq, dk, dv have q's, k's and v's shapes."""
     dt, ldq, ldk, ldv, T, nh, nkv, hd, scale, cap = args
-    device, dtype = q.device, q.dtype
-    dq, dk, dv = (torch.empty(t.shape, dtype=dtype, device=device) for t in (q, k, v))
-    ws = torch.empty(max(_lib.lib().fh_masked_attn_bwd_workspace_size(dt, T, nh, nkv, hd), 4), dtype=torch.uint8, device=device)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    ws = q.new_empty(max(_lib.lib().fh_masked_attn_bwd_workspace_size(dt, T, nh, nkv, hd), 4), dtype=torch.uint8)
     _launch("fh_masked_attn_bwd", q, dt, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), nh * hd,
             dout.data_ptr(), lddo, lse.data_ptr(), _ptr(o_low), dq.data_ptr(), nh * hd, dk.data_ptr(), nkv * hd, dv.data_ptr(),
             nkv * hd, table.data_ptr(), ws.data_ptr(), T, nh, nkv, hd, scale, cap, _ptr(slopes))

@@ -15,8 +15,8 @@
 // straight into the wave's own LDS, the next tile's while this one is multiplied, without a
 // barrier (vmcnt alone).  S^T = K Q^T with one column a lane, an online softmax in fp32,
 // O^T += V^T P^T, as in the forward under a mask; the waves' results meet in LDS, and the
-// shares' in a second kernel.  Where the room is small, one workgroup takes a sequence, and
-// there is no second kernel.
+// shares' in a second kernel.  Where the room is small or sequences are many, one workgroup
+// takes a sequence, and there is no second kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -539,9 +539,21 @@ __global__ __launch_bounds__(256) void k_cache_attn_f32(CacheArgs c) {
 // Workgroups that run at once: by their LDS one a CU at head_dim 128, two below.
 int64_t workgroups(int64_t head_dim) { return head_dim == 128 ? 256 : 512; }
 
-// The room up to which a workgroup takes a whole sequence: there the time is the loads one
-// after another and the launches, and one more launch costs more than tiles in turn.
-int64_t whole_room(int64_t head_dim) { return head_dim == 128 ? 1024 : 2048; }
+// Whether a workgroup takes a whole sequence: in small rooms, where the time is the loads one
+// after another and the launches, and one more launch costs more than tiles in turn; in larger
+// ones where the sequences give workgroups enough by themselves, as shares of short sequences
+// are several segments in turn and have to be joined.  The larger the room the more a single
+// long sequence among short ones would cost, so there more workgroups are asked for.  bf16,
+// lengths even over [1, room], in shares -> whole, 32/8 heads of 128: 64 sequences of 1280
+// 47 -> 37 us, of 4096 132 -> 118, 128 of 8192 422 -> 399 (one long among short: 41 -> 23,
+// 66 -> 41, 94 -> 87); 32/4 heads of 64: 256 of 8192 212 -> 199, but 128 of 16384 202 -> 225.
+// The fp32 kernel takes a place slower, and loses there: 256 of 8192 355 -> 539.
+bool whole_sequences(fh_dtype dt, int64_t room, int64_t head_dim, int64_t workgroups_of_all) {
+  const int64_t small = head_dim == 128 ? 1024 : 2048;
+  if (room <= small || dt == FH_F32) return room <= small;
+  return (room <= 4 * small && workgroups_of_all >= workgroups(head_dim)) ||
+         (room <= 8 * small && workgroups_of_all >= 2 * workgroups(head_dim));
+}
 
 struct CachePlan {
   int64_t tiles, wanted, slots, items;  // items: slots * kv heads * tiles
@@ -553,7 +565,7 @@ CachePlan cache_plan(fh_dtype dt, int64_t batch, int64_t n_new, int64_t room, in
   CachePlan p{};
   const int64_t cols = dt == FH_BF16 ? 32 : kColsF32;
   p.tiles = (n_heads / n_kv_heads * n_new + cols - 1) / cols;
-  p.split = room > whole_room(head_dim);
+  p.split = !whole_sequences(dt, room, head_dim, batch * n_kv_heads * p.tiles);
   if (p.split) {
     p.wanted = std::max<int64_t>(1, workgroups(head_dim) / (n_kv_heads * p.tiles));
     p.wanted = std::min(p.wanted, batch * ((room + kShare - 1) / kShare));

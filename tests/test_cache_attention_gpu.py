@@ -87,6 +87,11 @@ def test_more_columns_than_a_workgroup_takes():
     _compare(300, 20, 200, [200 - b % 190 for b in range(300)], 8, 4, 32, BF, seed=132)  # a chunk a sequence
 
 
+def test_sequences_enough_for_the_chip():
+    """A workgroup a sequence and head, whatever the room."""
+    _compare(1100, 1, 2300, [2300 if b % 100 == 0 else 1 + 7 * b % 60 for b in range(1100)], 4, 4, 32, BF, seed=135)
+
+
 def test_lengths_past_the_room_and_below_nothing():
     from femtotron_amd import cache_attention
     q, k, v = _inputs(4, 2, 300, 4, 2, 64, BF, 140)

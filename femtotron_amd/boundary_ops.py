@@ -76,6 +76,8 @@ class FusedEmbedding(nn.Module):
     """Token embedding on the fused kernels; ``weight`` is the replaced module's Parameter.
     Its rows come out times ``factor`` (``embedding``)."""
 
+    factor = 1.0  # of modules that were pickled before they had one
+
     def __init__(self, weight: nn.Parameter, padding_idx: int | None = None, factor: float = 1.0):
         super().__init__()
         self.weight = weight

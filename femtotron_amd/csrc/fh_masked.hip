@@ -125,6 +125,11 @@ __global__ __launch_bounds__(1024) void k_mask_order(MaskTable m, int T, int* __
   for (int i = tid; i < n; i += 1024) order[atomicAdd(&at[bucket(i)], 1)] = i;
 }
 
+constexpr float kMostScale = 1152921504606846976.f;  // what scores are made of stays finite
+// tanh as 1 - 2 r is off by 2^-23 of the cap: from here on that would be more in a score than
+// the rounding of a bf16 weight is in its logarithm (2^-9, halved twice).
+constexpr float kMostCap = 4096.f;
+
 int check_tokens(const char* name, int64_t tokens) {
   if (tokens < 0 || tokens > (int64_t(1) << 30)) return fail(FH_ERR_INVALID, std::string(name) + ": tokens must be 0 to 2^30");
   return FH_OK;
@@ -140,8 +145,10 @@ int masked_args(const char* name, fh_dtype dt, int64_t tokens, int64_t n_heads, 
   if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65535)
     return fail(FH_ERR_INVALID, n + ": n_heads must be a positive multiple of n_kv_heads, at most 65535");
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) return fail(FH_ERR_INVALID, n + ": head_dim must be 32, 64 or 128");
-  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(FH_ERR_INVALID, n + ": scale must be positive and finite");
+  if (!(scale > 0.f) || !(scale <= kMostScale)) return fail(FH_ERR_INVALID, n + ": scale must be positive, at most 2^60");
   if (!(cap >= 0.f) || !(cap < INFINITY)) return fail(FH_ERR_INVALID, n + ": cap must be 0 (none) or positive and finite");
+  if (dt == FH_BF16 && cap > kMostCap) return fail(FH_ERR_INVALID, n + ": cap must be at most 4096 in bf16");
+  if (cap > 0.f && !(scale / cap <= kMostScale)) return fail(FH_ERR_INVALID, n + ": cap is too small for the scale");
   a.tokens = tokens;
   a.n_heads = n_heads;
   a.n_kv_heads = n_kv_heads;
@@ -181,7 +188,8 @@ extern "C" int fh_attn_mask(const int64_t* starts, const int64_t* lengths, const
                             hipStream_t stream) {
   if (int e = check_tokens("attn_mask", tokens)) return e;
   FH_REQUIRE(n_documents >= 0 && n_documents <= (int64_t(1) << 31), "attn_mask: bad number of documents");
-  FH_REQUIRE(starts != nullptr || n_documents == 0 || (seq_len > 0 && n_documents * seq_len == tokens),
+  FH_REQUIRE(starts != nullptr || n_documents == 0 ||
+                 (seq_len > 0 && seq_len <= tokens && tokens % seq_len == 0 && tokens / seq_len == n_documents),
              "attn_mask: without starts the documents' seq_len rows must make up the tokens");
   FH_REQUIRE(window >= 0, "attn_mask: window must be 0 (none) or positive");
   FH_REQUIRE(prefix == nullptr || (causal && window == 0), "attn_mask: a prefix goes with causal and without a window");

@@ -64,7 +64,7 @@ __device__ __forceinline__ int4 mask_bounds(const int4* b, int t, int tiles) {
 // on every XCD (workgroup L runs on XCD L % 8): with a multiple of eight heads each XCD has
 // heads of its own, whose tensors stay in its L2; else ranks and heads are dealt out in turn.
 // 16384 tokens in rows of 2048, 32/4 heads of 64, backward: XCDs by position in the row (block
-// x on XCD x % 8) 956 us, dealt out by falling work 567.
+// x on XCD x % 8) 956 us, dealt out by falling work 635.
 __device__ __forceinline__ XcdOrder masked_order() {
   if (gridDim.y % 8 == 0) return xcd_order();
   const int L = blockIdx.x + gridDim.x * blockIdx.y, ny = gridDim.y;

@@ -83,17 +83,17 @@ class MaskedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, slopes, args, seq_len):
         o, lse, low = ops.masked_attn_fwd_checked(args, q, k, v, table, slopes, True)
-        ctx.save_for_backward(q, k, v, o, lse, low)
-        ctx.table, ctx.slopes, ctx.args, ctx.seq_len = table, slopes, args, seq_len  # the step's, not the layer's
+        ctx.save_for_backward(q, k, v, o, lse, low, slopes)
+        ctx.table, ctx.args, ctx.seq_len = table, args, seq_len  # the table is the step's, not the layer's
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, low = ctx.saved_tensors
+        q, k, v, o, lse, low, slopes = ctx.saved_tensors
         # autograd hands the gradient in of the output's shape, dtype and device
         do, lddo = _laid_out(do, ctx.seq_len)
-        return (*ops.masked_attn_bwd_checked(ctx.args, q, k, v, o, do, lddo, lse, low, ctx.table, ctx.slopes), None, None, None, None)
+        return (*ops.masked_attn_bwd_checked(ctx.args, q, k, v, o, do, lddo, lse, low, ctx.table, slopes), None, None, None, None)
 
 
 def _score(name: str, head_dim: int, scale: float | None, cap: float | None,
@@ -124,9 +124,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     it see; differentiable in q, k and v (once, and in reverse mode).
 
     head_dim 32, 64 or 128; ``scale`` (None: head_dim ** -0.5) on the products; ``cap``: scores
-    become cap * tanh(score / cap); ``slopes`` (fp32, one a query head): less slopes[h] times
-    the distance, after the cap.  bf16 or fp32 on a HIP device.  Nothing that a token does not
-    see reaches it, infinities and NaN included."""
+    become cap * tanh(score / cap) (bf16: a cap of at most 4096); ``slopes`` (fp32, one a
+    query head): less slopes[h] times the distance, after the cap.  bf16 or fp32 on a HIP
+    device.  Nothing that a token does not see reaches it, infinities and NaN included."""
     scale, cap = _score("masked_attention", head_dim, scale, cap, slopes)
     seq_len = mask.seq_len
     tokens = mask.batch * seq_len

@@ -952,13 +952,14 @@ def clip_grads(grads: list, outs: list | None, max_norm: float) -> torch.Tensor:
     for ts in (grads,) if outs is None or in_place else (grads, outs):
         if dev < 0 or any([t.get_device() != dev for t in ts]):
             _require_gpu(first, *ts)
-        if not all([t.is_contiguous() for t in ts]):
+        if not all([t.layout == torch.strided and t.is_contiguous() for t in ts]):
             all_contiguous = False
             if not all([t.layout == torch.strided and torch.ops.aten.is_non_overlapping_and_dense(t) for t in ts]):
                 raise ValueError("clip_gradients: gradients must be dense")
     if outs is not None and not in_place:
         if [t.shape for t in grads] != [t.shape for t in outs] \
-                or not (all_contiguous or [t.stride() for t in grads] == [t.stride() for t in outs]):
+                or not (all_contiguous or all([a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
+                                               for a, b in zip(grads, outs)])):
             raise ValueError("clip_gradients: an output must have its gradient's shape and strides")
     n = len(grads)
     table = (_lib.FhGrad * n)()

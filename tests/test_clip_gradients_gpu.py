@@ -79,6 +79,17 @@ def test_mixed_types_views_and_unaligned_tensors():
     assert torch.equal(base[9000:], rest) and float(base[8194]) == float(randn((40000,), 3)[8194])
 
 
+def test_outputs_of_mixed_strides():
+    """A pair of one transposed layout beside a pair whose strides differ in a dim of one alone."""
+    from femtotron_amd.optim import clip_gradients
+    a, b = randn((30, 20), 7).to(DEV).t(), randn((1, 50), 8).to(DEV)
+    oa, ob = torch.empty(30, 20, device=DEV).t(), torch.empty(50, device=DEV).as_strided((1, 50), (77, 1))
+    norm, f = _expect([a, b], 1.0)
+    clip_gradients([a, b], 1.0, out=[oa, ob])
+    _close(oa, a, f)
+    _close(ob, b, f)
+
+
 def test_as_torch_clips():
     """torch's own clipping of the same gradients: its norm is a sum in fp32 (here of 1e5 squares:
     2^-24 times their number's root, tenfold), its factor rounded in fp32."""
@@ -166,6 +177,8 @@ def test_refusals():
     for bad in (-1.0, float("nan")):
         with pytest.raises(ValueError):
             clip_gradients([g], bad)
+    with pytest.raises((ValueError, RuntimeError, TypeError)):
+        clip_gradients([torch.eye(4, device=DEV).to_sparse()], 1.0)
     assert torch.equal(g, torch.ones_like(g))
     assert float(clip_gradients([], 1.0)) == 0.0
     assert float(clip_gradients([g[:0]], 1.0)) == 0.0

@@ -110,6 +110,15 @@ def test_scores(score, hd, dtype):
     _compare(2, 100, dict(window=30, causal=False), nh, 4, hd, dtype, std=3.0, seed=31, **score)
 
 
+def test_large_and_small_caps():
+    """A cap that scores never reach is none, one far below them leaves its sign: within the bounds,
+    which hold 2^-23 of the cap."""
+    for cap in (4096.0, 500.0, 0.01):
+        _compare(1, 130, {}, 2, 1, 64, BF, seed=35, std=2.0, cap=cap)
+    for cap in (1e6, 1e-3):
+        _compare(1, 130, {}, 2, 1, 64, FP, seed=36, std=2.0, cap=cap)
+
+
 def test_a_long_row_in_every_kernel():
     """Several steps of every loop, documents that end inside tiles; heads enough to pair."""
     starts = [0, 700, 701, 1500, 1777]

@@ -78,6 +78,7 @@ def test_entry_points_validate_on_the_host():
     assert L.fh_attn_mask(None, None, None, 0, 0, 5, 0, 1, None, None) == 0  # no tokens
     refused(L.fh_attn_mask(None, None, None, 2, 10, 4, 0, 1, 16, None), b"seq_len")
     refused(L.fh_attn_mask(None, None, None, 1, BIG, BIG, 0, 1, 16, None), b"tokens")
+    refused(L.fh_attn_mask(None, None, None, 1 << 31, 1 << 30, 1 << 62, 0, 1, 16, None), b"seq_len")
     refused(L.fh_attn_mask(16, None, 16, 1, 10, 10, 3, 1, 16, None), b"prefix")
     refused(L.fh_attn_mask(16, None, 16, 1, 10, 10, 0, 0, 16, None), b"prefix")
     refused(L.fh_attn_mask(16, None, None, 1, 10, 10, -1, 1, 16, None), b"window")
@@ -96,6 +97,9 @@ def test_entry_points_validate_on_the_host():
     refused(fwd_(scale=float("nan")), b"scale")
     refused(fwd_(cap=-1.0), b"cap")
     refused(fwd_(cap=float("inf")), b"cap")
+    refused(fwd_(cap=4097.0), b"cap")
+    refused(fwd_(cap=1e-30, scale=1.0), b"cap")
+    refused(fwd_(scale=2.0 ** 61), b"scale")
     refused(fwd_(q=None), b"null")
     refused(fwd_(q=8), b"aligned")
     refused(fwd_(dt=1, low=16), b"o_low")
@@ -120,6 +124,7 @@ def test_entry_points_validate_on_the_host():
     assert cache(batch=0) == 0 and cache(n_new=0) == 0
     assert L.fh_cache_attn_workspace_size(0, 2, 1, 100, 2, 1, 64) == 0  # a workgroup a sequence: nothing to join
     assert L.fh_cache_attn_workspace_size(0, 2, 1, 5000, 2, 1, 64) > 0
+    assert L.fh_cache_attn_workspace_size(0, 4096, 1, 5000, 2, 1, 64) == 0  # sequences enough for the chip
 
     refused(L.fh_embedding_scaled_fwd(0, 16, 16, 16, 1, 10, 64, float("inf"), None), b"factor")
     refused(L.fh_embedding_scaled_bwd(0, 16, 16, 16, 1, 10, 64, -1, float("nan"), 16, None), b"factor")
@@ -237,6 +242,9 @@ def test_the_embedding_modules_cpu_path_has_the_factor():
     assert torch.equal(y[0], 3 * w[3]) and torch.equal(y[3], 3 * w[0]) and not y[1:3].any()
     y.sum().backward()
     assert float(w.grad.sum()) == 2 * 16 * 3.0
+    old = FusedEmbedding(w)
+    del old.__dict__["factor"]  # as a module pickled before it had one
+    assert torch.equal(old(ids)[0], w[3])
 
 
 # --------------------------------------------------------------------- the oracle

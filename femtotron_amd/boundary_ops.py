@@ -66,6 +66,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, factor: float = 1.0,
     if ops.wants_derivative(factor):
         raise TypeError("embedding: factor is a constant and gets no gradient")
     factor = float(factor)
+    if padding_idx is not None and not (weight.dim() == 2 and 0 <= padding_idx < weight.shape[0]):
+        raise ValueError(f"embedding: padding_idx must be an id of the vocabulary, or None, got {padding_idx}")
     ids, weight = ids.contiguous(), ops.aligned(weight)
     if ops.differentiated(weight):
         return FusedEmbeddingFunction.apply(ids, weight, padding_idx, factor)

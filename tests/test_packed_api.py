@@ -247,6 +247,14 @@ def test_the_embedding_modules_cpu_path_has_the_factor():
     assert torch.equal(old(ids)[0], w[3])
 
 
+@pytest.mark.parametrize("padding_idx", [-1, 10, -11])
+def test_an_embeddings_padding_idx_is_an_id(padding_idx):
+    """Python's negative index would be taken for no padding."""
+    from femtotron_amd import embedding
+    with pytest.raises(ValueError, match="padding_idx"):
+        embedding(torch.tensor([3]), torch.zeros(10, 16), padding_idx=padding_idx)
+
+
 # --------------------------------------------------------------------- the oracle
 def test_the_oracle_is_softmax_attention():
     """Against torch's own fp64 attention and its gradients, where the mask is one that it has."""

@@ -293,6 +293,9 @@ __device__ __forceinline__ void cache_segment(const CacheArgs& c, char* lds, flo
   }
 }
 
+// 32 sequences in a room of 8192, 32/8 heads of 128, capped: 100-105 us, 4.8-5.1 TB/s; 2 of up
+// to 32768, 32 heads of 128, 5 new tokens: 135-141 us, 5.3-5.5; one of 2048, 32/4 heads of
+// 64: 10 us, the loads of one workgroup a head one after another.
 template <int HD, int MODE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 1 : 2))) void k_cache_attn(CacheArgs c) {
   constexpr int TILE = kPlaces * 2 * HD;

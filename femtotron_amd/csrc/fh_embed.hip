@@ -299,7 +299,7 @@ __global__ __launch_bounds__(kGroupThreads) void k_embed_group(const int64_t* __
 // V = 32000, H = 2048, whose bytes take 38 us.  So the grid's first workgroups
 // take the rows of kHotTokens and more: a wave sums 128 columns of such a row
 // (2 per lane) with the rows of up to kHotDepth tokens in flight, the additions
-// still one after the other in token order: 58-62 us there.  (One wave per row and
+// still one after the other in token order: 54-56 us there.  (One wave per row and
 // 1024 threads per workgroup, the tokens read as scalars: 132 us.)
 //
 // A hot workgroup looks through hot_ids consecutive ids and sums its frequent ones

@@ -70,7 +70,9 @@ __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, con
 }
 
 // Also writes -lse * log2(e) (plus cap_log2: see Score) and delta, put right by the sum of dZ,
-// which the dK/dV kernels read.
+// which the dK/dV kernels read.  142-147 us at 16384 tokens, 32/4 heads of 64, documents of
+// about 600; 1100-1140 at 8192 tokens, 32/8 heads of 128, capped: bound by the vector work of
+// scores and dS and, at 128, by two waves a SIMD that cover each other's waits in part.
 template <int HD, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 3 : 2))) void k_masked_dq(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
@@ -263,7 +265,8 @@ __device__ __forceinline__ void masked_dkdv_item(const char* Q, const char* G, c
 
 // Up to head_dim 64: 8 waves, 128 keys; wave w holds K and V of keys 32 (w % 4) .. +31 in
 // registers and takes queries 32 (w / 4) .. +31 of each 64-query item; the halves' sums
-// meet in LDS at the end, in a fixed order.  Two items a stage, two stages.
+// meet in LDS at the end, in a fixed order.  Two items a stage, two stages.  190-199 us at
+// 16384 tokens, 32/4 heads of 64, documents of about 600.
 constexpr int kFusedKeys = 128;
 
 template <int HD, int MODE>
@@ -400,6 +403,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
 
 // head_dim 128: 4 waves, 64 keys; each 32 keys are shared by a wave that holds K and sums
 // dV (role A: S, P, handed over through LDS) and one that holds V and sums dK (role B).
+// 1650-1770 us at 8192 tokens, 32/8 heads of 128, capped: the matrix units are busy 28% of it
+// and the vector units 36%, the rest are the roles' waits for one another and for LDS.  (The
+// roles of a workgroup's waves swapped in every other one, so that each SIMD has both: 2631
+// -> 2644 us for the backward.)
 constexpr int kSplitKeys = 64;
 
 template <int HD, int MODE>

@@ -92,8 +92,10 @@ __device__ __forceinline__ void masked_step(const char* K, const char* V, const 
 }
 
 // Four waves a SIMD up to head_dim 64: what the registers (128) then lack is spilled in the
-// careful pass alone.  16384 tokens, 32/4 heads of 64, documents of about 600: 124 us with
-// three waves a SIMD (one workgroup a CU), 104 with four.
+// careful pass alone.  16384 tokens, 32/4 heads of 64, documents of about 600: 105 us with
+// three waves a SIMD (one workgroup a CU), 83 with four (390 TFLOP/s; the softmax's vector
+// work is of the order of the products' time).  8192 tokens, 32/8 heads of 128, capped: 657 us,
+// 840 TFLOP/s; without the cap 542.
 // HPB = 2: 8 waves take the same rows of two query heads of one kv head, which read the
 // same K and V tiles.
 template <int HD, int HPB, int MODE>
@@ -198,8 +200,11 @@ __global__ __launch_bounds__(256 * HPB) __attribute__((amdgpu_waves_per_eu(HD ==
 
 void masked_fwd_bf16(const MaskedFwd& c, const MaskedArgs& a, hipStream_t stream) {
   const int group = static_cast<int>(a.n_heads / a.n_kv_heads);
-  const bool pair = group % 2 == 0 && (a.n_heads / 2) % 8 == 0;
-  const dim3 grid(static_cast<unsigned>((a.tokens + 127) / 128), static_cast<unsigned>(a.n_heads / (pair ? 2 : 1)));
+  const int64_t blocks = (a.tokens + 127) / 128;
+  // Pairs of heads where they leave a workgroup for every CU: 8192 tokens, 32/8 heads of 128, 565
+  // -> 542 us, 16384 tokens of 32/4 heads of 64 183 -> 171; but 999 tokens of those 16 -> 18 (capped 22).
+  const bool pair = group % 2 == 0 && (a.n_heads / 2) % 8 == 0 && blocks * (a.n_heads / 2) >= 256;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.n_heads / (pair ? 2 : 1)));
   dispatch_masked(a.head_dim, a.mode, [&](auto hd, auto mode) {
     auto launch = [&](auto hpb) {
       hipLaunchKernelGGL((k_masked_fwd<hd(), hpb(), mode()>), grid, dim3(256 * hpb()), 0, stream,

@@ -420,8 +420,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
   // stage's array, so the compiler knows which array a read touches.
   __shared__ __align__(16) char st0[2 * TILE], st1[2 * TILE];
   __shared__ __align__(16) float sl0[64], sl1[64], sd0[64], sd1[64];
-  // P and, under a cap, dz/ds of each 32 keys, [j/4][lane][4].
-  __shared__ __align__(16) float sp[NKS][16 * 64], st[(MODE & kCap) ? NKS : 1][(MODE & kCap) ? 16 * 64 : 1];
+  // P, under a cap times dz/ds, of each 32 keys, [j/4][lane][4].
+  __shared__ __align__(16) float sp[NKS][16 * 64];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool role_a = wave < NKS;
@@ -495,11 +495,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
             mask_range(x, ends, starts, lo, hi, 0, 0.f);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
+              if constexpr (MODE & kCap) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ds[4 * g + e] *= x[4 * g + e];
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ds[4 * g + e] = x[4 * g + e];
+              }
               *reinterpret_cast<float4*>(&sp[sub][(g * 64 + lane) * 4]) =
-                  make_float4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]);
-              if constexpr (MODE & kCap)
-                *reinterpret_cast<float4*>(&st[sub][(g * 64 + lane) * 4]) =
-                    make_float4(ds[4 * g], ds[4 * g + 1], ds[4 * g + 2], ds[4 * g + 3]);
+                  make_float4(ds[4 * g], ds[4 * g + 1], ds[4 * g + 2], ds[4 * g + 3]);
             }
           }
         }
@@ -512,16 +516,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
               const float4 P4 = *reinterpret_cast<const float4*>(&sp[sub][(g * 64 + lane) * 4]);
               const float Dv[4] = {D4.x, D4.y, D4.z, D4.w};
               const float Pv[4] = {P4.x, P4.y, P4.z, P4.w};
-              float Sv[4] = {1.f, 1.f, 1.f, 1.f};
-              if constexpr (MODE & kCap) {
-                const float4 S4 = *reinterpret_cast<const float4*>(&st[sub][(g * 64 + lane) * 4]);
-                Sv[0] = S4.x; Sv[1] = S4.y; Sv[2] = S4.z; Sv[3] = S4.w;
-              }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float dz = Pv[e] * (x[4 * g + e] - Dv[e]);
-                x[4 * g + e] = (MODE & kCap) ? dz * Sv[e] : dz;
-              }
+              for (int e = 0; e < 4; ++e) x[4 * g + e] = Pv[e] * (x[4 * g + e] - Dv[e]);
             }
             // P is 0 there, but what it is multiplied by need not be finite
             mask_range(x, ends, starts, lo, hi, 0, 0.f);

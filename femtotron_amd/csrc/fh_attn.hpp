@@ -224,10 +224,9 @@ __device__ __forceinline__ void store_rows_T_f32(float* out_row, const f32x16 (&
 
 // One thread: dims d .. d+3 and d + HD/2 .. of one (token, kv head) of dK and dV.
 template <int HD>
-__global__ __launch_bounds__(256) void k_attn_dkdv_sum(HeadSplit hs, uint16_t* __restrict__ dk, int64_t lddk,
-                                                       uint16_t* __restrict__ dv, int64_t lddv, int S,
-                                                       int64_t tokens, int nkv, float scale,
-                                                       RopeRows<uint16_t> rope) {
+__device__ __forceinline__ void attn_dkdv_sum(HeadSplit hs, uint16_t* __restrict__ dk, int64_t lddk,
+                                              uint16_t* __restrict__ dv, int64_t lddv, int S, int64_t tokens, int nkv,
+                                              float scale, RopeRows<uint16_t> rope) {
   constexpr int C = HD / 8;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= tokens * nkv * C) return;
@@ -268,6 +267,14 @@ __global__ __launch_bounds__(256) void k_attn_dkdv_sum(HeadSplit hs, uint16_t* _
     *reinterpret_cast<uint2*>(out) = make_uint2(pk_bf16(a[0], a[1]), pk_bf16(a[2], a[3]));
     *reinterpret_cast<uint2*>(out + HD / 2) = make_uint2(pk_bf16(a[4], a[5]), pk_bf16(a[6], a[7]));
   }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void k_attn_dkdv_sum(HeadSplit hs, uint16_t* __restrict__ dk, int64_t lddk,
+                                                       uint16_t* __restrict__ dv, int64_t lddv, int S,
+                                                       int64_t tokens, int nkv, float scale,
+                                                       RopeRows<uint16_t> rope) {
+  attn_dkdv_sum<HD>(hs, dk, lddk, dv, lddv, S, tokens, nkv, scale, rope);
 }
 
 // ------------------------------------------------------------- fp32 operands

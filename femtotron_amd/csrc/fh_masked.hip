@@ -97,7 +97,7 @@ __global__ __launch_bounds__(1024) void k_mask_order(MaskTable m, int T, int* __
   const int4* bounds = which == 0 ? m.keys : m.queries;
   int* order = which == 0 ? order_q : which == 1 ? order_k128 : order_k64;
   const int n = (T + rows - 1) / rows, tiles = (T + kMaskRows - 1) / kMaskRows, per = rows / kMaskRows;
-  const int unit = max(32, (T + 1022) / 1023);
+  const int unit = order_unit(T);
   auto bucket = [&](int i) {
     int lo = 0x7fffffff, hi = 0;
     for (int t = i * per; t < min((i + 1) * per, tiles); ++t) {

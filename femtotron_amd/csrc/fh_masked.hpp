@@ -60,6 +60,9 @@ __device__ __forceinline__ int4 mask_bounds(const int4* b, int t, int tiles) {
                    __builtin_amdgcn_readfirstlane(r.z), __builtin_amdgcn_readfirstlane(r.w));
 }
 
+// The order's buckets: blocks whose lengths are the same in these units come in any order.
+__device__ __forceinline__ int order_unit(int T) { return max(32, (T + 1022) / 1023); }
+
 // Which block and head (y) a workgroup takes.  Ranks run by falling work, the heaviest first
 // on every XCD (workgroup L runs on XCD L % 8): with a multiple of eight heads each XCD has
 // heads of its own, whose tensors stay in its L2; else ranks and heads are dealt out in turn.
@@ -69,6 +72,14 @@ __device__ __forceinline__ XcdOrder masked_order() {
   if (gridDim.y % 8 == 0) return xcd_order();
   const int L = blockIdx.x + gridDim.x * blockIdx.y, ny = gridDim.y;
   return {L / ny, L % ny};
+}
+// The same of the grid's first `ny` heads' worth of workgroups; y = ny: none is left.
+__device__ __forceinline__ XcdOrder masked_order(int ny) {
+  const int L = blockIdx.x + gridDim.x * blockIdx.y;
+  if (L >= static_cast<int>(gridDim.x) * ny) return {0, ny};
+  if (ny % 8 != 0) return {L / ny, L % ny};
+  const int j = L >> 3, nyx = ny >> 3;
+  return {j / nyx, (L & 7) * nyx + j % nyx};
 }
 
 // --------------------------------------------------------------------- scores
@@ -283,7 +294,7 @@ void masked_bwd_f32(const MaskedBwd& c, const MaskedArgs& a, hipStream_t stream)
 // from `parts` on the sums of a kv head's query heads where they are split.
 struct MaskedWorkspace {
   int64_t parts, total;
-  int split;
+  int split, long_split;  // where what sees the keys is long (long_split >= split)
 };
 MaskedWorkspace masked_workspace(fh_dtype dt, int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim);
 

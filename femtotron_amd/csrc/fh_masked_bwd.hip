@@ -403,18 +403,42 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
 
 // head_dim 128: 4 waves, 64 keys; each 32 keys are shared by a wave that holds K and sums
 // dV (role A: S, P, handed over through LDS) and one that holds V and sums dK (role B).
-// 1650-1770 us at 8192 tokens, 32/8 heads of 128, capped: the matrix units are busy 28% of it
-// and the vector units 36%, the rest are the roles' waits for one another and for LDS.  (The
+// 1350-1450 us at 8192 tokens, 32/8 heads of 128, capped: the matrix units are busy a third of it
+// and the vector units 40%, the rest are the roles' waits for one another.  (The
 // roles of a workgroup's waves swapped in every other one, so that each SIMD has both: 2631
 // -> 2644 us for the backward.)
 constexpr int kSplitKeys = 64;
+
+// Workgroups that a kv head's query heads are split over: `split`, or hs.n where the block
+// that is seen by most is seen by about kLongRows rows or more (in the order's buckets, so that it
+// does not hang on which of a bucket comes first).  The workgroups of long rows are few and of
+// unlike length, and the last of them leave a CU to themselves; the sums of the parts cost the same
+// in short ones, where nothing is gained.  The backward with twice the parts, 8192 tokens, 32/8
+// heads: one document 2303 -> 2155 us, documents of 600 283 -> 316.
+constexpr int kLongRows = 4096;
+__device__ __forceinline__ int dkdv_split(const MaskTable& mask, int T, const HeadSplit& hs, int split) {
+  if (split == hs.n || mask.order_k64 == nullptr) return split;
+  const int4 most = mask_bounds<kSplitKeys / kMaskRows>(mask.queries, mask.order_k64[0] * (kSplitKeys / kMaskRows),
+                                                        (T + kMaskRows - 1) / kMaskRows);
+  const int unit = order_unit(T);
+  return most.y > most.x && (most.y - most.x + unit - 1) / unit * unit >= kLongRows ? hs.n : split;
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void k_masked_dkdv_sum(HeadSplit hs, int split, MaskTable mask, uint16_t* __restrict__ dk,
+                                                         int64_t lddk, uint16_t* __restrict__ dv, int64_t lddv, int T,
+                                                         int nkv, float scale) {
+  hs.n = dkdv_split(mask, T, hs, split);
+  if (hs.n > 1) attn_dkdv_sum<HD>(hs, dk, lddk, dv, lddv, T, T, nkv, scale, RopeRows<uint16_t>{nullptr, nullptr, 0});
+}
 
 template <int HD, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k_masked_dkdv(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
     const uint16_t* __restrict__ v, int64_t ldv, const uint16_t* __restrict__ dO, int64_t lddo,
     const float* __restrict__ nl2, const float* __restrict__ delta, uint16_t* __restrict__ dk, int64_t lddk,
-    uint16_t* __restrict__ dv, int64_t lddv, int T, int nkv, int group, ScoreArgs args, MaskTable mask, HeadSplit hs) {
+    uint16_t* __restrict__ dv, int64_t lddv, int T, int nkv, int group, ScoreArgs args, MaskTable mask, HeadSplit hs,
+    int n_split) {
   constexpr int NKS = 2, NT = 256, BQ = 32, NS = HD / 16, ND = HD / 32, TILE = BQ * 2 * HD;
   // Two stages, each the Q tile and then the dO tile: a role picks by offset within the
   // stage's array, so the compiler knows which array a read touches.
@@ -426,9 +450,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool role_a = wave < NKS;
   const int sub = role_a ? wave : wave - NKS;
-  const XcdOrder ord = masked_order();
-  const int kvh = ord.y / hs.n, split = ord.y - kvh * hs.n;
-  const int gs = group / hs.n, h0 = kvh * group + split * gs;
+  const int parts = dkdv_split(mask, T, hs, n_split);
+  const XcdOrder ord = masked_order(nkv * parts);
+  if (ord.y == nkv * parts) return;  // (the last of the grid: among the others they would take every other CU)
+  const int kvh = ord.y / parts, split = ord.y - kvh * parts;
+  const int gs = group / parts, h0 = kvh * group + split * gs;
   const int k0 = (mask.order_k64 != nullptr ? mask.order_k64[ord.rank] : ord.rank) * kSplitKeys, kw = k0 + sub * 32, ki = kw + l32;
   const int tiles = (T + kMaskRows - 1) / kMaskRows;
   const int4 all = mask_bounds<kSplitKeys / kMaskRows>(mask.queries, k0 / kMaskRows, tiles);
@@ -559,7 +585,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
     for (int dt = 0; dt < ND; ++dt) acc[dt] = zero16();
   }
   if (ki < T) {
-    if (hs.n > 1) {
+    if (parts > 1) {
       store_rows_T_f32<HD>(hs.row(split, role_a ? 1 : 0, T, ki, nkv, kvh, HD), acc, hl);
     } else {
       uint16_t* row = role_a ? dv + static_cast<int64_t>(ki) * lddv : dk + static_cast<int64_t>(ki) * lddk;
@@ -571,20 +597,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
 }  // namespace
 
 // Workgroups that a kv head's query heads are split over: the smallest divisor of the
-// group that gives every CU a workgroup (two at head_dim 128), whose fp32 sums a second
-// kernel then adds.  Only the sums' bytes limit it: 64 MB.
+// group that gives every CU a workgroup (at head_dim 128 four, of which three run at once, and
+// eight in long rows: dkdv_split), whose fp32 sums a second kernel then adds.  Only the sums'
+// bytes limit it: 64 MB, 256 at 128.  head_dim 128, four a CU instead of two: 4096 tokens, 32/8
+// heads, 844 -> 631 us for the backward, 8192 of 32/4 3343 -> 2313, in documents of 600 191 -> 166
+// and 369 -> 296.  Up to 64 more than one loses: 16384 tokens, 32/4 heads, documents of 600 308 -> 332.
 MaskedWorkspace masked_workspace(fh_dtype dt, int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim) {
   MaskedWorkspace w{};
-  w.split = 1;
+  w.split = w.long_split = 1;
   w.parts = (2 * tokens * n_heads + 3) / 4 * 4;
   w.total = w.parts;
   if (dt != FH_BF16) return w;
   const int64_t keys = head_dim <= 64 ? kFusedKeys : kSplitKeys, group = n_heads / n_kv_heads;
-  const int64_t blocks = (tokens + keys - 1) / keys * n_kv_heads, want = head_dim <= 64 ? 256 : 512;
+  const int64_t blocks = (tokens + keys - 1) / keys * n_kv_heads, want = head_dim <= 64 ? 256 : 1024;
+  const int64_t most = int64_t(head_dim <= 64 ? 16 : 64) << 20;
   const int64_t part = 2 * tokens * n_kv_heads * head_dim;
-  for (int64_t d = 2; d <= group && blocks * w.split < want; ++d)
-    if (group % d == 0 && d * part <= int64_t(16) << 20) w.split = static_cast<int>(d);
-  if (w.split > 1) w.total += w.split * part;
+  auto split = [&](int64_t wanted) {
+    int s = 1;
+    for (int64_t d = 2; d <= group && blocks * s < wanted; ++d)
+      if (group % d == 0 && d * part <= most) s = static_cast<int>(d);
+    return s;
+  };
+  w.split = split(want);
+  w.long_split = head_dim <= 64 || tokens < kLongRows ? w.split : split(2 * want);
+  if (w.long_split > 1) w.total += w.long_split * part;
   return w;
 }
 
@@ -594,7 +630,7 @@ void masked_bwd_bf16(const MaskedBwd& c, const MaskedArgs& a, hipStream_t stream
   float* nl2 = delta + a.tokens * a.n_heads;
   const int T = static_cast<int>(a.tokens), nkv = static_cast<int>(a.n_kv_heads);
   const int group = static_cast<int>(a.n_heads / a.n_kv_heads);
-  const HeadSplit hs{c.workspace + w.parts, w.split};
+  const HeadSplit hs{c.workspace + w.parts, w.long_split};
   const auto q = static_cast<const uint16_t*>(c.q), k = static_cast<const uint16_t*>(c.k);
   const auto v = static_cast<const uint16_t*>(c.v), g = static_cast<const uint16_t*>(c.dout);
   const auto dk = static_cast<uint16_t*>(c.dk), dv = static_cast<uint16_t*>(c.dv);
@@ -610,12 +646,11 @@ void masked_bwd_bf16(const MaskedBwd& c, const MaskedArgs& a, hipStream_t stream
                          c.lddo, nl2, delta, dk, c.lddk, dv, c.lddv, T, nkv, group, a.score, c.table, hs);
     else
       hipLaunchKernelGGL((k_masked_dkdv<HD, MODE>), grid, dim3(256), 0, stream, q, c.ldq, k, c.ldk, v, c.ldv, g, c.lddo,
-                         nl2, delta, dk, c.lddk, dv, c.lddv, T, nkv, group, a.score, c.table, hs);
+                         nl2, delta, dk, c.lddk, dv, c.lddv, T, nkv, group, a.score, c.table, hs, w.split);
     if (hs.n > 1) {
       const int64_t threads = a.tokens * nkv * (HD / 8);
-      hipLaunchKernelGGL((k_attn_dkdv_sum<HD>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream,
-                         hs, dk, c.lddk, dv, c.lddv, T, a.tokens, nkv, (MODE & kCap ? 4.f : 1.f) * a.score.scale,
-                         RopeRows<uint16_t>{nullptr, nullptr, 0});
+      hipLaunchKernelGGL((k_masked_dkdv_sum<HD>), dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream,
+                         hs, w.split, c.table, dk, c.lddk, dv, c.lddv, T, nkv, (MODE & kCap ? 4.f : 1.f) * a.score.scale);
     }
   });
 }

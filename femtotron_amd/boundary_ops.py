@@ -145,13 +145,23 @@ def fuse_boundary_ops(model: nn.Module, *, embedding_factor: float = 1.0) -> int
     Embeddings with max_norm, sparse gradients or scale_grad_by_freq are left
     alone, and so is a norm already wrapped for activation checkpointing (the
     checkpoint path fuses it).  ``embedding_factor``: what the swapped embeddings' rows are
-    multiplied by.  Returns the number of modules swapped."""
+    multiplied by; refused where an embedding would be left without it.  Returns the number of
+    modules swapped."""
     from transformers.models.llama.modeling_llama import LlamaRMSNorm
+
+    def swapped(emb) -> bool:
+        return type(emb) is nn.Embedding and emb.max_norm is None and not emb.sparse and not emb.scale_grad_by_freq
+
+    if embedding_factor != 1.0:
+        for m in model.modules():
+            emb = getattr(m, "embed_tokens", None)
+            if isinstance(emb, nn.Module) and not swapped(emb) \
+                    and not (isinstance(emb, FusedEmbedding) and emb.factor == embedding_factor):
+                raise ValueError(f"fuse_boundary_ops: embed_tokens, {emb}, cannot have the factor {embedding_factor}")
     n = 0
     for owner in list(model.modules()):
         emb = getattr(owner, "embed_tokens", None)
-        if type(emb) is nn.Embedding and emb.max_norm is None and not emb.sparse \
-                and not emb.scale_grad_by_freq:
+        if swapped(emb):
             owner.embed_tokens = FusedEmbedding.from_module(emb, embedding_factor)
             n += 1
         norm = getattr(owner, "norm", None)

@@ -255,6 +255,21 @@ def test_an_embeddings_padding_idx_is_an_id(padding_idx):
         embedding(torch.tensor([3]), torch.zeros(10, 16), padding_idx=padding_idx)
 
 
+def test_no_embedding_is_left_without_the_factor():
+    """An embedding that is not swapped, or has another factor already, would answer unscaled."""
+    from femtotron_amd.boundary_ops import FusedEmbedding, fuse_boundary_ops
+    for emb in (torch.nn.Embedding(10, 16, max_norm=1.0), torch.nn.Embedding(10, 16, sparse=True),
+                FusedEmbedding(torch.nn.Parameter(torch.zeros(10, 16))), torch.nn.Identity()):
+        model = torch.nn.Module()
+        model.embed_tokens = emb
+        with pytest.raises(ValueError, match="factor"):
+            fuse_boundary_ops(model, embedding_factor=4.0)
+        assert model.embed_tokens is emb and fuse_boundary_ops(model) == 0
+    model.embed_tokens = torch.nn.Embedding(10, 16)
+    assert fuse_boundary_ops(model, embedding_factor=4.0) == 1 and model.embed_tokens.factor == 4.0
+    assert fuse_boundary_ops(model, embedding_factor=4.0) == 0  # as it is
+
+
 # --------------------------------------------------------------------- the oracle
 def test_the_oracle_is_softmax_attention():
     """Against torch's own fp64 attention and its gradients, where the mask is one that it has."""

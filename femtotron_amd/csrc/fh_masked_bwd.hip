@@ -403,8 +403,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
 
 // head_dim 128: 4 waves, 64 keys; each 32 keys are shared by a wave that holds K and sums
 // dV (role A: S, P, handed over through LDS) and one that holds V and sums dK (role B).
-// 1350-1450 us at 8192 tokens, 32/8 heads of 128, capped: the matrix units are busy a third of it
-// and the vector units 40%, the rest are the roles' waits for one another.  (The
+// 1400-1520 us at 8192 tokens, 32/8 heads of 128, capped: the matrix units are busy 35% of it
+// and the vector units 46%, the rest are the roles' waits for one another.  (The
 // roles of a workgroup's waves swapped in every other one, so that each SIMD has both: 2631
 // -> 2644 us for the backward.)
 constexpr int kSplitKeys = 64;

@@ -263,18 +263,44 @@ __device__ __forceinline__ void masked_dkdv_item(const char* Q, const char* G, c
   }
 }
 
+// Workgroups that a kv head's query heads are split over: `split`, or hs.n where the block
+// that is seen by most is seen by about kLongRows rows or more (in the order's buckets, so that it
+// does not hang on which of a bucket comes first).  The workgroups of long rows are few and of
+// unlike length, and the last of them leave a CU to themselves; the sums of the parts cost the same
+// in short ones, where nothing is gained.  The backward with twice the parts, 8192 tokens, 32/8
+// heads of 128: one document 2303 -> 2155 us, documents of 600 283 -> 316; with up to four times
+// the parts, 32/4 heads of 64: one document 1835 -> 1226 (4096 tokens 490 -> 365).
+constexpr int kLongRows = 4096;
+constexpr int kFusedKeys = 128, kSplitKeys = 64;  // of a workgroup, up to head_dim 64 and at 128
+template <int HD>
+__device__ __forceinline__ int dkdv_split(const MaskTable& mask, int T, const HeadSplit& hs, int split) {
+  const int* order = HD <= 64 ? mask.order_k128 : mask.order_k64;
+  if (split == hs.n || order == nullptr) return split;
+  constexpr int TILES = (HD <= 64 ? kFusedKeys : kSplitKeys) / kMaskRows;
+  const int4 most = mask_bounds<TILES>(mask.queries, order[0] * TILES, (T + kMaskRows - 1) / kMaskRows);
+  const int unit = order_unit(T);
+  return most.y > most.x && (most.y - most.x + unit - 1) / unit * unit >= kLongRows ? hs.n : split;
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void k_masked_dkdv_sum(HeadSplit hs, int split, MaskTable mask, uint16_t* __restrict__ dk,
+                                                         int64_t lddk, uint16_t* __restrict__ dv, int64_t lddv, int T,
+                                                         int nkv, float scale) {
+  hs.n = dkdv_split<HD>(mask, T, hs, split);
+  if (hs.n > 1) attn_dkdv_sum<HD>(hs, dk, lddk, dv, lddv, T, T, nkv, scale, RopeRows<uint16_t>{nullptr, nullptr, 0});
+}
+
 // Up to head_dim 64: 8 waves, 128 keys; wave w holds K and V of keys 32 (w % 4) .. +31 in
 // registers and takes queries 32 (w / 4) .. +31 of each 64-query item; the halves' sums
 // meet in LDS at the end, in a fixed order.  Two items a stage, two stages.  190-199 us at
 // 16384 tokens, 32/4 heads of 64, documents of about 600.
-constexpr int kFusedKeys = 128;
-
 template <int HD, int MODE>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k_masked_dkdv_fused(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
     const uint16_t* __restrict__ v, int64_t ldv, const uint16_t* __restrict__ dO, int64_t lddo,
     const float* __restrict__ nl2, const float* __restrict__ delta, uint16_t* __restrict__ dk, int64_t lddk,
-    uint16_t* __restrict__ dv, int64_t lddv, int T, int nkv, int group, ScoreArgs args, MaskTable mask, HeadSplit hs) {
+    uint16_t* __restrict__ dv, int64_t lddv, int T, int nkv, int group, ScoreArgs args, MaskTable mask, HeadSplit hs,
+    int n_split) {
   constexpr int NWH = 4, NT = 512, BQ = 64, NS = HD / 16, ND = HD / 32, TILE = BQ * 2 * HD;
   // The tiles first, below 64 KB: their bases are the reads' immediate offsets.
   struct Lds {
@@ -288,9 +314,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
   const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = wave / NWH, wq = wave % NWH;
-  const XcdOrder ord = masked_order();
-  const int kvh = ord.y / hs.n, split = ord.y - kvh * hs.n;
-  const int gs = group / hs.n;  // query heads of this workgroup
+  const int parts = dkdv_split<HD>(mask, T, hs, n_split);
+  const XcdOrder ord = masked_order(nkv * parts);
+  if (ord.y == nkv * parts) return;  // (as below)
+  const int kvh = ord.y / parts, split = ord.y - kvh * parts;
+  const int gs = group / parts;  // query heads of this workgroup
   const int h0 = kvh * group + split * gs;
   const int k0 = (mask.order_k128 != nullptr ? mask.order_k128[ord.rank] : ord.rank) * kFusedKeys, kw = k0 + wq * 32, ki = kw + l32;
   const int tiles = (T + kMaskRows - 1) / kMaskRows;
@@ -392,7 +420,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
       sum[dt][j] = !some ? 0.f : half == 0 ? dkacc[dt][j] + b : b + dvacc[dt][j];
     }
   if (ki < T) {
-    if (hs.n > 1) {
+    if (parts > 1) {
       store_rows_T_f32<HD>(hs.row(split, half, T, ki, nkv, kvh, HD), sum, hl);
     } else {
       uint16_t* row = half == 0 ? dk + static_cast<int64_t>(ki) * lddk : dv + static_cast<int64_t>(ki) * lddv;
@@ -407,31 +435,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
 // and the vector units 46%, the rest are the roles' waits for one another.  (The
 // roles of a workgroup's waves swapped in every other one, so that each SIMD has both: 2631
 // -> 2644 us for the backward.)
-constexpr int kSplitKeys = 64;
-
-// Workgroups that a kv head's query heads are split over: `split`, or hs.n where the block
-// that is seen by most is seen by about kLongRows rows or more (in the order's buckets, so that it
-// does not hang on which of a bucket comes first).  The workgroups of long rows are few and of
-// unlike length, and the last of them leave a CU to themselves; the sums of the parts cost the same
-// in short ones, where nothing is gained.  The backward with twice the parts, 8192 tokens, 32/8
-// heads: one document 2303 -> 2155 us, documents of 600 283 -> 316.
-constexpr int kLongRows = 4096;
-__device__ __forceinline__ int dkdv_split(const MaskTable& mask, int T, const HeadSplit& hs, int split) {
-  if (split == hs.n || mask.order_k64 == nullptr) return split;
-  const int4 most = mask_bounds<kSplitKeys / kMaskRows>(mask.queries, mask.order_k64[0] * (kSplitKeys / kMaskRows),
-                                                        (T + kMaskRows - 1) / kMaskRows);
-  const int unit = order_unit(T);
-  return most.y > most.x && (most.y - most.x + unit - 1) / unit * unit >= kLongRows ? hs.n : split;
-}
-
-template <int HD>
-__global__ __launch_bounds__(256) void k_masked_dkdv_sum(HeadSplit hs, int split, MaskTable mask, uint16_t* __restrict__ dk,
-                                                         int64_t lddk, uint16_t* __restrict__ dv, int64_t lddv, int T,
-                                                         int nkv, float scale) {
-  hs.n = dkdv_split(mask, T, hs, split);
-  if (hs.n > 1) attn_dkdv_sum<HD>(hs, dk, lddk, dv, lddv, T, T, nkv, scale, RopeRows<uint16_t>{nullptr, nullptr, 0});
-}
-
 template <int HD, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k_masked_dkdv(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool role_a = wave < NKS;
   const int sub = role_a ? wave : wave - NKS;
-  const int parts = dkdv_split(mask, T, hs, n_split);
+  const int parts = dkdv_split<HD>(mask, T, hs, n_split);
   const XcdOrder ord = masked_order(nkv * parts);
   if (ord.y == nkv * parts) return;  // (the last of the grid: among the others they would take every other CU)
   const int kvh = ord.y / parts, split = ord.y - kvh * parts;
@@ -597,11 +600,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3))) void k
 }  // namespace
 
 // Workgroups that a kv head's query heads are split over: the smallest divisor of the
-// group that gives every CU a workgroup (at head_dim 128 four, of which three run at once, and
-// eight in long rows: dkdv_split), whose fp32 sums a second kernel then adds.  Only the sums'
-// bytes limit it: 64 MB, 256 at 128.  head_dim 128, four a CU instead of two: 4096 tokens, 32/8
+// group that gives every CU one workgroup (at head_dim 128 four, of which three run at once), and
+// in long rows four (eight): dkdv_split.  A second kernel then adds their fp32 sums, whose
+// bytes alone limit it: 256 MB.  head_dim 128, four a CU instead of two: 4096 tokens, 32/8
 // heads, 844 -> 631 us for the backward, 8192 of 32/4 3343 -> 2313, in documents of 600 191 -> 166
-// and 369 -> 296.  Up to 64 more than one loses: 16384 tokens, 32/4 heads, documents of 600 308 -> 332.
+// and 369 -> 296.  Up to 64 more than one loses in short rows: 16384 tokens, 32/4 heads of 64,
+// documents of 600 308 -> 332.
 MaskedWorkspace masked_workspace(fh_dtype dt, int64_t tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim) {
   MaskedWorkspace w{};
   w.split = w.long_split = 1;
@@ -610,7 +614,7 @@ MaskedWorkspace masked_workspace(fh_dtype dt, int64_t tokens, int64_t n_heads, i
   if (dt != FH_BF16) return w;
   const int64_t keys = head_dim <= 64 ? kFusedKeys : kSplitKeys, group = n_heads / n_kv_heads;
   const int64_t blocks = (tokens + keys - 1) / keys * n_kv_heads, want = head_dim <= 64 ? 256 : 1024;
-  const int64_t most = int64_t(head_dim <= 64 ? 16 : 64) << 20;
+  const int64_t most = int64_t(64) << 20;
   const int64_t part = 2 * tokens * n_kv_heads * head_dim;
   auto split = [&](int64_t wanted) {
     int s = 1;
@@ -619,7 +623,7 @@ MaskedWorkspace masked_workspace(fh_dtype dt, int64_t tokens, int64_t n_heads, i
     return s;
   };
   w.split = split(want);
-  w.long_split = head_dim <= 64 || tokens < kLongRows ? w.split : split(2 * want);
+  w.long_split = tokens < kLongRows ? w.split : split(head_dim <= 64 ? 4 * want : 2 * want);
   if (w.long_split > 1) w.total += w.long_split * part;
   return w;
 }
@@ -643,7 +647,7 @@ void masked_bwd_bf16(const MaskedBwd& c, const MaskedArgs& a, hipStream_t stream
     const dim3 grid(static_cast<unsigned>((a.tokens + keys - 1) / keys), static_cast<unsigned>(nkv * hs.n));
     if constexpr (HD <= 64)
       hipLaunchKernelGGL((k_masked_dkdv_fused<HD, MODE>), grid, dim3(512), 0, stream, q, c.ldq, k, c.ldk, v, c.ldv, g,
-                         c.lddo, nl2, delta, dk, c.lddk, dv, c.lddv, T, nkv, group, a.score, c.table, hs);
+                         c.lddo, nl2, delta, dk, c.lddk, dv, c.lddv, T, nkv, group, a.score, c.table, hs, w.split);
     else
       hipLaunchKernelGGL((k_masked_dkdv<HD, MODE>), grid, dim3(256), 0, stream, q, c.ldq, k, c.ldk, v, c.ldv, g, c.lddo,
                          nl2, delta, dk, c.lddk, dv, c.lddv, T, nkv, group, a.score, c.table, hs, w.split);

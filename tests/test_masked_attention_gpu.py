@@ -126,11 +126,11 @@ def test_a_long_row_in_every_kernel():
         _compare(1, 2100, dict(starts=starts), nh, nkv, hd, BF, seed=40)
 
 
-@pytest.mark.parametrize("nh,nkv", [(32, 16), (32, 8)])
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 16, 128), (32, 8, 128), (16, 2, 64), (9, 3, 32)])
 @pytest.mark.parametrize("starts", [[0], [0, 1000, 1600, 1700, 3333]])
-def test_sums_in_parts_of_heads_by_what_the_mask_holds(starts, nh, nkv):
+def test_sums_in_parts_of_heads_by_what_the_mask_holds(starts, nh, nkv, hd):
     """Enough keys that a kv head's sums come in more parts of its heads where a row is long."""
-    _compare(1, 4160, dict(starts=starts), nh, nkv, 128, BF, seed=41, cap=30.0)
+    _compare(1, 4160, dict(starts=starts), nh, nkv, hd, BF, seed=41, cap=30.0)
 
 
 def test_the_gradient_by_differences():

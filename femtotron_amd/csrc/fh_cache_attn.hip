@@ -181,9 +181,10 @@ __device__ __forceinline__ void cache_segment(const CacheArgs& c, char* lds, flo
   const int kvh = blockIdx.y, tile = blockIdx.z;
   const Column col = column_of(c, kvh, tile, l32);
   const int p = seq_end - c.n_new + col.u;  // the column's place
-  const int sees = col.real && c.window > 0 ? max(0, p + 1 - c.window) : 0;
-  const int past = col.real ? min(p + 1, end) : 0;
-  const bool some = col.real && p >= 0;
+  // It sees places sees <= t < past of the part, which may be none where the sequence has some.
+  const int sees = max(begin, c.window > 0 ? p + 1 - c.window : 0);
+  const int past = col.real ? min(p + 1, end) : begin;
+  const bool here = sees < past, some = col.real && p >= 0;
   // Every new token sees places [last_first, first_end).
   const int first_end = min(seq_end - c.n_new + 1, end), last_first = c.window > 0 ? max(0, seq_end - c.window) : 0;
   const float a = (MODE & kCap) ? c.score.in2 : c.score.scale_log2;
@@ -238,7 +239,7 @@ __device__ __forceinline__ void cache_segment(const CacheArgs& c, char* lds, flo
     }
   };
   run(std::false_type{});
-  if (__builtin_expect(wave_any(sees < past && not_finite<ND>(oacc)), 0)) {
+  if (__builtin_expect(wave_any(here && not_finite<ND>(oacc)), 0)) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     run(std::true_type{});
   }
@@ -261,7 +262,7 @@ __device__ __forceinline__ void cache_segment(const CacheArgs& c, char* lds, flo
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) red[wave][dt * 16 + j][lane] = oacc[dt][j] * alpha;
+    for (int j = 0; j < 16; ++j) red[wave][dt * 16 + j][lane] = here ? oacc[dt][j] * alpha : 0.f;  // (0 * inf is a NaN)
   __syncthreads();
   // The waves share the ND * 16 entries out, four dims at a time.
   const int64_t item = (static_cast<int64_t>(slot) * c.nkv + kvh) * gridDim.z + tile;

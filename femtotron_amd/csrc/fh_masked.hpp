@@ -127,12 +127,14 @@ struct Score {
     if constexpr (MODE & kCap) return fmaf(c, half_sigmoid(x), low);
     return fmaf(x, a, low);
   }
-  // e^(z - lse) with nl = b - lse * log2(e), and under a cap a quarter of the score's derivative.
+  // e^(z - lse) with nl = b - lse * log2(e), and under a cap a quarter of the score's derivative,
+  // 0 for a score that is NaN (the weight is NaN then, and 0 where the score is not seen: 0 times
+  // this stays 0).  The bounds are a modifier of the fma.
   __device__ __forceinline__ float weight(float x, float away, float nl, float& quarter) const {
     const float low = (MODE & kBias) ? fmaf(-slope, fabsf(away), nl) : nl;
     if constexpr (MODE & kCap) {
       const float r = half_sigmoid(x);
-      quarter = fmaf(-r, r, r);
+      quarter = __builtin_amdgcn_fmed3f(fmaf(-r, r, r), 0.f, 1.f);
       return fast_exp2(fmaf(c, r, low));
     } else {
       quarter = 1.f;

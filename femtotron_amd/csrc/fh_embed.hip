@@ -299,22 +299,20 @@ __global__ __launch_bounds__(kGroupThreads) void k_embed_group(const int64_t* __
 // V = 32000, H = 2048, whose bytes take 38 us.  So the grid's first workgroups
 // take the rows of kHotTokens and more: a wave sums 128 columns of such a row
 // (2 per lane) with the rows of up to kHotDepth tokens in flight, the additions
-// still one after the other in token order: 54-56 us there.  (One wave per row and
+// still one after the other in token order: 58-62 us there.  (One wave per row and
 // 1024 threads per workgroup, the tokens read as scalars: 132 us.)
 //
 // A hot workgroup looks through hot_ids consecutive ids and sums its frequent ones
-// one after the other: 256 of them where the vocabulary gives workgroups enough, as
+// one after the other: 64 of them where the vocabulary gives workgroups enough, as
 // few of whose ids are frequent, fewer (down to one) in a small vocabulary, whose
 // ids may all be: fh_embedding_bwd halves them until there are kHotWaves waves.
-// With 64 for any vocabulary, uniform ids of a small vocabulary were 32 waves' work at
+// With 64 throughout, uniform ids of a small vocabulary were 32 waves' work at
 // V = 1024, H = 256 (16384 tokens: 91 us, now 17; one wave per row 40) and 64 at
 // V = 64, H = 2048 (4096 tokens: 203 us, now 11; one wave per row 64).
 constexpr int kRowChunks = 4;
 constexpr int kHotTokens = 8;
 constexpr int kHotCols = 2 * kWave;  // columns that a wave sums of a hot row
 constexpr int64_t kHotWaves = 4096;  // 16 per CU
-constexpr int64_t kMostHotIds = 256;
-constexpr int64_t kRowWaves = 8192;  // 32 per CU
 template <typename T>
 constexpr int kHotDepth = sizeof(T) == 2 ? 64 : 32;
 
@@ -373,13 +371,9 @@ __device__ __forceinline__ void hot_columns(const T* __restrict__ dy, const uint
   else *reinterpret_cast<float2*>(dst + c) = make_float2(a0, a1);
 }
 
-// Workgroups [0, hot_blocks): hot_blocks / hot_parts groups of hot_ids ids, and for each
-// group hot_parts workgroups of kRowsPerBlock column slices; then up to 64 rows a wave,
-// whose ranges it loads at once (in a large vocabulary most rows have no token, and a wave
-// for each of them waits for its range to write one row of zeros), dealt out in turn, so
-// that what is written at one time lies together.  V = 128256, H = 4096, 8192 tokens: a wave
-// a row 221-228 us for the kernel, runs of rows 232, rows in turn 220-231; V = 32000, H =
-// 2048, 16384 tokens 58-61 us and, in turn, 54-56.
+// Workgroups [0, hot_blocks): hot_blocks / hot_parts groups of hot_ids (at most 64)
+// ids, and for each group hot_parts workgroups of kRowsPerBlock column slices; then
+// one wave per row.
 template <typename T>
 __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const T* __restrict__ dy,
                                                             const uint32_t* __restrict__ tok,
@@ -395,63 +389,48 @@ __global__ __launch_bounds__(kEmbThreads) void k_embed_rows(const T* __restrict_
     const int64_t v0 = static_cast<int64_t>(block / hot_parts) * hot_ids;
     const int64_t c0 = static_cast<int64_t>(block % hot_parts * kRowsPerBlock + wave) * kHotCols;
     if (c0 >= hidden) return;
-    for (int g = 0; g < hot_ids; g += kWave) {
-      uint32_t lo = 0, len = 0;
-      if (g + lane < hot_ids && v0 + g + lane < vocab) {
-        lo = seg_start[v0 + g + lane];
-        len = seg_end[v0 + g + lane] - lo;
-      }
-      for (uint64_t hot = __ballot(len >= kHotTokens); hot != 0; hot &= hot - 1) {
-        const int l = __builtin_ctzll(hot);
-        hot_columns<T>(dy, tok + __builtin_amdgcn_readlane(lo, l), __builtin_amdgcn_readlane(len, l),
-                       dw + (v0 + g + l) * hidden, c0 + 2 * lane, hidden, lane, factor);
-      }
+    uint32_t lo = 0, len = 0;
+    if (lane < hot_ids && v0 + lane < vocab) {
+      lo = seg_start[v0 + lane];
+      len = seg_end[v0 + lane] - lo;
+    }
+    for (uint64_t hot = __ballot(len >= kHotTokens); hot != 0; hot &= hot - 1) {
+      const int l = __builtin_ctzll(hot);
+      hot_columns<T>(dy, tok + __builtin_amdgcn_readlane(lo, l), __builtin_amdgcn_readlane(len, l),
+                     dw + (v0 + l) * hidden, c0 + 2 * lane, hidden, lane, factor);
     }
     return;
   }
-  const int64_t first = static_cast<int64_t>(block - hot_blocks) * kRowsPerBlock + wave;
-  const int64_t step = static_cast<int64_t>(gridDim.x - hot_blocks) * kRowsPerBlock;
-  uint32_t los = 0, his = 0;  // of rows first + lane * step
-  const int64_t mine = first + lane * step;
-  if (mine < vocab) {
-    los = seg_start[mine];
-    his = seg_end[mine];
-  }
-  for (int r = 0; first + r * step < vocab; ++r) {
-    const uint32_t lo = __builtin_amdgcn_readlane(los, r), hi = __builtin_amdgcn_readlane(his, r);
-    if (hi - lo >= kHotTokens) continue;
-    T* dst = dw + (first + r * step) * hidden;
-    if (lo == hi) {
-      const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int64_t c = lane * 8; c < hidden; c += kWave * 8) Elem<T>::store8(dst + c, z);
-      continue;
-    }
-    for (int64_t c0 = lane * 8; c0 < hidden; c0 += kRowChunks * kWave * 8) {
-      float acc[kRowChunks][8];
+  const int64_t v = static_cast<int64_t>(block - hot_blocks) * kRowsPerBlock + wave;
+  if (v >= vocab) return;
+  const uint32_t lo = seg_start[v], hi = seg_end[v];
+  if (hi - lo >= kHotTokens) return;
+  T* dst = dw + v * hidden;
+  for (int64_t c0 = lane * 8; c0 < hidden; c0 += kRowChunks * kWave * 8) {
+    float acc[kRowChunks][8];
+#pragma unroll
+    for (int k = 0; k < kRowChunks; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[k][e] = 0.f;
+    for (uint32_t j = lo; j < hi; ++j) {
+      const T* src = dy + static_cast<int64_t>(tok[j]) * hidden + c0;
+      float g[kRowChunks][8];
 #pragma unroll
       for (int k = 0; k < kRowChunks; ++k)
+        if (c0 + k * kWave * 8 < hidden) Elem<T>::load8(src + k * kWave * 8, g[k]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[k][e] = 0.f;
-      for (uint32_t j = lo; j < hi; ++j) {
-        const T* src = dy + static_cast<int64_t>(tok[j]) * hidden + c0;
-        float g[kRowChunks][8];
+      for (int k = 0; k < kRowChunks; ++k)
+        if (c0 + k * kWave * 8 < hidden)
 #pragma unroll
-        for (int k = 0; k < kRowChunks; ++k)
-          if (c0 + k * kWave * 8 < hidden) Elem<T>::load8(src + k * kWave * 8, g[k]);
+          for (int e = 0; e < 8; ++e) acc[k][e] += g[k][e];
+    }
 #pragma unroll
-        for (int k = 0; k < kRowChunks; ++k)
-          if (c0 + k * kWave * 8 < hidden)
+    for (int k = 0; k < kRowChunks; ++k)
+      if (c0 + k * kWave * 8 < hidden) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[k][e] += g[k][e];
+        for (int e = 0; e < 8; ++e) acc[k][e] *= factor;
+        Elem<T>::store8(dst + c0 + k * kWave * 8, acc[k]);
       }
-#pragma unroll
-      for (int k = 0; k < kRowChunks; ++k)
-        if (c0 + k * kWave * 8 < hidden) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[k][e] *= factor;
-          Elem<T>::store8(dst + c0 + k * kWave * 8, acc[k]);
-        }
-    }
   }
 }
 
@@ -582,11 +561,10 @@ int embedding_bwd_impl(fh_dtype dt, const void* dy, const int64_t* ids, void* dw
   }
   // A row of kHotTokens tokens needs that many.
   const int64_t hot_parts = (hidden + kRowsPerBlock * kHotCols - 1) / (kRowsPerBlock * kHotCols);
-  int64_t hot_ids = kMostHotIds;
+  int64_t hot_ids = kWave;
   while (hot_ids > 1 && (vocab + hot_ids - 1) / hot_ids * hot_parts * kRowsPerBlock < kHotWaves) hot_ids /= 2;
   const int64_t hot_blocks = n_tokens >= kHotTokens ? (vocab + hot_ids - 1) / hot_ids * hot_parts : 0;
-  const int64_t wave_rows = vocab / kRowWaves < 1 ? 1 : vocab / kRowWaves < kWave ? vocab / kRowWaves : kWave;
-  const int64_t blocks = hot_blocks + (vocab + kRowsPerBlock * wave_rows - 1) / (kRowsPerBlock * wave_rows);
+  const int64_t blocks = hot_blocks + (vocab + kRowsPerBlock - 1) / kRowsPerBlock;
   FH_REQUIRE(blocks <= 0x7fffffff, "embedding_bwd: vocab * hidden too large");
   auto rows = [&](auto tag) {
     using T = decltype(tag);

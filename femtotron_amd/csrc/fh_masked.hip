@@ -129,6 +129,9 @@ constexpr float kMostScale = 1152921504606846976.f;  // what scores are made of 
 // tanh as 1 - 2 r is off by 2^-23 of the cap: from here on that would be more in a score than
 // the rounding of a bf16 weight is in its logarithm (2^-9, halved twice).
 constexpr float kMostCap = 4096.f;
+// In fp32 scale / cap is a normal number, so that scores keep their bits, and cap * log2(e) finite.
+constexpr float kMostCapF32 = 8.507059173023462e37f;  // 2^126
+constexpr float kLeastRatioF32 = 1.1754943508222875e-38f;  // 2^-126
 
 int check_tokens(const char* name, int64_t tokens) {
   if (tokens < 0 || tokens > (int64_t(1) << 30)) return fail(FH_ERR_INVALID, std::string(name) + ": tokens must be 0 to 2^30");
@@ -148,6 +151,8 @@ int masked_args(const char* name, fh_dtype dt, int64_t tokens, int64_t n_heads, 
   if (!(scale > 0.f) || !(scale <= kMostScale)) return fail(FH_ERR_INVALID, n + ": scale must be positive, at most 2^60");
   if (!(cap >= 0.f) || !(cap < INFINITY)) return fail(FH_ERR_INVALID, n + ": cap must be 0 (none) or positive and finite");
   if (dt == FH_BF16 && cap > kMostCap) return fail(FH_ERR_INVALID, n + ": cap must be at most 4096 in bf16");
+  if (dt == FH_F32 && cap > 0.f && !(cap <= kMostCapF32 && scale / cap >= kLeastRatioF32))
+    return fail(FH_ERR_INVALID, n + ": cap must be at most 2^126, and 2^126 times the scale, in fp32");
   if (cap > 0.f && !(scale / cap <= kMostScale)) return fail(FH_ERR_INVALID, n + ": cap is too small for the scale");
   a.tokens = tokens;
   a.n_heads = n_heads;

@@ -11,6 +11,7 @@ over the j that token i sees, which ``attention_mask`` says.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -109,10 +110,10 @@ def _score(name: str, head_dim: int, scale: float | None, cap: float | None,
         raise ValueError(f"{name}: scale must be positive, got {scale}")
     if cap is None:
         return scale, 0.0
-    cap = float(cap)
-    if not 0 < cap < math.inf:
-        raise ValueError(f"{name}: cap must be positive, or None, got {cap}")
-    return scale, cap
+    cap32 = ctypes.c_float(cap).value  # the kernels', for which 0 is no cap
+    if not 0 < cap32 < math.inf:
+        raise ValueError(f"{name}: cap must be positive and finite in fp32, or None, got {cap}")
+    return scale, cap32
 
 
 def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: AttentionMask, *, head_dim: int,
@@ -124,7 +125,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     it see; differentiable in q, k and v (once, and in reverse mode).
 
     head_dim 32, 64 or 128; ``scale`` (None: head_dim ** -0.5) on the products; ``cap``: scores
-    become cap * tanh(score / cap) (bf16: a cap of at most 4096); ``slopes`` (fp32, one a
+    become cap * tanh(score / cap) (a cap of at most 2^126 times the scale, in bf16 of at most 4096); ``slopes`` (fp32, one a
     query head): less slopes[h] times the distance, after the cap.  bf16 or fp32 on a HIP
     device.  Nothing that a token does not see reaches it, infinities and NaN included."""
     scale, cap = _score("masked_attention", head_dim, scale, cap, slopes)

@@ -46,8 +46,9 @@ int fh_attn_mask(const int64_t* starts, const int64_t* lengths, const int64_t* p
 /* ------------------------------------------------- attention under a mask
  * For each query head h, which reads kv head h / (n_heads / n_kv_heads):
  *   s_ij = scale q_i . k_j                  (0 < scale <= 2^60)
- *   z_ij = cap tanh(s_ij / cap)             (z = s for cap 0; bf16: cap <= 4096, whose
- *                                            tanh is off by 2^-23)
+ *   z_ij = cap tanh(s_ij / cap)             (z = s for cap 0; scale / cap <= 2^60; bf16: cap
+ *                                            <= 4096, whose tanh is off by 2^-23; fp32: cap <=
+ *                                            2^126 and scale / cap >= 2^-126)
  *          - slopes[h] |i - j|              (without slopes: none)
  *   o_i  = sum_j softmax_j(z_ij) v_j        over the j that i sees; 0 where it sees none
  * Token-major: head h of q, o at columns h * head_dim of its row, row strides in

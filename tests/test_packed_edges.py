@@ -1,0 +1,37 @@
+"""The operators of a step over packed documents at the edges of what they take, without a GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+from tests.test_packed_api import _lib, _mask, no_kernel  # noqa: F401
+
+
+@pytest.mark.parametrize("cap", [1e-50, 1e-46, 1e39, float("inf"), float("nan"), -1e-50])
+def test_a_cap_that_fp32_does_not_hold_is_refused(cap, no_kernel):
+    """One that it rounds to 0 would be none."""
+    from femtotron_amd import cache_attention, masked_attention
+    q, k = torch.randn(4, 128), torch.randn(4, 64)
+    for call in (lambda c: masked_attention(q, k, k, _mask(4), head_dim=64, cap=c),
+                 lambda c: cache_attention(q[:1, None], k[None], k[None], torch.tensor([3]), head_dim=64, cap=c)):
+        call(30.0)
+        call(torch.tensor(30.0))
+        with pytest.raises(ValueError, match="cap"):
+            call(cap)
+
+
+def test_a_cap_that_is_too_large_for_the_scale_is_refused():
+    """cap * log2(e) would overflow, or scale / cap lose its bits."""
+    lib = _lib()
+    L = lib.lib()
+
+    def status(dt, scale, cap):
+        return L.fh_masked_attn_fwd(dt, 16, 64, 16, 64, 16, 64, 16, 64, None, None, 16, 0, 1, 1, 64, scale, cap, None, None)
+
+    for cap in (2.4e38, 2.0 ** 126 * 1.01):
+        assert status(1, 1.0, cap) == 1 and b"cap" in L.fh_last_error()
+    assert status(1, 1e-3, 1e36) == 1 and b"cap" in L.fh_last_error()
+    for dt, scale, cap in ((1, 1.0, 2.0 ** 125), (1, 0.125, 1e6), (1, 2.0 ** -40, 2.0 ** 86), (0, 0.125, 4096.0), (0, 1e-36, 50.0),
+                           (1, 0.125, 0.0)):
+        assert status(dt, scale, cap) == 0, (dt, scale, cap)

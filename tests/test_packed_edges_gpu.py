@@ -1,0 +1,24 @@
+"""The operators of a step over packed documents at the edges of what they take, on the GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.helpers import randn
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def test_large_caps_in_fp32_are_none():
+    """cap tanh(s / cap) is s to s^3 / (3 cap^2), below fp32's rounding from |s| = 2^-12 cap on."""
+    from femtotron_amd import attention_mask, cache_attention, masked_attention
+    q, k, v = (randn((1, 70, 128), i).to(DEV) for i in range(3))
+    mask, lengths = attention_mask(1, 70, device=DEV), torch.tensor([70], device=DEV)
+    plain = masked_attention(q, k, v, mask, head_dim=64)
+    one = cache_attention(q[:, -2:], k, v, lengths, head_dim=64)
+    # fp32 of scores of up to 2^4 (three roundings of each, 2^-20 all told) and of 128 terms' sums
+    bound = 2.0 ** -18 * float(v.abs().max())
+    for cap in (1e6, 1e20, 2.0 ** 122):
+        assert float((masked_attention(q, k, v, mask, head_dim=64, cap=cap) - plain).abs().max()) <= bound
+        assert float((cache_attention(q[:, -2:], k, v, lengths, head_dim=64, cap=cap) - one).abs().max()) <= bound

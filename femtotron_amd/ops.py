@@ -941,6 +941,11 @@ def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, vocab: int, padding_idx: 
 
 
 # ------------------------------------------------------------- gradient norm
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether tensors of one shape lie alike; the stride of a dim of one is anything."""
+    return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n > 1)
+
+
 def clip_grads(grads: list, outs: list | None, max_norm: float) -> torch.Tensor:
     """The 2-norm of all grads (a one-element fp32 tensor) and, with outs, each of them times
     min(1, max_norm / (norm + 1e-6)) (fh_clip_grads).  Tensors are dense, an out of its
@@ -959,7 +964,7 @@ def clip_grads(grads: list, outs: list | None, max_norm: float) -> torch.Tensor:
     if outs is not None and not in_place:
         if [t.shape for t in grads] != [t.shape for t in outs] \
                 or not (all_contiguous or all([a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous())
-                                               for a, b in zip(grads, outs)])):
+                                               or _same_order(a, b) for a, b in zip(grads, outs)])):
             raise ValueError("clip_gradients: an output must have its gradient's shape and strides")
     n = len(grads)
     table = (_lib.FhGrad * n)()

@@ -35,3 +35,14 @@ def test_a_cap_that_is_too_large_for_the_scale_is_refused():
     for dt, scale, cap in ((1, 1.0, 2.0 ** 125), (1, 0.125, 1e6), (1, 2.0 ** -40, 2.0 ** 86), (0, 0.125, 4096.0), (0, 1e-36, 50.0),
                            (1, 0.125, 0.0)):
         assert status(dt, scale, cap) == 0, (dt, scale, cap)
+
+
+def test_outputs_whose_strides_differ_in_dims_of_one(no_kernel):
+    from femtotron_amd.optim import clip_gradients
+    a = torch.randn(20, 30).t()[None]                                # strides (600, 1, 30)
+    b = torch.empty(20, 30).t().as_strided((1, 30, 20), (7, 1, 30))
+    clip_gradients([a, torch.randn(3)], 1.0, out=[b, torch.empty(3)])
+    clip_gradients([b], 1.0, out=[a])
+    assert no_kernel.count("fh_clip_grads") == 2
+    with pytest.raises(ValueError, match="strides"):
+        clip_gradients([a], 1.0, out=[torch.empty(1, 30, 20)])

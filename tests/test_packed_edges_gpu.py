@@ -10,6 +10,17 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
 
+def test_clipping_into_outputs_whose_strides_differ_in_dims_of_one():
+    """The factor rounds once (2^-24), the product once."""
+    from femtotron_amd.optim import clip_gradients
+    a = randn((20, 30), 1).to(DEV).t()[None]
+    b = torch.empty(600, device=DEV).as_strided((1, 30, 20), (7, 1, 30))
+    norm = float(clip_gradients([a], 2.0, out=[b]))
+    want = a.double() * (2.0 / (float(a.double().square().sum().sqrt()) + 1e-6))
+    assert abs(norm - float(a.double().norm())) <= 2.0 ** -23 * norm
+    assert ((b.double() - want).abs() <= 2.0 ** -23 * want.abs()).all()
+
+
 def test_large_caps_in_fp32_are_none():
     """cap tanh(s / cap) is s to s^3 / (3 cap^2), below fp32's rounding from |s| = 2^-12 cap on."""
     from femtotron_amd import attention_mask, cache_attention, masked_attention

@@ -23,6 +23,7 @@ import math
 from typing import Iterable
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from ._lib import FhAdamHyper
@@ -226,8 +227,9 @@ def clip_gradients(grads: Iterable[torch.Tensor], max_norm: float, *,
 
     The reference's ``ClipGradNorm`` (femtotron/training/grad_transform.py:13-63) for programs
     whose optimizer is not ``FusedAdamW`` (which clips by itself).  The sum of squares is fp64
-    in a fixed order.  A norm that is NaN makes every gradient NaN, as torch's has it.  A
-    tensor may not stand in the list twice, nor overlap another."""
+    in a fixed order.  A norm that is NaN makes every gradient NaN, as torch's has it.  As
+    torch's, under no_grad: neither the norm nor the outputs have derivatives.  A tensor may not
+    stand in the list twice, nor overlap another."""
     grads = list(grads)
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
@@ -252,6 +254,10 @@ def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm:
 
 
 def gradient_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
-    """The joint 2-norm of ``grads``, a device scalar, in one pass over them."""
+    """The joint 2-norm of ``grads``, a device scalar, in one pass over them.  Without derivatives:
+    refused where one is asked for."""
     grads = list(grads)
+    if (torch.is_grad_enabled() and any([g.requires_grad for g in grads])) or \
+            (forward_ad._current_level >= 0 and any([ops.wants_derivative(g) for g in grads])):
+        raise TypeError("gradient_norm has no derivatives, and a tensor wants one (use it under torch.no_grad())")
     return ops.clip_grads(grads, None, 0.0) if grads else torch.zeros(())

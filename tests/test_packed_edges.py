@@ -46,3 +46,21 @@ def test_outputs_whose_strides_differ_in_dims_of_one(no_kernel):
     assert no_kernel.count("fh_clip_grads") == 2
     with pytest.raises(ValueError, match="strides"):
         clip_gradients([a], 1.0, out=[torch.empty(1, 30, 20)])
+
+
+def test_a_norm_that_is_to_be_differentiated_is_refused(no_kernel):
+    from femtotron_amd.optim import clip_grad_norm_, gradient_norm
+    p = torch.nn.Parameter(torch.ones(5))
+    g, = torch.autograd.grad((p ** 3).sum(), p, create_graph=True)
+    with pytest.raises(TypeError, match="derivative"):
+        gradient_norm([g.detach(), g])
+    with torch.no_grad():
+        gradient_norm([g])
+    gradient_norm([g.detach()])
+    with fwd.dual_level():
+        gradient_norm([g.detach()])
+        with pytest.raises(TypeError, match="derivative"):
+            gradient_norm([fwd.make_dual(g.detach(), torch.ones(5))])
+    p.grad = g.detach().clone()
+    clip_grad_norm_([p], 1.0)
+    assert no_kernel.count("fh_clip_grads") == 4

@@ -691,12 +691,12 @@ def attn_mask(tokens: int, seq_len: int, starts: torch.Tensor | None, lengths: t
     (int64, ascending) of lengths (None: up to the next), or, starts None, one for each
     seq_len rows; window 0: none."""
     dev = device.index if device.index is not None else torch.cuda.current_device()
-    n = tokens // max(seq_len, 1) if starts is None else starts.numel()
+    n = starts.numel() if starts is not None else tokens // seq_len if seq_len else 0
     if starts is not None:
         _int64_vector("attention_mask: starts", starts, None, dev)
     for t, name in ((lengths, "lengths"), (prefix, "prefix")):
-        if t is not None:
-            _int64_vector("attention_mask: " + name, t, n, dev)
+        if t is not None:  # (rows of no tokens are as many as they are)
+            _int64_vector("attention_mask: " + name, t, n if starts is not None or seq_len else None, dev)
     nbytes = _lib.lib().fh_attn_mask_size(tokens)
     table = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _launch("fh_attn_mask", table, _ptr(starts), _ptr(lengths), _ptr(prefix), n, tokens, seq_len, window, int(causal),

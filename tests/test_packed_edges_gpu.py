@@ -10,6 +10,18 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
 
+def test_rows_of_no_tokens_have_lengths():
+    from femtotron_amd import attention_mask, masked_attention
+    zeros = torch.zeros(3, dtype=torch.int64, device=DEV)
+    for mask in (attention_mask(3, 0, lengths=zeros), attention_mask(3, 0, lengths=zeros, prefix=zeros), attention_mask(3, 0, zeros, zeros)):
+        x = torch.empty(3, 0, 128, dtype=torch.bfloat16, device=DEV)
+        assert masked_attention(x, x, x, mask, head_dim=64).shape == x.shape
+    with pytest.raises(ValueError, match="3"):
+        attention_mask(3, 2, lengths=zeros[:2])
+    with pytest.raises(ValueError, match="2"):
+        attention_mask(0, 2, zeros[:2], zeros)
+
+
 def test_clipping_into_outputs_whose_strides_differ_in_dims_of_one():
     """The factor rounds once (2^-24), the product once."""
     from femtotron_amd.optim import clip_gradients

@@ -88,3 +88,17 @@ def test_a_later_key_of_the_own_document(score, hd, dtype):
         assert torch.isfinite(a).all(), name
         assert float((a - b).abs().max()) <= torch.finfo(dtype).eps * 4 * float(b.abs().max()), name
         assert got[name][at:].isnan().all(), name
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 4, 64), (32, 8, 32), (32, 8, 128)])
+@pytest.mark.parametrize("score", [dict(), dict(cap=20.0)], ids=str)
+@pytest.mark.parametrize("spoil", SPOILT, ids=str)
+def test_in_rows_of_every_kernel(spoil, score, nh, nkv, hd):
+    """Blocks in the order of their work, pairs of heads, sums in parts of heads."""
+    _unseen(2200, [0, 700, 1100, 1500], [700, 400, 370, 500], nh, nkv, hd, BF, 90, bad_document=1, spoil=spoil, **score)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(16, 2, 64), (16, 2, 128)])
+@pytest.mark.parametrize("score", [dict(), dict(cap=20.0)], ids=str)
+def test_beside_a_row_long_enough_for_more_parts(score, nh, nkv, hd):
+    _unseen(4600, [0, 4200], [4200, 300], nh, nkv, hd, BF, 100, bad_document=1, spoil=dict(q=NAN, k=-INF, v=INF, do=NAN), **score)

@@ -544,14 +544,17 @@ __global__ __launch_bounds__(256) void k_cache_attn_f32(CacheArgs c) {
 int64_t workgroups(int64_t head_dim) { return head_dim == 128 ? 256 : 512; }
 
 // Whether a workgroup takes a whole sequence: in small rooms, where the time is the loads one
-// after another and the launches, and one more launch costs more than tiles in turn; in larger
-// ones where the sequences give workgroups enough by themselves, as shares of short sequences
+// after another and the launches, and one more launch costs more than tiles in turn (bf16, calls
+// of one sequence, in shares -> whole, 32/4 heads of 64: room 256 to 2048 18 -> 13 us, 4096 17.6
+// -> 16.1, 8192 21 -> 28; 32/8 heads of 128: 1024 18 -> 13, 1536 17.3 -> 14.3, 2048 17.5 -> 17.3,
+// 4096 22 -> 29; in fp32 up to 512 places at 64 and 256 at 128 18 -> 13, but 1024 at 64 18 -> 19
+// and at 128 18 -> 34, 2048 at 64 18 -> 34); in larger ones where the sequences give workgroups enough by themselves, as shares of short sequences
 // are several segments in turn and have to be joined.  The larger the room the more a single
 // long sequence among short ones would cost, so there more workgroups are asked for.  bf16,
 // lengths even over [1, room], in shares -> whole, 32/8 heads of 128: 64 sequences of 1280
 // 47 -> 37 us, of 4096 132 -> 118, 128 of 8192 422 -> 399 (one long among short: 41 -> 23,
 // 66 -> 41, 94 -> 87); 32/4 heads of 64: 256 of 8192 212 -> 199, but 128 of 16384 202 -> 225.
-// The fp32 kernel takes a place slower, and loses there: 256 of 8192 355 -> 539.
+// The fp32 kernel takes a place slower: 256 of 8192 would go 355 -> 539.
 bool whole_sequences(fh_dtype dt, int64_t room, int64_t head_dim, int64_t workgroups_of_all) {
   const int64_t small = head_dim == 128 ? 1024 : 2048;
   if (room <= small || dt == FH_F32) return room <= small;

@@ -7,9 +7,11 @@
 // contiguous run of chunks of kChunkElems elements, across tensors; its sum of squares (in
 // fp64: exact products of fp32 values, no overflow below 1e154) is one partial, and every
 // workgroup of the second pass folds the at most kPartials partials by itself, in
-// one order, which is cheaper than a launch in between.  The second pass takes the runs from
-// the last to the first: what the first pass read last is still in the cache.  TinyLlama's
-// 1.1e9 gradients, bf16 to fp32: 376 us for the sums (5.9 TB/s) and 1286 for the outputs
+// one order, which is cheaper than a launch in between.  Within a launch the second pass takes
+// the runs from the last to the first: of up to kTensors tensors, what the first pass read last
+// is still in the cache.  (More tensors are several launches, the same way round in both
+// passes: there the cache holds the end of the last.)  TinyLlama's 1.1e9 gradients, two
+// launches, bf16 to fp32: 376 us for the sums (5.9 TB/s) and 1286 for the outputs
 // (5.1, a third of it read); 5 + 6 us for a few small layers.
 #include <algorithm>
 #include <new>

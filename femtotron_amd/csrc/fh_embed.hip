@@ -308,7 +308,10 @@ __global__ __launch_bounds__(kGroupThreads) void k_embed_group(const int64_t* __
 // ids may all be: fh_embedding_bwd halves them until there are kHotWaves waves.
 // With 64 throughout, uniform ids of a small vocabulary were 32 waves' work at
 // V = 1024, H = 256 (16384 tokens: 91 us, now 17; one wave per row 40) and 64 at
-// V = 64, H = 2048 (4096 tokens: 203 us, now 11; one wave per row 64).
+// V = 64, H = 2048 (4096 tokens: 203 us, now 11; one wave per row 64).  Not more than
+// 64: frequent ids may lie side by side, and 4096 tokens of 256 byte values at V = 128256,
+// H = 2048 take 240 us, with 256 ids a workgroup 638.  (Rows dealt out in turn, up to 64 a
+// wave: 57 -> 52 us for text at V = 32000, H = 2048, but 135 -> 156 for uniform ids at V = 128256.)
 constexpr int kRowChunks = 4;
 constexpr int kHotTokens = 8;
 constexpr int kHotCols = 2 * kWave;  // columns that a wave sums of a hot row

@@ -72,7 +72,10 @@ __device__ __forceinline__ void masked_dq_step(const char* K, const char* V, con
 // Also writes -lse * log2(e) (plus cap_log2: see Score) and delta, put right by the sum of dZ,
 // which the dK/dV kernels read.  142-147 us at 16384 tokens, 32/4 heads of 64, documents of
 // about 600; 1100-1140 at 8192 tokens, 32/8 heads of 128, capped: bound by the vector work of
-// scores and dS and, at 128, by two waves a SIMD that cover each other's waits in part.
+// scores and dS and, at 128, by two waves a SIMD that cover each other's waits in part.  (The
+// scratch of the compiled kernels, 964 to 1540 bytes a lane at 128 and 276 or 616 at 64 under
+// a cap, belongs to the careful pass, at 64 also to the addresses of tiles that end past the
+// last row.)
 template <int HD, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 3 : 2))) void k_masked_dq(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
@@ -293,7 +296,9 @@ __global__ __launch_bounds__(256) void k_masked_dkdv_sum(HeadSplit hs, int split
 // Up to head_dim 64: 8 waves, 128 keys; wave w holds K and V of keys 32 (w % 4) .. +31 in
 // registers and takes queries 32 (w / 4) .. +31 of each 64-query item; the halves' sums
 // meet in LDS at the end, in a fixed order.  Two items a stage, two stages.  190-199 us at
-// 16384 tokens, 32/4 heads of 64, documents of about 600.
+// 16384 tokens, 32/4 heads of 64, documents of about 600: 133 KB of LDS let one workgroup onto
+// a CU, 1.6 waves a SIMD on average, and the matrix units are busy 16% of it, the vector units
+// 25%: it waits.
 template <int HD, int MODE>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k_masked_dkdv_fused(
     const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ k, int64_t ldk,
@@ -432,7 +437,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void k
 // head_dim 128: 4 waves, 64 keys; each 32 keys are shared by a wave that holds K and sums
 // dV (role A: S, P, handed over through LDS) and one that holds V and sums dK (role B).
 // 1400-1520 us at 8192 tokens, 32/8 heads of 128, capped: the matrix units are busy 35% of it
-// and the vector units 46%, the rest are the roles' waits for one another.  (The
+// and the vector units 46%, the rest are the roles' waits for one another.  (344 bytes of
+// scratch a lane, of the careful pass.  The
 // roles of a workgroup's waves swapped in every other one, so that each SIMD has both: 2631
 // -> 2644 us for the backward.)
 template <int HD, int MODE>

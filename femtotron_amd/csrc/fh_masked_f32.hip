@@ -3,7 +3,10 @@
 // a head (16 keys of a kv head) a workgroup, the blocks of 32 keys that they see (the
 // blocks of 32 queries that see them, of each query head) shared out over its waves.
 // tanh is the math library's: v_exp and v_rcp leave 2^-23 of the cap in the scores, ten
-// times what the products leave.
+// times what the products leave.  One causal document, 32/4 heads of 64, forward and backward:
+// 1024 tokens 96 and 425 us (45 and 25 TFLOP/s), 4096 909 and 3860 (76 and 45); 32/8 heads of
+// 128, 4096 tokens, 1762 and 7365 (78 and 47), the causal kernels' times; a large fp32
+// product runs at 153.
 #include <type_traits>
 
 #include "fh_masked.hpp"

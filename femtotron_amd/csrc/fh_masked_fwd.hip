@@ -91,10 +91,11 @@ __device__ __forceinline__ void masked_step(const char* K, const char* V, const 
   l += lsum;
 }
 
-// Four waves a SIMD up to head_dim 64: what the registers (128) then lack is spilled in the
-// careful pass alone.  16384 tokens, 32/4 heads of 64, documents of about 600: 105 us with
-// three waves a SIMD (one workgroup a CU), 83 with four (390 TFLOP/s; the softmax's vector
-// work is of the order of the products' time).  8192 tokens, 32/8 heads of 128, capped: 657 us,
+// Four waves a SIMD up to head_dim 64: what the registers (128) then lack, at 64 with a pair of
+// heads 68 bytes a lane (204 under a cap), is spilled in the careful pass and in the addresses
+// of tiles that end past the last row.  16384 tokens, 32/4 heads of 64, documents of about 600: 105 us with
+// three waves a SIMD (one workgroup a CU), 83 with four (390 TFLOP/s; the matrix units are
+// busy 17% of it and the vector units 45%).  8192 tokens, 32/8 heads of 128, capped: 657 us,
 // 840 TFLOP/s; without the cap 542.
 // HPB = 2: 8 waves take the same rows of two query heads of one kv head, which read the
 // same K and V tiles.
